@@ -82,6 +82,23 @@ std::vector<at::Tensor> cross_entropy_fused(at::Tensor& logits, const at::Tensor
 std::vector<at::Tensor> token_logprob_fwd(const at::Tensor& logits, const at::Tensor& targets, double temperature);
 at::Tensor token_logprob_bwd(const at::Tensor& logits, const at::Tensor& targets, const at::Tensor& lse,
                              const at::Tensor& dlogp, double temperature);
+// token_stats.cu
+std::vector<at::Tensor> token_stats_fwd(const at::Tensor& logits, const c10::optional<at::Tensor>& targets,
+                                        double temperature, int64_t top, int64_t ignore_index, bool save);
+at::Tensor token_stats_bwd(const at::Tensor& logits, const c10::optional<at::Tensor>& targets,
+                           const at::Tensor& top_ids, const at::Tensor& saved, double temperature,
+                           const c10::optional<at::Tensor>& g_log_probs, const c10::optional<at::Tensor>& g_entropy,
+                           const c10::optional<at::Tensor>& g_top);
+// lm_head.cu
+std::vector<at::Tensor> lm_head_stats_fwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
+                                          double temperature, int64_t ignore_index);
+at::Tensor lm_head_stats_bwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
+                             const at::Tensor& saved, double temperature, int64_t ignore_index,
+                             const c10::optional<at::Tensor>& g_log_probs, const c10::optional<at::Tensor>& g_entropy);
+// distill.cu
+std::vector<at::Tensor> distill_fwd(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher,
+                                    const c10::optional<at::Tensor>& weights, double temperature, bool tail, bool grad);
+void distill_scale(at::Tensor& dlogits, const at::Tensor& factor);
 // optim.cu
 void adamw_step(at::Tensor& master, const at::Tensor& grad, at::Tensor& m, at::Tensor& v,
                 const c10::optional<at::Tensor>& out, double lr, double beta1, double beta2, double eps,
@@ -205,6 +222,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cross_entropy_fused", &tdsv::cross_entropy_fused);
   m.def("token_logprob_fwd", &tdsv::token_logprob_fwd);
   m.def("token_logprob_bwd", &tdsv::token_logprob_bwd);
+  m.def("token_stats_fwd", &tdsv::token_stats_fwd, "log-probability, entropy and top alternatives of rows of logits");
+  m.def("token_stats_bwd", &tdsv::token_stats_bwd);
+  m.def("lm_head_stats_fwd", &tdsv::lm_head_stats_fwd, "token statistics fused with the LM head's product");
+  m.def("lm_head_stats_bwd", &tdsv::lm_head_stats_bwd);
+  m.def("distill_fwd", &tdsv::distill_fwd, "KL from a teacher's top alternatives, with its gradient");
+  m.def("distill_scale", &tdsv::distill_scale);
   m.def("adamw_step", &tdsv::adamw_step, py::arg("master"), py::arg("grad"), py::arg("m"), py::arg("v"),
         py::arg("out"), py::arg("lr"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"),
         py::arg("step"), py::arg("grad_scale"), py::arg("grad_scale_t"), py::arg("step_t") = py::none(),

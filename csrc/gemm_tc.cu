@@ -373,10 +373,20 @@ void bind_primary_context() {
 
 namespace {
 
+// A contiguous tensor, or a matrix whose rows are padded (a vocabulary that is no multiple of 8 columns).
+void check_operand(const at::Tensor& t, const char* name) {
+  if (t.dim() != 2 || t.is_contiguous()) return check_cuda_tensor(t, name);
+  TDSV_CHECK(t.is_cuda() && t.has_storage() && t.numel() > 0, name, " must be a CUDA tensor with device storage");
+  TDSV_CHECK(t.stride(1) == 1 && t.stride(0) >= t.size(1), name, " must have contiguous rows");
+  TDSV_CHECK(static_cast<int64_t>(t.storage().nbytes()) >=
+                 (t.storage_offset() + (t.size(0) - 1) * t.stride(0) + t.size(1)) * static_cast<int64_t>(t.element_size()),
+             name, " is larger than its storage");
+}
+
 // Row-major tensor [outer..., rows, inner] with a box of {box_inner, box_rows, 1...}, 128B swizzle.
 CUtensorMap make_map(const at::Tensor& t, int box_rows, int box_inner = 64) {
   bind_primary_context();
-  check_cuda_tensor(t, "gemm operand");
+  check_operand(t, "gemm operand");
   const bool bf16 = t.scalar_type() == at::kBFloat16;
   TDSV_CHECK(bf16 || t.scalar_type() == at::kFloat, "gemm tensors must be bf16 (operands) or fp32 (outputs)");
   const int esize = bf16 ? 2 : 4;
@@ -389,8 +399,12 @@ CUtensorMap make_map(const at::Tensor& t, int box_rows, int box_inner = 64) {
   cuuint32_t estr[3] = {1, 1, 1};
   dims[0] = static_cast<cuuint64_t>(t.size(rank - 1));
   dims[1] = static_cast<cuuint64_t>(t.size(rank - 2));
-  TDSV_CHECK((dims[0] * esize) % 16 == 0, "gemm inner dimension must be a multiple of 16 bytes");
-  strides[0] = dims[0] * esize;
+  // (the stride of a single row is never used; it only has to be a legal one)
+  const int64_t row_stride = rank == 2 && t.size(0) == 1 ? (t.size(1) * esize + 15) / 16 * 16 / esize
+                             : t.is_contiguous()         ? t.size(rank - 1)
+                                                         : t.stride(0);
+  TDSV_CHECK((row_stride * esize) % 16 == 0, "gemm rows must be a multiple of 16 bytes apart");
+  strides[0] = static_cast<cuuint64_t>(row_stride) * esize;
   if (rank == 3) {
     dims[2] = static_cast<cuuint64_t>(t.size(0));
     strides[1] = dims[0] * dims[1] * esize;
@@ -473,9 +487,9 @@ int epi_code(const at::Tensor& out, bool accumulate) {
 }  // namespace
 
 // out[M, N] (+)= A * B^T with A [M, K] (a_mn=false) or [K, M] (a_mn=true) and
-// B [N, K] (b_mn=false) or [K, N] (b_mn=true).
+// B [N, K] (b_mn=false) or [K, N] (b_mn=true). The rows of A may be padded.
 void gemm(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, bool a_mn, bool b_mn, bool accumulate) {
-  check_cuda_tensor(a, "a");
+  check_operand(a, "a");
   check_cuda_tensor(b, "b");
   check_cuda_tensor(out, "out");
   TDSV_CHECK(a.dim() == 2 && b.dim() == 2 && out.dim() == 2, "gemm: 2-D operands");

@@ -13,9 +13,10 @@ from .quant import fake_quant, quantize_activation
 from . import rope
 from .rope import inv_freq, qk_norm_rope, rope_interleaved
 from .router import AuxGradient, route
+from .statistics import DistillationLoss, TokenStatistics, distillation_loss, linear_token_statistics, token_statistics
 
 __all__ = [
-    "AuxGradient", "DeviceStatusError", "Routing", "StatusMonitor", "available", "build_routing", "causal_attention", "check_status", "combine",
-    "dequantize_fp4", "ext", "fake_quant", "fp4_grouped_linear", "gather", "grouped_linear", "inv_freq", "linear", "linear_cross_entropy", "matmul_nt", "on_gpu", "peer_wait_limit",
-    "qk_norm_rope", "quantize_activation", "rms_norm", "rope_interleaved", "route", "set_peer_wait_limit", "swiglu", "token_log_probs",
+    "AuxGradient", "DeviceStatusError", "DistillationLoss", "Routing", "StatusMonitor", "TokenStatistics", "available", "build_routing", "causal_attention", "check_status", "combine",
+    "dequantize_fp4", "distillation_loss", "ext", "fake_quant", "fp4_grouped_linear", "gather", "grouped_linear", "inv_freq", "linear", "linear_cross_entropy", "linear_token_statistics", "matmul_nt", "on_gpu", "peer_wait_limit",
+    "qk_norm_rope", "quantize_activation", "rms_norm", "rope_interleaved", "route", "set_peer_wait_limit", "swiglu", "token_log_probs", "token_statistics",
 ]
