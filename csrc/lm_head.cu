@@ -4,8 +4,8 @@
 //
 //   statistics  each 128 x BN tile of X is reduced, row by row, to (m, S, W) of logit_rows.cuh; the column
 //               of the row's target is kept. A second kernel joins the tiles of a row in a fixed order.
-//   gradient    the tile is recomputed and leaves as  dX = p (a + b log2 p) + d_it g / T  in bf16, with p
-//               from the fp32 accumulators and the saved row statistics (logits rounded to bf16 first
+//   gradient    the tile is recomputed and leaves as  dX = 2^y (a + b y) + d_it g / T  in bf16, with y
+//               from the fp32 accumulators and a, b from the saved row statistics (logits rounded to bf16 first
 //               would put an error of 2^-9 |x| into ln p). dX feeds the plain GEMMs of dhidden and dweight.
 //
 // Roles inside a CTA (192 threads, one CTA per SM): warp 0 feeds a ring of 128B-swizzled stages by TMA,
@@ -38,7 +38,7 @@ struct HeadParams {
   float *part_m, *part_s, *part_w;  // [column tiles, M]
   float* target_logit;              // [M]
   // gradient
-  const float4* saved;  // [M]: m, log2 S, H
+  const float4* saved;  // [M]: m, 1 / S, W / S
   const float *g, *h;   // [M] or null
   int64_t ignore_index;
   int* status;
@@ -154,15 +154,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the target's column inside this tile, or a column no chunk has
       const int64_t rel = target - t.n0;
       const int hit = rel >= 0 && rel < BN && target < p.N ? static_cast<int>(rel) : -1;
-      float4 sv = make_float4(0.f, INFINITY, 0.f, 0.f);
-      float a = 0.f, b = 0.f, bonus = 0.f;
+      // dx = 2^y (a + b y) with 1 / (S T) inside a and b; a row without a gradient has y = -inf throughout
+      float m = INFINITY, a = 0.f, b = 0.f, bonus = 0.f;
       if (GRAD && live && target != p.ignore_index) {
-        sv = p.saved[row];
-        if (sv.y != INFINITY) {
+        const float4 sv = p.saved[row];
+        if (sv.y != 0.f) {
           const float g = p.g != nullptr && target >= 0 && target < p.N ? p.g[row] : 0.f;
-          const float h = p.h != nullptr ? p.h[row] : 0.f;
-          a = -p.inv_t * (g + h * sv.z);
-          b = -p.inv_t * h * kLn2;
+          const float h = p.h != nullptr ? p.h[row] * kLn2 : 0.f;
+          const float scale = p.inv_t * sv.y;
+          m = sv.x;
+          a = -scale * (g - h * sv.z);
+          b = -scale * h;
           bonus = p.inv_t * g;
         }
       }
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float d[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const float y = fmaxf((__uint_as_float(raw[q * 8 + i]) - sv.x) * p.c2 - sv.y, kMinExponent);
+              const float y = fmaxf((__uint_as_float(raw[q * 8 + i]) - m) * p.c2, kMinExponent);
               d[i] = exp2_fast(y) * (a + b * y) + (q * 8 + i == at ? bonus : 0.f);
             }
             uint4 v;
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(32 * kJoinSlices)
   }
   log_probs[r] = lp;
   entropy[r] = ent;
-  saved[r] = make_float4(st.s == 0.f ? 0.f : st.m, st.s == 0.f ? INFINITY : log2f(st.s), ent, 0.f);
+  saved[r] = saved_stats(st);
 }
 
 CUtensorMap head_map(const at::Tensor& t, int64_t row_stride, int box_rows) {

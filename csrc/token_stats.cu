@@ -7,10 +7,15 @@
 // and the gradient of all three. With upstream g (log-probability), h (entropy), u_j (alternatives):
 //   dx_i = [ g (d_it - p_i) + sum_j u_j (d_ij - p_i) - h p_i (ln p_i + H) ] / T
 //
+// where ln p_i + H = ln 2 (y_i - W / S) in the terms of logit_rows.cuh: the logarithm of S drops out, so the
+// entropy's gradient stays exact where one token has nearly all of the mass.
+//
 // A row whose target is the ignore index is not read: zeros, ids -1, zero gradient. Masked logits
 // (-inf) have p = 0 and are never alternatives (id -1, ln p = -inf). A row that is masked throughout
 // has ln p = -inf, H = 0 and no gradient. NaN or +inf in a row that is read gives NaN.
 #include "logit_rows.cuh"
+
+#include <cooperative_groups.h>
 
 namespace tdsv {
 
@@ -18,132 +23,451 @@ namespace {
 
 constexpr int kStatThreads = 256;
 constexpr int kMaxTop = 128;
+constexpr int kUnroll = 4;          // vectors a thread has in flight
+constexpr int kBatch = kStatThreads * kUnroll;
+constexpr int kCandidates = 2048;   // candidates for the alternatives that a block can hold
+constexpr int kMaxCluster = 8;
 
-// Saved for the backward: m, log2 S, H and a spare per row; S = 0 is stored as log2 S = +inf.
-__device__ __forceinline__ float4 saved_stats(const RowStats& st, float entropy) {
-  return make_float4(st.s == 0.f ? 0.f : st.m, st.s == 0.f ? INFINITY : log2f(st.s), entropy, 0.f);
+// Floats as whole numbers of the same order (both zeros are one value), and back.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+constexpr uint32_t kMaskedKey = 0x007fffffu;  // of -inf: every finite value's key is larger
+// A candidate: the larger value first, then the lower index.
+__device__ __forceinline__ uint64_t candidate(uint32_t key, int i) {
+  return static_cast<uint64_t>(key) << 32 | (0xffffffffu - static_cast<uint32_t>(i));
+}
+__device__ __forceinline__ uint32_t candidate_key(uint64_t c) { return static_cast<uint32_t>(c >> 32); }
+
+// The largest threshold found in [lo, hi) at which at least `want` keys are counted, given that this holds
+// at lo and not at hi: halving steps, until at most `want + slack` are left or nothing lies between.
+// `count(t)` is this thread's number of keys >= t; every thread of the block calls it.
+template <typename F>
+__device__ __forceinline__ uint32_t raise_threshold(uint32_t lo, uint32_t hi, int want, int slack, F&& count,
+                                                    int* scratch, int& kept) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int parity = 0;
+  kept = 0x7fffffff;
+  while (hi - lo > 1) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    const int mine = __reduce_add_sync(0xffffffffu, count(mid));
+    int* slot = scratch + 8 * parity;
+    if (lane == 0) slot[warp] = mine;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < kStatThreads / 32; ++w) all += slot[w];
+    parity ^= 1;  // (the next round writes the other half, so one barrier a round is enough)
+    if (all >= want) {
+      lo = mid;
+      kept = all;
+      if (all <= want + slack) break;
+    } else {
+      hi = mid;
+    }
+  }
+  return lo;
 }
 
-// The larger logit first, then the lower index.
-__device__ __forceinline__ bool before(float a, int ia, float b, int ib) { return a > b || (a == b && ia < ib); }
+// Block-wide maximum of a key.
+__device__ __forceinline__ uint32_t block_key_max(uint32_t k, uint32_t* scratch) {
+  k = __reduce_max_sync(0xffffffffu, k);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = k;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kStatThreads / 32; ++w) k = max(k, scratch[w]);
+  return k;
+}
 
+struct TopScratch {
+  uint64_t kept[kStatThreads];  // candidates at or above the final threshold
+  uint32_t maxima[8];
+  int counts[16];
+  int n, survivors;
+};
+
+// Exactly the first `want` of the n candidates in `buf` (fewer where there are fewer), each handed to
+// emit(rank, candidate) once. Keys are halved down to the want-th largest; what is left is ranked by
+// counting, which also settles equal keys by index.
+template <typename F>
+__device__ __forceinline__ void select_top(const uint64_t* buf, int n, int want, TopScratch& sc, F&& emit) {
+  uint32_t top_key = 0;
+  for (int i = threadIdx.x; i < n; i += kStatThreads) top_key = max(top_key, candidate_key(buf[i]));
+  top_key = block_key_max(top_key, sc.maxima);
+  uint32_t cut = 1;  // (key 0 fills places without a candidate)
+  if (n > want) {
+    int kept;
+    auto count = [&](uint32_t t) {
+      int c = 0;
+      for (int i = threadIdx.x; i < n; i += kStatThreads) c += candidate_key(buf[i]) >= t;
+      return c;
+    };
+    cut = raise_threshold(0, top_key + 1, want, 0, count, sc.counts, kept);
+    cut = max(cut, 1u);
+  }
+  if (threadIdx.x == 0) sc.survivors = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kStatThreads) {
+    if (candidate_key(buf[i]) < cut) continue;
+    const int at = atomicAdd(&sc.survivors, 1);
+    if (at < kStatThreads) sc.kept[at] = buf[i];
+  }
+  __syncthreads();
+  // many equal keys at the threshold do not fit: rank against all candidates then
+  const bool fits = sc.survivors <= kStatThreads;
+  const uint64_t* from = fits ? sc.kept : buf;
+  const int m = fits ? sc.survivors : n;
+  for (int i = threadIdx.x; i < m; i += kStatThreads) {
+    const uint64_t c = from[i];
+    if (candidate_key(c) < cut) continue;
+    int rank = 0;
+    for (int j = 0; j < m; ++j) rank += from[j] > c;
+    if (rank < want) emit(rank, c);
+  }
+}
+
+// The exact way for a block's part of a row whose candidates do not fit (rows in rising order, thousands of
+// equal values): halve the value, then the index among equals, re-reading the part each time, until what is
+// left fits. Returns the number of candidates put into `buf`.
 template <typename T>
-__global__ void __launch_bounds__(kStatThreads)
+__device__ __noinline__ int collect_again(const T* row, int first, int last, int want, uint64_t* buf, TopScratch& sc) {
+  auto count_keys = [&](uint32_t t) {
+    int c = 0;
+    for (int i = first + threadIdx.x; i < last; i += kStatThreads) c += order_key(to_float<T>(row[i])) >= t;
+    return c;
+  };
+  int kept;
+  // (+inf is the largest key that counts; NaN lies above it)
+  uint32_t cut = raise_threshold(kMaskedKey, 0xff800001u, want, kCandidates - want, count_keys, sc.counts, kept);
+  __syncthreads();
+  uint32_t none_after = 0xffffffffu;  // of the elements equal to `cut`, those up to this index
+  if (cut == kMaskedKey) cut = kMaskedKey + 1;  // fewer than `want` are unmasked
+  else if (kept > kCandidates) {
+    const int above = __reduce_add_sync(0xffffffffu, count_keys(cut + 1));
+    if ((threadIdx.x & 31) == 0) sc.counts[threadIdx.x >> 5] = above;
+    __syncthreads();
+    int more = 0;
+    for (int w = 0; w < kStatThreads / 32; ++w) more += sc.counts[w];
+    __syncthreads();
+    // indices count downwards so that "at least" still means a threshold from below
+    auto count_equal = [&](uint32_t t) {
+      int c = 0;
+      for (int i = first + threadIdx.x; i < last; i += kStatThreads)
+        c += order_key(to_float<T>(row[i])) == cut && static_cast<uint32_t>(last - i) >= t;
+      return c;
+    };
+    const uint32_t t = raise_threshold(0, static_cast<uint32_t>(last - first) + 1, want - more, 0, count_equal, sc.counts, kept);
+    none_after = static_cast<uint32_t>(last) - max(t, 1u);
+  }
+  if (threadIdx.x == 0) sc.n = 0;
+  __syncthreads();
+  for (int i = first + threadIdx.x; i < last; i += kStatThreads) {
+    const uint32_t key = order_key(to_float<T>(row[i]));
+    if (key > cut || (key == cut && static_cast<uint32_t>(i) <= none_after)) {
+      if (key > 0xff800000u) continue;
+      const int at = atomicAdd(&sc.n, 1);
+      if (at < kCandidates) buf[at] = candidate(key, i);
+    }
+  }
+  __syncthreads();
+  return min(sc.n, kCandidates);
+}
+
+// A block (or a cluster of blocks, each on a stretch of the row) reads a row once in 16-byte vectors.
+//
+// Alternatives: a value is a candidate when it reaches a threshold that at least `top` values of the row
+// reach. The first threshold comes from the threads' own maxima of the first batch; it is raised after 1,
+// 2, 4, ... batches from the candidates so far, so that a row of V values gives some top * log2(V / 8192)
+// candidates, and the common step costs one comparison for a thread's whole batch.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kStatThreads, 4)
     stats_fwd_kernel(const T* __restrict__ logits, RowLayout layout, int v, const int64_t* __restrict__ targets,
                      int64_t ignore_index, float c2, int top, float* __restrict__ log_probs,
                      float* __restrict__ entropy, int64_t* __restrict__ top_ids, float* __restrict__ top_lp,
                      float4* __restrict__ saved, int* status) {
+  namespace cg = cooperative_groups;
+  constexpr int kSize = LogitVec<T>::kSize;
+  extern __shared__ uint64_t top_smem[];  // [kCandidates], then [blocks of the cluster][top]
   __shared__ RowStats scratch[33];
-  __shared__ float best_v[32];
-  __shared__ int best_i[32];
-  const int64_t r = blockIdx.x;
-  const T* row = logits + layout.offset(r);
+  __shared__ RowStats parts[kMaxCluster];
+  __shared__ TopScratch sc;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x / blocks;
   const int64_t target = targets != nullptr ? targets[r] : 0;
-  if (targets != nullptr && target == ignore_index) {
-    if (threadIdx.x == 0) {
+  if (targets != nullptr && target == ignore_index) {  // (the whole cluster leaves)
+    if (part != 0) return;
+    if (tid == 0) {
       log_probs[r] = 0.f;
       entropy[r] = 0.f;
-      if (saved != nullptr) saved[r] = make_float4(0.f, INFINITY, 0.f, 0.f);
+      if (saved != nullptr) saved[r] = saved_stats(RowStats());
     }
-    for (int j = threadIdx.x; j < top; j += blockDim.x) {
+    for (int j = tid; j < top; j += kStatThreads) {
       top_ids[r * top + j] = -1;
       top_lp[r * top + j] = -INFINITY;
     }
     return;
   }
-  RowStats st;
-  for (int i = threadIdx.x; i < v; i += blockDim.x) st.add(to_float<T>(row[i]), c2);
-  st = block_merge(st, c2, scratch);
-  const float log2s = log2f(st.s);
-  if (threadIdx.x == 0) {
-    const float ent = st.s == 0.f ? 0.f : kLn2 * (log2s - st.w / st.s);
+  // every block of the cluster runs before another writes to its shared memory (waited for below)
+  if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const T* row = logits + layout.offset(r);
+  const RowCut cut = cut_row(row, v);
+  const int per = (cut.vecs + blocks - 1) / blocks;
+  const int v0 = min(cut.vecs, part * per), v1 = min(cut.vecs, v0 + per);
+  const uint4* base = reinterpret_cast<const uint4*>(row + cut.head);
+
+  // the values before the first vector and after the last: one per thread, of two warps
+  float single = -INFINITY;
+  int single_at = 0;
+  if (part == 0 && tid < cut.head) single_at = tid, single = to_float<T>(row[tid]);
+  if (part == blocks - 1 && tid >= 32 && tid < 32 + cut.tail)
+    single_at = v - cut.tail + tid - 32, single = to_float<T>(row[single_at]);
+  VecStats st;
+  if (single != -INFINITY) st.add_one(single, c2);
+
+  uint4 next[kUnroll];
+  auto load = [&](int from) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = from + u * kStatThreads + tid;
+      if (i < v1) next[u] = load_stream(base + i);
+    }
+  };
+  uint32_t threshold = kMaskedKey + 1;
+  float threshold_value = -INFINITY;
+  auto push = [&](float x, int i) {
+    const uint32_t key = order_key(x);
+    if (key < threshold || key > 0xff800000u) return;
+    const int at = atomicAdd(&sc.n, 1);
+    if (at < kCandidates) top_smem[at] = candidate(key, i);
+  };
+  if (TOP && tid == 0) sc.n = 0;
+  load(v0);
+  int batch = 0;
+  for (int from = v0; from < v1; from += kBatch, ++batch) {
+    uint4 now[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) now[u] = next[u];
+    // vectors past the end repeat the thread's first one for the maximum and are skipped in the sums
+    const int mine = (v1 - from - tid + kStatThreads - 1) / kStatThreads;  // valid ones of this thread
+    float mx = -INFINITY;
+    if (mine >= kUnroll) {
+      mx = vec_max<T, kUnroll>(now);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (u < mine) {
+          const uint4 one[1] = {now[u]};
+          mx = fmaxf(mx, vec_max<T, 1>(one));
+        }
+    }
+    if (from + kBatch < v1) load(from + kBatch);
+    if (mx > st.limit) st.raise(mx, c2);
+    if (mine >= kUnroll) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) st.add_vec<T>(now[u], c2);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (u < mine) st.add_vec<T>(now[u], c2);
+    }
+    if constexpr (TOP) {
+      if (batch == 0) {
+        const uint32_t own = max(order_key(mx), order_key(single));
+        const uint32_t hi = block_key_max(own, sc.maxima);
+        if (hi > kMaskedKey && hi <= 0xff800000u) {
+          int kept;
+          threshold = raise_threshold(kMaskedKey, hi + 1, top, top / 4, [&](uint32_t t) { return own >= t ? 1 : 0; },
+                                      sc.counts, kept);
+          threshold = max(threshold, kMaskedKey + 1);
+        }
+        threshold_value = key_value(threshold);
+        __syncthreads();
+      }
+      if (mx >= threshold_value) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          if (u >= mine) break;
+          const uint4 one[1] = {now[u]};
+          if (vec_max<T, 1>(one) < threshold_value) continue;
+          const int i0 = cut.head + (from + u * kStatThreads + tid) * kSize;
+#pragma unroll
+          for (int i = 0; i < LogitVec<T>::kPairs; ++i) {
+            const float2 x = unpack_pair<T>(now[u], i);
+            if (x.x >= threshold_value) push(x.x, i0 + 2 * i);
+            if (x.y >= threshold_value) push(x.y, i0 + 2 * i + 1);
+          }
+        }
+      }
+      if (((batch + 1) & batch) == 0 && from + kBatch < v1) {
+        __syncthreads();
+        const int n = min(sc.n, kCandidates);
+        if (n > top) {
+          uint32_t hi = 0;
+          for (int i = tid; i < n; i += kStatThreads) hi = max(hi, candidate_key(top_smem[i]));
+          hi = block_key_max(hi, sc.maxima);
+          int kept;
+          auto count = [&](uint32_t t) {
+            int c = 0;
+            for (int i = tid; i < n; i += kStatThreads) c += candidate_key(top_smem[i]) >= t;
+            return c;
+          };
+          threshold = raise_threshold(threshold, hi + 1, top, top / 4, count, sc.counts, kept);
+          threshold_value = key_value(threshold);
+        }
+        __syncthreads();
+      }
+    }
+  }
+  RowStats all = block_merge(st.total(), c2, scratch);
+  if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if constexpr (TOP) {
+    if (single > -INFINITY && single >= threshold_value) push(single, single_at);
+    __syncthreads();
+    int n = sc.n;
+    __syncthreads();
+    if (n > kCandidates) {
+      const int first = part == 0 ? 0 : cut.head + v0 * kSize;
+      const int last = part == blocks - 1 ? v : cut.head + v1 * kSize;
+      n = collect_again(row, first, last, top, top_smem, sc);
+    }
+    if (blocks > 1) {
+      // this block's first `top`, at its place in the leader's shared memory
+      uint64_t* lead = cluster.map_shared_rank(top_smem, 0) + kCandidates + part * top;
+      for (int j = min(n, top) + tid; j < top; j += kStatThreads) lead[j] = 0;
+      select_top(top_smem, n, top, sc, [&](int rank, uint64_t c) { lead[rank] = c; });
+    } else {
+      const float log2s = log2f(all.s);
+      for (int j = min(n, top) + tid; j < top; j += kStatThreads) {
+        top_ids[r * top + j] = -1;
+        top_lp[r * top + j] = -INFINITY;
+      }
+      select_top(top_smem, n, top, sc, [&](int rank, uint64_t c) {
+        top_ids[r * top + rank] = 0xffffffffu - static_cast<uint32_t>(c);
+        top_lp[r * top + rank] = kLn2 * ((key_value(candidate_key(c)) - all.m) * c2 - log2s);
+      });
+    }
+  }
+  if (blocks > 1) {
+    if (tid == 0) *cluster.map_shared_rank(&parts[part], 0) = all;
+    cluster.sync();
+    if (part != 0) return;
+    all = parts[0];
+    for (int b = 1; b < blocks; ++b) all.merge(parts[b], c2);
+    if constexpr (TOP) {
+      const float log2s = log2f(all.s);
+      const uint64_t* gathered = top_smem + kCandidates;
+      int there = 0;
+      for (int j = tid; j < blocks * top; j += kStatThreads) there += gathered[j] != 0;
+      there = __reduce_add_sync(0xffffffffu, there);
+      if ((tid & 31) == 0) sc.counts[tid >> 5] = there;
+      __syncthreads();
+      int n = 0;
+      for (int w = 0; w < kStatThreads / 32; ++w) n += sc.counts[w];
+      __syncthreads();
+      for (int j = min(n, top) + tid; j < top; j += kStatThreads) {
+        top_ids[r * top + j] = -1;
+        top_lp[r * top + j] = -INFINITY;
+      }
+      select_top(gathered, blocks * top, top, sc, [&](int rank, uint64_t c) {
+        top_ids[r * top + rank] = 0xffffffffu - static_cast<uint32_t>(c);
+        top_lp[r * top + rank] = kLn2 * ((key_value(candidate_key(c)) - all.m) * c2 - log2s);
+      });
+    }
+  }
+  if (tid == 0) {
+    const float log2s = log2f(all.s);
+    const float ent = all.s == 0.f ? 0.f : kLn2 * (log2s - all.w / all.s);
     entropy[r] = ent;
     if (targets != nullptr) {
       float lp = NAN;
       if (target >= 0 && target < v) {
-        lp = st.s == 0.f ? -INFINITY : kLn2 * ((to_float<T>(row[target]) - st.m) * c2 - log2s);
+        lp = all.s == 0.f ? -INFINITY : kLn2 * ((to_float<T>(row[target]) - all.m) * c2 - log2s);
       } else {
         report_status(status, kOutOfBounds);
       }
       log_probs[r] = lp;
     }
-    if (saved != nullptr) saved[r] = saved_stats(st, ent);
-  }
-  float last = INFINITY;
-  int last_i = -1;
-  for (int j = 0; j < top; ++j) {
-    float b = -INFINITY;
-    int bi = 0x7fffffff;
-    for (int i = threadIdx.x; i < v; i += blockDim.x) {
-      const float x = to_float<T>(row[i]);
-      if (before(last, last_i, x, i) && before(x, i, b, bi)) b = x, bi = i;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float ob = __shfl_xor_sync(0xffffffffu, b, o);
-      const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-      if (before(ob, oi, b, bi)) b = ob, bi = oi;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) best_v[threadIdx.x >> 5] = b, best_i[threadIdx.x >> 5] = bi;
-    __syncthreads();
-    b = best_v[0], bi = best_i[0];
-    for (int w = 1; w < kStatThreads / 32; ++w)
-      if (before(best_v[w], best_i[w], b, bi)) b = best_v[w], bi = best_i[w];
-    if (threadIdx.x == 0) {
-      const bool none = b == -INFINITY;
-      top_ids[r * top + j] = none ? -1 : bi;
-      top_lp[r * top + j] = none ? -INFINITY : kLn2 * ((b - st.m) * c2 - log2s);
-    }
-    last = b, last_i = bi;
+    if (saved != nullptr) saved[r] = saved_stats(all);
   }
 }
 
+// A block writes the gradient of one stretch of a row (kStretch values of 2 bytes: enough to hide the
+// start, small enough that the last wave of blocks is short).
+constexpr int kStretchBytes = 32768;
+
 template <typename T>
 __global__ void __launch_bounds__(kStatThreads)
-    stats_bwd_kernel(const T* __restrict__ logits, RowLayout layout, int v, const int64_t* __restrict__ targets,
-                     float c2, float inv_t, int top, const int64_t* __restrict__ top_ids,
-                     const float4* __restrict__ saved, const float* __restrict__ g_lp, const float* __restrict__ g_ent,
-                     const float* __restrict__ g_top, T* __restrict__ dlogits) {
-  __shared__ int64_t at[kMaxTop + 1];
+    stats_bwd_kernel(const T* __restrict__ logits, RowLayout layout, int v, int parts,
+                     const int64_t* __restrict__ targets, float c2, float inv_t, int top,
+                     const int64_t* __restrict__ top_ids, const float4* __restrict__ saved,
+                     const float* __restrict__ g_lp, const float* __restrict__ g_ent, const float* __restrict__ g_top,
+                     T* __restrict__ dlogits) {
+  __shared__ int at[kMaxTop + 1];
   __shared__ float grad[kMaxTop + 1];
   __shared__ float scratch[32];
-  const int64_t r = blockIdx.x;
+  constexpr int kStretch = kStretchBytes / static_cast<int>(sizeof(T));
+  const int64_t r = blockIdx.x / parts;
+  const int first = static_cast<int>(blockIdx.x % parts) * kStretch, n = min(kStretch, v - first);
   const T* row = logits + layout.offset(r);
   T* out = dlogits + r * v;
   const float4 s = saved[r];
-  if (s.y == INFINITY) {  // ignored, or nothing unmasked
-    for (int i = threadIdx.x; i < v; i += blockDim.x) out[i] = from_float<T>(0.f);
+  if (s.y == 0.f) {  // ignored, or nothing unmasked
+    write_zeros<T, kStatThreads>(out + first, n);
     return;
   }
   // places that are not only -p_i (...): the target and the alternatives
-  const int places = g_top != nullptr ? top + 1 : 1;
-  float mine = 0.f;
-  for (int j = threadIdx.x; j < places; j += blockDim.x) {
-    const int64_t id = j < places - 1 ? top_ids[r * top + j] : (targets != nullptr ? targets[r] : -1);
-    const bool there = id >= 0 && id < v;
-    float u = 0.f;
-    if (there) u = j < places - 1 ? g_top[r * top + j] : (g_lp != nullptr ? g_lp[r] : 0.f);
-    at[j] = there ? id : -1;
-    grad[j] = u;
-    mine += u;
+  const int64_t target = targets != nullptr ? targets[r] : -1;
+  const bool has_target = g_lp != nullptr && target >= 0 && target < v;
+  float g = has_target ? g_lp[r] : 0.f;
+  if (g_top != nullptr) {
+    float mine = 0.f;
+    for (int j = threadIdx.x; j <= top; j += kStatThreads) {
+      const int64_t id = j < top ? top_ids[r * top + j] : (has_target ? target : -1);
+      const bool there = id >= 0 && id < v;
+      const float u = !there ? 0.f : j < top ? g_top[r * top + j] : g;
+      at[j] = there ? static_cast<int>(id) : -1;
+      grad[j] = u;
+      mine += u;
+    }
+    g = block_sum(mine, scratch);
   }
-  const float g = block_sum(mine, scratch);
-  const float h = g_ent != nullptr ? g_ent[r] : 0.f;
-  // T dx_i = p_i (a + b log2 p_i) + (d_i terms)
-  const float a = -(g + h * s.z), b = -h * kLn2;
-  for (int i = threadIdx.x; i < v; i += blockDim.x) {
-    const float y = fmaxf((to_float<T>(row[i]) - s.x) * c2 - s.y, kMinExponent);
-    out[i] = from_float<T>(inv_t * (exp2_fast(y) * (a + b * y)));
-  }
+  const float h = g_ent != nullptr ? g_ent[r] * kLn2 : 0.f;
+  // T dx_i = 2^y_i (a + b y_i) / S + (d_i terms),  y_i = (x_i - m) c2
+  const float a = -(g - h * s.z), b = -h;
+  const float scale = inv_t * s.y;
+  write_gradient<T, kStatThreads>(row + first, out + first, n, s.x, c2, scale * a, scale * b);
   __syncthreads();
-  for (int j = threadIdx.x; j < places; j += blockDim.x) {
-    if (at[j] < 0) continue;
-    float u = 0.f;  // equal places write the same sum
-    for (int k = 0; k < places; ++k) u += at[k] == at[j] ? grad[k] : 0.f;
-    const float y = fmaxf((to_float<T>(row[at[j]]) - s.x) * c2 - s.y, kMinExponent);
-    out[at[j]] = from_float<T>(inv_t * (u + exp2_fast(y) * (a + b * y)));  // (u and a cancel where p = 1)
+  // (u and a cancel where p = 1: they are added before anything is scaled)
+  auto special = [&](int i, float u) {
+    const float y = fmaxf((to_float<T>(row[i]) - s.x) * c2, kMinExponent);
+    out[i] = from_float<T>(inv_t * (u + s.y * exp2_fast(y) * (a + b * y)));
+  };
+  if (g_top == nullptr) {
+    if (threadIdx.x == 0 && has_target && target >= first && target < first + n) special(static_cast<int>(target), g);
+    return;
   }
+  for (int j = threadIdx.x; j <= top; j += kStatThreads) {
+    if (at[j] < first || at[j] >= first + n) continue;
+    float u = 0.f;  // equal places write the same sum
+    for (int k = 0; k <= top; ++k) u += at[k] == at[j] ? grad[k] : 0.f;
+    special(at[j], u);
+  }
+}
+
+// A row is split over a cluster while there are too few rows for every SM to hold four blocks, and while
+// each part is still several batches of loads.
+int blocks_per_row(int64_t rows, int64_t vocab, int64_t item) {
+  int blocks = 1;
+  while (blocks < kMaxCluster && rows * blocks * 2 <= 4 * num_sms() && vocab * item / (blocks * 2) >= kStatThreads * 16)
+    blocks *= 2;
+  return blocks;
 }
 
 }  // namespace
@@ -176,14 +500,30 @@ std::vector<at::Tensor> token_stats_fwd(const at::Tensor& logits_in, const c10::
   auto saved = at::empty({save ? rows : 0, 4}, f32);
   if (rows == 0) return {log_probs, entropy, top_ids, top_lp, saved};
   const float c2 = static_cast<float>(1.4426950408889634 / temperature);
+  const int blocks = blocks_per_row(rows, vocab, logits.element_size());
   with_logit_type(logits.scalar_type(), [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    stats_fwd_kernel<T><<<static_cast<unsigned>(rows), kStatThreads, 0, stream()>>>(
-        static_cast<const T*>(logits.data_ptr()), layout, static_cast<int>(vocab),
-        has_target ? targets->data_ptr<int64_t>() : nullptr, ignore_index, c2, static_cast<int>(top),
-        has_target ? log_probs.data_ptr<float>() : nullptr, entropy.data_ptr<float>(),
-        top ? top_ids.data_ptr<int64_t>() : nullptr, top ? top_lp.data_ptr<float>() : nullptr,
-        save ? reinterpret_cast<float4*>(saved.data_ptr<float>()) : nullptr, status_word_ptr());
+    auto launch = [&](auto kern, size_t smem) {
+      cudaLaunchConfig_t config{};
+      config.gridDim = dim3(static_cast<unsigned>(rows * blocks));
+      config.blockDim = dim3(kStatThreads);
+      config.dynamicSmemBytes = smem;
+      config.stream = stream();
+      cudaLaunchAttribute attr{};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = static_cast<unsigned>(blocks);
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      config.attrs = &attr;
+      config.numAttrs = 1;
+      TDSV_CUDA_CHECK(cudaLaunchKernelEx(
+          &config, kern, static_cast<const T*>(logits.data_ptr()), layout, static_cast<int>(vocab),
+          static_cast<const int64_t*>(has_target ? targets->data_ptr<int64_t>() : nullptr), ignore_index, c2,
+          static_cast<int>(top), has_target ? log_probs.data_ptr<float>() : nullptr, entropy.data_ptr<float>(),
+          top ? top_ids.data_ptr<int64_t>() : nullptr, top ? top_lp.data_ptr<float>() : nullptr,
+          save ? reinterpret_cast<float4*>(saved.data_ptr<float>()) : nullptr, status_word_ptr()));
+    };
+    if (top > 0) launch(stats_fwd_kernel<T, true>, (kCandidates + (blocks > 1 ? blocks * top : 0)) * sizeof(uint64_t));
+    else launch(stats_fwd_kernel<T, false>, 0);
   });
   TDSV_LAUNCH_CHECK();
   return {log_probs, entropy, top_ids, top_lp, saved};
@@ -223,10 +563,12 @@ at::Tensor token_stats_bwd(const at::Tensor& logits_in, const c10::optional<at::
   TDSV_CHECK(top <= kMaxTop, "token_statistics: too many alternatives");
   const float *g_lp = pointer(g_log_probs, rows), *g_ent = pointer(g_entropy, rows), *g_alt = pointer(g_top, rows * top);
   const float c2 = static_cast<float>(1.4426950408889634 / temperature), inv_t = static_cast<float>(1.0 / temperature);
+  const int64_t stretch = kStretchBytes / logits.element_size(), parts = (vocab + stretch - 1) / stretch;
+  TDSV_CHECK(rows * parts < (int64_t(1) << 31), "token_statistics: too many rows");
   with_logit_type(logits.scalar_type(), [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    stats_bwd_kernel<T><<<static_cast<unsigned>(rows), kStatThreads, 0, stream()>>>(
-        static_cast<const T*>(logits.data_ptr()), layout, static_cast<int>(vocab),
+    stats_bwd_kernel<T><<<static_cast<unsigned>(rows * parts), kStatThreads, 0, stream()>>>(
+        static_cast<const T*>(logits.data_ptr()), layout, static_cast<int>(vocab), static_cast<int>(parts),
         has_target ? targets->data_ptr<int64_t>() : nullptr, c2, inv_t, top,
         top ? top_ids.data_ptr<int64_t>() : nullptr, reinterpret_cast<const float4*>(saved.data_ptr<float>()), g_lp,
         g_ent, top ? g_alt : nullptr, static_cast<T*>(dlogits.data_ptr()));

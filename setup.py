@@ -61,6 +61,7 @@ setup(
         CUDAExtension(
             name="tiny_dsv41_b200._C",
             sources=SOURCES,
+            depends=sorted(glob.glob(os.path.join("csrc", "*.cuh")) + glob.glob(os.path.join("csrc", "*.h"))),
             include_dirs=[os.path.join(ROOT, "csrc")],
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
             extra_link_args=LINK_ARGS,
