@@ -22,126 +22,305 @@
 // dropped. Repeated ids count as one token whose q is the sum.
 #include "logit_rows.cuh"
 
+#include <cooperative_groups.h>
+#include <mutex>
+
 namespace tdsv {
 
 namespace {
 
 constexpr int kDistillThreads = 256;
 constexpr int kMaxAlternatives = 128;
+constexpr int kPerLane = kMaxAlternatives / 32;
+constexpr int kAhead = 4;        // vectors a thread has in flight
+constexpr int kMaxCluster = 16;  // above 8 the kernel is allowed it explicitly
 
+// What one warp works out for a row and the block then uses.
+struct RowPlan {
+  int read;       // whether the row is read at all
+  float base;     // reference of the pass that writes the gradient
+  float outside;  // A above
+};
+
+// A cluster of blocks takes a row, each block a stretch of it. The block's stretch is read from memory once:
+// it is summed as it arrives and kept in shared memory, from where the gradient is formed after the cluster
+// has joined its sums. So a row costs one read and one write, whatever its length (up to the shared memory
+// of 16 blocks). Several blocks on an SM are in different phases, which keeps loads, sums and stores going
+// at once.
+//
+// One warp deals with the alternatives, up to four a lane, without block barriers.
 template <typename T, typename I, bool GRAD>
-__global__ void __launch_bounds__(kDistillThreads)
+__global__ void __launch_bounds__(kDistillThreads, 4)
     distill_kernel(const T* __restrict__ logits, RowLayout layout, int v, const I* __restrict__ ids,
                    const float* __restrict__ teacher, int k, const float* __restrict__ weights, float c2, float inv_t,
                    bool tail, float* __restrict__ rows_out, float* __restrict__ weighted, T* __restrict__ dlogits,
                    int* status) {
-  extern __shared__ uint32_t bitmap[];
+  namespace cg = cooperative_groups;
+  constexpr int kSize = LogitVec<T>::kSize;
+  extern __shared__ uint4 smem[];  // GRAD: the stretch (one vector ahead of it, one after); then its bitmap
   __shared__ RowStats scratch[33];
-  __shared__ float fscratch[32];
+  __shared__ RowStats parts[kMaxCluster];
+  __shared__ int repeats[kMaxCluster];  // whether a block met an id twice
   __shared__ int at[kMaxAlternatives];
   __shared__ float q_s[kMaxAlternatives];
-  const int64_t r = blockIdx.x;
+  __shared__ float d_s[kMaxAlternatives];
+  __shared__ RowPlan plan;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
+  if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int64_t r = blockIdx.x / blocks;
   const T* row = logits + layout.offset(r);
-  T* out = GRAD ? dlogits + r * v : nullptr;
-  for (int i = threadIdx.x; i < (v + 31) / 32; i += blockDim.x) bitmap[i] = 0;
+
+  // this block's stretch: vectors [v0, v1) of the row, and the single values at the row's ends
+  const RowCut cut = cut_row(row, v);
+  const int per = (cut.vecs + blocks - 1) / blocks;
+  const int v0 = min(cut.vecs, part * per), v1 = min(cut.vecs, v0 + per);
+  const int e_vec = cut.head + v0 * kSize;  // the first vector's first element
+  const int first = part == 0 ? 0 : e_vec, last = part == blocks - 1 ? v : cut.head + v1 * kSize;
+  const uint4* base = reinterpret_cast<const uint4*>(row + cut.head) + v0;
+  const int vecs = v1 - v0;
+  uint4* kept = smem + 1;                                        // GRAD
+  T* kept_values = reinterpret_cast<T*>(kept) - (e_vec - first);  // element `first`
+  uint32_t* bitmap = reinterpret_cast<uint32_t*>(smem + (GRAD ? per + 2 : 0));  // element e is bit e - e_vec + 32
+  uint4 next[kAhead];
+  auto load = [&](int from) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = from + u * kDistillThreads + tid;
+      if (i < vecs) next[u] = load_stream(base + i);
+    }
+  };
+  load(0);
+  float single = -INFINITY;
+  int single_at = -1;
+  if (tid < e_vec - first) single_at = first + tid;
+  const int after = last - e_vec - vecs * kSize;
+  if (tid >= 32 && tid < 32 + after) single_at = last - after + tid - 32;
+  if (single_at >= 0) single = to_float<T>(row[single_at]);
+  if (GRAD && single_at >= 0) kept_values[single_at - first] = row[single_at];
+
+  const int words = (vecs * kSize + kSize + 31) / 32 + 1;
+  for (int i = tid; i < words; i += kDistillThreads) bitmap[i] = 0;
   __syncthreads();
-  // one thread per alternative
-  const int j = threadIdx.x;
-  int id = -1;
-  float t = -INFINITY;
-  bool bad = false;
-  if (j < k) {
-    const int64_t raw = static_cast<int64_t>(ids[r * k + j]);
-    bad = raw >= v;
-    if (raw >= 0 && raw < v) id = static_cast<int>(raw), t = teacher[r * k + j];
-    at[j] = id;
+
+  // ---- the teacher's distribution and the student at its tokens (warp 0)
+  int id[kPerLane];
+  float t[kPerLane], x[kPerLane], q[kPerLane], log_q[kPerLane];
+  float shift = 0.f, q_sum = 0.f, q_rest = 0.f;
+  bool any_bad = false;
+  if (tid < 32) {
+    bool bad = false, nan = false, repeated = false;
+    float top = -INFINITY;
+    int found = 0;
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) {
+      const int a = j * 32 + lane;
+      id[j] = -1, t[j] = -INFINITY, x[j] = -INFINITY;
+      if (a < k) {
+        const int64_t raw = static_cast<int64_t>(ids[r * k + a]);
+        bad |= raw >= v;
+        if (raw >= 0 && raw < v) id[j] = static_cast<int>(raw), t[j] = teacher[r * k + a];
+        at[a] = id[j];
+      }
+      if (id[j] >= 0) {
+        ++found;
+        nan |= t[j] != t[j];
+        top = fmaxf(top, t[j]);
+        x[j] = to_float<T>(row[id[j]]);
+        if (id[j] >= first && id[j] < last) {
+          const int bit = id[j] - e_vec + 32;
+          repeated |= (atomicOr(&bitmap[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u) != 0;
+        }
+      }
+    }
+    any_bad = __any_sync(0xffffffffu, bad);
+    nan = __any_sync(0xffffffffu, nan);
+    found = __reduce_add_sync(0xffffffffu, found);
+    repeated = __any_sync(0xffffffffu, repeated);
+    shift = warp_max(top);
+    if (lane == 0) {
+      plan.read = any_bad || nan || (found > 0 && (tail || shift != -INFINITY));
+      repeats[part] = repeated;
+    }
+    if (bad && part == 0) report_status(status, kOutOfBounds);
   }
-  if (bad) report_status(status, kOutOfBounds);
-  bool first = false;
-  if (id >= 0) first = !(atomicOr(&bitmap[id >> 5], 1u << (id & 31)) >> (id & 31) & 1u);
-  const int found = __syncthreads_count(id >= 0);
-  if (__syncthreads_or(id >= 0 && !first)) {  // repeated ids: the first of each counts, whatever the order above
-    first = id >= 0;
-    for (int i = 0; i < j && first; ++i) first = at[i] != id;
-  }
-  const bool any_bad = __syncthreads_or(bad);
-  const float tmax = block_max(t, fscratch);
-  const bool any_nan = __syncthreads_or(t != t);
-  const float w = weights != nullptr ? weights[r] : 1.f;
-  if (!any_bad && !any_nan && (found == 0 || (!tail && tmax == -INFINITY))) {
-    if (threadIdx.x == 0) rows_out[r] = 0.f, weighted[r] = 0.f;
-    if (GRAD)
-      for (int i = threadIdx.x; i < v; i += blockDim.x) out[i] = from_float<T>(0.f);
+  __syncthreads();
+  if (!plan.read) {  // the same for the whole cluster
+    if (tid == 0 && part == 0) rows_out[r] = 0.f, weighted[r] = 0.f;
+    if (GRAD) write_zeros<T, kDistillThreads>(dlogits + r * v + first, last - first);
+    if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     return;
   }
-  // the teacher's distribution
-  const float shift = tail ? 0.f : tmax;
-  float q = t == -INFINITY ? 0.f : expf(t - shift);
-  const float qsum = block_sum(q, fscratch);
-  float log_q = t - shift;
-  float q_rest = 0.f;
-  if (tail) {
-    q_rest = fmaxf(0.f, 1.f - qsum);
-  } else {
-    q /= qsum;
-    log_q -= logf(qsum);
+  if (tid < 32) {
+    if (tail) shift = 0.f;
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) {
+      q[j] = t[j] == -INFINITY ? 0.f : expf(t[j] - shift);
+      q_sum += q[j];
+    }
+    q_sum = warp_sum(q_sum);
+    if (tail) q_rest = fmaxf(0.f, 1.f - q_sum);
+    const float log_sum = tail ? 0.f : logf(q_sum);
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) {
+      log_q[j] = t[j] - shift - log_sum;
+      if (!tail) q[j] /= q_sum;
+      q_s[j * 32 + lane] = q[j];
+    }
   }
-  if (j < k) q_s[j] = q;
-  // the student outside the alternatives, and at them
-  RowStats rest;
-  for (int i = threadIdx.x; i < v; i += blockDim.x) {
-    if (bitmap[i >> 5] >> (i & 31) & 1u) continue;
-    rest.add(to_float<T>(row[i]), c2);
+
+  // ---- the student outside the alternatives: one pass
+  VecSum st;
+  const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bitmap);
+  for (int from = 0; from < vecs; from += kDistillThreads * kAhead) {
+    uint4 now[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) now[u] = next[u];
+    if (from + kDistillThreads * kAhead < vecs) load(from + kDistillThreads * kAhead);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = from + u * kDistillThreads + tid;
+      if (i < vecs) {
+        if (GRAD) kept[i] = now[u];
+        const uint32_t chosen = sizeof(T) == 2 ? bytes[i + 4] : bytes[(i >> 1) + 4] >> (4 * (i & 1)) & 15u;
+        if (chosen != 0) {
+          uint32_t w[4] = {now[u].x, now[u].y, now[u].z, now[u].w};
+#pragma unroll
+          for (int e = 0; e < kSize; ++e) {
+            if (!(chosen >> e & 1u)) continue;
+            if constexpr (sizeof(T) == 4) {
+              w[e] = 0xff800000u;
+            } else {
+              const uint32_t masked = std::is_same_v<T, __half> ? 0xfc00u : 0xff80u;
+              w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | masked << 16 : (w[e >> 1] & 0xffff0000u) | masked;
+            }
+          }
+          now[u] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        const uint4 one[1] = {now[u]};
+        mx = fmaxf(mx, vec_max<T, 1>(one));
+      }
+    }
+    if (mx > st.limit) st.raise(mx, c2);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (from + u * kDistillThreads + tid < vecs) st.add_vec<T>(now[u], c2);
   }
-  rest = block_merge(rest, c2, scratch);
-  const float x = id >= 0 ? to_float<T>(row[id]) : -INFINITY;
-  RowStats one;
-  if (first) one.add(x, c2);
-  const RowStats chosen = block_merge(one, c2, scratch);
-  RowStats all = chosen;
-  all.merge(rest, c2);
-  const float log2s = log2f(all.s);
-  if (tail && rest.s == 0.f) q_rest = 0.f;
-  float part = 0.f;
-  if (j < k && id >= 0 && q != 0.f) part = q * (log_q - kLn2 * ((x - all.m) * c2 - log2s));
-  float loss = block_sum(part, fscratch);
-  if (q_rest > 0.f) loss += q_rest * (logf(q_rest) - kLn2 * ((rest.m - all.m) * c2 + log2f(rest.s) - log2s));
-  const bool empty = all.s == 0.f;  // every logit is masked: no distribution, no gradient
-  if (empty) loss = INFINITY;
-  if (any_bad) loss = NAN;
-  if (threadIdx.x == 0) rows_out[r] = loss, weighted[r] = w * loss;
-  if (!GRAD) return;
-  const float whole = tail ? qsum + q_rest : 1.f;
-  const float scale = w * inv_t;
-  float outside = 0.f;
-  if (rest.s != 0.f) {
-    const float p_rest = exp2_fast((rest.m - all.m) * c2) * rest.s / all.s;
-    const float p_chosen = chosen.s == 0.f ? 0.f : exp2_fast((chosen.m - all.m) * c2) * chosen.s / all.s;
-    outside = scale * ((tail ? qsum : 1.f) * p_rest - q_rest * p_chosen) / rest.s;
+  if (single_at >= 0) {
+    const int bit = single_at - e_vec + 32;
+    if (!(bitmap[bit >> 5] >> (bit & 31) & 1u)) st.add_one(single, c2);
   }
-  const float base = rest.s == 0.f ? 0.f : rest.m;  // (every other logit is -inf there)
-  if (any_bad) outside = NAN;
-  for (int i = threadIdx.x; i < v; i += blockDim.x) {
-    const float y = (to_float<T>(row[i]) - base) * c2;
-    out[i] = from_float<T>(outside * exp2_fast(y));
+  RowStats rest = block_merge(st.total(), c2, scratch);
+  if (blocks > 1) {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (tid < blocks) {
+      *cluster.map_shared_rank(&parts[part], tid) = rest;
+      if (tid != part) *cluster.map_shared_rank(&repeats[part], tid) = repeats[part];
+    }
+    cluster.sync();
+    rest = parts[0];
+    for (int b = 1; b < blocks; ++b) rest.merge(parts[b], c2);
   }
-  __syncthreads();
-  if (j < k && id >= 0) {
-    float mass = 0.f;
-    for (int i = 0; i < k; ++i) mass += at[i] == id ? q_s[i] : 0.f;
-    const float d = empty ? 0.f : scale * (whole * exp2_fast((x - all.m) * c2 - log2s) - mass);
-    out[id] = from_float<T>(any_bad ? NAN : d);
+
+  // ---- the row's loss and constants (warp 0 of every block, the same everywhere)
+  const float w = weights != nullptr ? weights[r] : 1.f;
+  if (tid < 32) {
+    // repeated ids: the first place of each counts, with the mass of all
+    const bool repeated = __any_sync(0xffffffffu, lane < blocks && repeats[lane] != 0);
+    RowStats chosen;
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) {
+      bool counts = id[j] >= 0;
+      float mass = q[j];
+      if (repeated) {
+        for (int i = 0; i < j * 32 + lane && counts; ++i) counts = at[i] != id[j];
+        mass = 0.f;
+        for (int i = 0; i < k; ++i) mass += at[i] == id[j] ? q_s[i] : 0.f;
+      }
+      d_s[j * 32 + lane] = mass;
+      if (counts) chosen.add(x[j], c2);
+    }
+    chosen = warp_merge(chosen, c2);
+    RowStats all = chosen;
+    all.merge(rest, c2);
+    const float log2s = log2f(all.s);
+    if (rest.s == 0.f) q_rest = 0.f;
+    float loss = 0.f;
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j)
+      if (q[j] != 0.f) loss += q[j] * (log_q[j] - kLn2 * ((x[j] - all.m) * c2 - log2s));
+    loss = warp_sum(loss);
+    if (q_rest > 0.f) loss += q_rest * (logf(q_rest) - kLn2 * ((rest.m - all.m) * c2 + log2f(rest.s) - log2s));
+    const bool empty = all.s == 0.f;  // every logit is masked: no distribution, no gradient
+    if (empty) loss = INFINITY;
+    if (any_bad) loss = NAN;
+    const float mass = tail ? q_sum : 1.f, whole = mass + q_rest, scale = w * inv_t;
+    float outside = 0.f;
+    if (rest.s != 0.f) {
+      const float p_rest = exp2_fast((rest.m - all.m) * c2) * rest.s / all.s;
+      const float p_chosen = chosen.s == 0.f ? 0.f : exp2_fast((chosen.m - all.m) * c2) * chosen.s / all.s;
+      outside = scale * (mass * p_rest - q_rest * p_chosen) / rest.s;
+    }
+    if (GRAD) {
+#pragma unroll
+      for (int j = 0; j < kPerLane; ++j) {
+        const int a = j * 32 + lane;
+        const float d = empty ? 0.f : scale * (whole * exp2_fast((x[j] - all.m) * c2 - log2s) - d_s[a]);
+        d_s[a] = any_bad ? NAN : d;
+      }
+    }
+    if (lane == 0) {
+      plan.base = rest.s == 0.f ? 0.f : rest.m;  // (every other logit is -inf there)
+      plan.outside = any_bad ? NAN : outside;
+      if (part == 0) rows_out[r] = loss, weighted[r] = w * loss;
+    }
+  }
+  if constexpr (GRAD) {
+    __syncthreads();
+    T* out = dlogits + r * v;
+    write_gradient<T, kDistillThreads>(kept_values, out + first, last - first, plan.base, c2, plan.outside, 0.f);
+    __syncthreads();
+    if (tid < k && at[tid] >= first && at[tid] < last) out[at[tid]] = from_float<T>(d_s[tid]);
   }
 }
 
-// x *= *factor, unless it is one: the gradient was written for an upstream gradient of one.
+// x *= *factor, unless it is one: the gradient was written for an upstream gradient of one. x is an
+// allocation's start, so its vectors are aligned.
 template <typename T>
 __global__ void scale_kernel(T* __restrict__ x, int64_t n, const float* __restrict__ factor) {
   const float f = *factor;
   if (f == 1.f) return;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x)
-    x[i] = from_float<T>(to_float<T>(x[i]) * f);
+  const int64_t vecs = n / LogitVec<T>::kSize, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const int64_t me = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  uint4* xv = reinterpret_cast<uint4*>(x);
+  for (int64_t i = me; i < vecs; i += step) {
+    const uint4 v = xv[i];
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int p = 0; p < LogitVec<T>::kPairs; ++p) {
+      const float2 d = unpack_pair<T>(v, p);
+      if constexpr (sizeof(T) == 2) w[p] = pack_pair<T>(d.x * f, d.y * f);
+      else w[2 * p] = __float_as_uint(d.x * f), w[2 * p + 1] = __float_as_uint(d.y * f);
+    }
+    xv[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  const int64_t i = vecs * LogitVec<T>::kSize + me;
+  if (i < n) x[i] = from_float<T>(to_float<T>(x[i]) * f);
+}
+
+constexpr int kMostShared = 200 * 1024;
+
+// A row is split so that a block's stretch takes at most about 40 KB (with the gradient: five blocks' worth
+// of shared memory on an SM) or, where rows are few, until every SM holds four blocks; a stretch stays
+// several vectors a thread.
+int blocks_per_row(int64_t rows, int64_t vocab, int64_t item, bool grad) {
+  int blocks = 1;
+  while (grad && blocks < kMaxCluster && vocab * item > 40960 * blocks) blocks *= 2;
+  while (blocks < 8 && rows * blocks * 2 <= 4 * num_sms() && vocab * item / (blocks * 2) >= kDistillThreads * 16)
+    blocks *= 2;
+  return blocks;
 }
 
 }  // namespace
@@ -178,19 +357,40 @@ std::vector<at::Tensor> distill_fwd(const at::Tensor& logits_in, const at::Tenso
                       : at::empty({0}, logits.options());
   if (rows == 0) return {weighted.sum(), row_loss, dlogits};
   const int k = static_cast<int>(ids.size(1));
-  const int bitmap_bytes = static_cast<int>((vocab + 31) / 32 * 4);
-  TDSV_CHECK(bitmap_bytes <= 200 * 1024, "distillation_loss: vocabulary too large");
+  const int item = static_cast<int>(logits.element_size());
+  const int blocks = blocks_per_row(rows, vocab, item, grad);
+  // the largest stretch of a block: its vectors, one ahead and one after, and a bit for each value
+  const int64_t vecs = (vocab * item / 16 + blocks - 1) / blocks, values = vecs * 16 / item;
+  const int64_t smem = (grad ? (vecs + 2) * 16 : 0) + ((values + 16 / item + 31) / 32 + 1) * 4;
+  TDSV_CHECK(smem <= kMostShared, "distillation_loss: vocabulary too large");
+  TDSV_CHECK(rows * blocks < (int64_t(1) << 31), "distillation_loss: too many rows");
   const float c2 = static_cast<float>(1.4426950408889634 / temperature), inv_t = static_cast<float>(1.0 / temperature);
   auto run = [&](auto* tag, auto* itag, auto has_grad) {
     using T = std::remove_pointer_t<decltype(tag)>;
     using I = std::remove_pointer_t<decltype(itag)>;
     auto kern = distill_kernel<T, I, decltype(has_grad)::value>;
-    TDSV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-    kern<<<static_cast<unsigned>(rows), kDistillThreads, bitmap_bytes, stream()>>>(
-        static_cast<const T*>(logits.data_ptr()), layout, static_cast<int>(vocab), ids.data_ptr<I>(),
-        teacher.data_ptr<float>(), k, weighted_rows ? weights->data_ptr<float>() : nullptr, c2, inv_t, tail,
+    static std::once_flag once;
+    std::call_once(once, [&] {
+      TDSV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
+      TDSV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    });
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(rows * blocks));
+    config.blockDim = dim3(kDistillThreads);
+    config.dynamicSmemBytes = static_cast<size_t>(smem);
+    config.stream = stream();
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(blocks);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    TDSV_CUDA_CHECK(cudaLaunchKernelEx(
+        &config, kern, static_cast<const T*>(logits.data_ptr()), layout, static_cast<int>(vocab),
+        static_cast<const I*>(ids.data_ptr<I>()), static_cast<const float*>(teacher.data_ptr<float>()), k,
+        static_cast<const float*>(weighted_rows ? weights->data_ptr<float>() : nullptr), c2, inv_t, tail,
         row_loss.data_ptr<float>(), weighted.data_ptr<float>(), grad ? static_cast<T*>(dlogits.data_ptr()) : nullptr,
-        status_word_ptr());
+        status_word_ptr()));
   };
   with_logit_type(logits.scalar_type(), [&](auto* tag) {
     auto with_ids = [&](auto* itag) {
