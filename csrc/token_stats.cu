@@ -15,6 +15,8 @@
 // has ln p = -inf, H = 0 and no gradient. NaN or +inf in a row that is read gives NaN.
 #include "logit_rows.cuh"
 
+#include <cfloat>
+
 #include <cooperative_groups.h>
 
 namespace tdsv {
@@ -37,31 +39,25 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 constexpr uint32_t kMaskedKey = 0x007fffffu;  // of -inf: every finite value's key is larger
+constexpr uint32_t kInfKey = 0xff800000u;     // of +inf: NaN's keys are larger
 // A candidate: the larger value first, then the lower index.
 __device__ __forceinline__ uint64_t candidate(uint32_t key, int i) {
   return static_cast<uint64_t>(key) << 32 | (0xffffffffu - static_cast<uint32_t>(i));
 }
 __device__ __forceinline__ uint32_t candidate_key(uint64_t c) { return static_cast<uint32_t>(c >> 32); }
 
-// The largest threshold found in [lo, hi) at which at least `want` keys are counted, given that this holds
-// at lo and not at hi: halving steps, until at most `want + slack` are left or nothing lies between.
-// `count(t)` is this thread's number of keys >= t; every thread of the block calls it.
+// Values of a 16-bit type differ in the key's upper bits alone: thresholds move in those.
+template <typename T>
+constexpr int kKeyShift = std::is_same_v<T, __nv_bfloat16> ? 16 : std::is_same_v<T, __half> ? 13 : 0;
+
+// The largest threshold found in [lo, hi) that at least `want` reach, given that this holds at lo and not at
+// hi: halving steps, until at most `want + slack` reach it or nothing lies between. `count(t)` gives every
+// caller the number that reach t; `kept` is that number at the result, if it was counted.
 template <typename F>
-__device__ __forceinline__ uint32_t raise_threshold(uint32_t lo, uint32_t hi, int want, int slack, F&& count,
-                                                    int* scratch, int& kept) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int parity = 0;
-  kept = 0x7fffffff;
+__device__ __forceinline__ uint32_t raise_threshold(uint32_t lo, uint32_t hi, int want, int slack, int& kept, F&& count) {
   while (hi - lo > 1) {
     const uint32_t mid = lo + (hi - lo) / 2;
-    const int mine = __reduce_add_sync(0xffffffffu, count(mid));
-    int* slot = scratch + 8 * parity;
-    if (lane == 0) slot[warp] = mine;
-    __syncthreads();
-    int all = 0;
-#pragma unroll
-    for (int w = 0; w < kStatThreads / 32; ++w) all += slot[w];
-    parity ^= 1;  // (the next round writes the other half, so one barrier a round is enough)
+    const int all = count(mid);
     if (all >= want) {
       lo = mid;
       kept = all;
@@ -73,106 +69,143 @@ __device__ __forceinline__ uint32_t raise_threshold(uint32_t lo, uint32_t hi, in
   return lo;
 }
 
-// Block-wide maximum of a key.
-__device__ __forceinline__ uint32_t block_key_max(uint32_t k, uint32_t* scratch) {
-  k = __reduce_max_sync(0xffffffffu, k);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = k;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kStatThreads / 32; ++w) k = max(k, scratch[w]);
-  return k;
-}
-
+constexpr int kKept = kMaxTop + 64;
 struct TopScratch {
-  uint64_t kept[kStatThreads];  // candidates at or above the final threshold
-  uint32_t maxima[8];
+  uint64_t kept[kKept];          // the selected candidates, before they are ranked
+  uint32_t maxima[kStatThreads]; // of each thread's first batch
   int counts[16];
-  int n, survivors;
+  int n;
+  float threshold;
 };
 
-// Exactly the first `want` of the n candidates in `buf` (fewer where there are fewer), each handed to
-// emit(rank, candidate) once. Keys are halved down to the want-th largest; what is left is ranked by
-// counting, which also settles equal keys by index.
-template <typename F>
-__device__ __forceinline__ void select_top(const uint64_t* buf, int n, int want, TopScratch& sc, F&& emit) {
-  uint32_t top_key = 0;
-  for (int i = threadIdx.x; i < n; i += kStatThreads) top_key = max(top_key, candidate_key(buf[i]));
-  top_key = block_key_max(top_key, sc.maxima);
-  uint32_t cut = 1;  // (key 0 fills places without a candidate)
+// One warp's threshold over n keys, `stride` words apart, from `lo` up (or from below, should fewer than `want`
+// reach it). A selection is a chain of short steps: one warp takes it through without a block barrier, at an
+// eighth of the instructions that eight warps would issue. The keys may still be arriving: a threshold
+// that enough of them reach only gets easier to reach.
+template <typename T>
+__device__ __forceinline__ uint32_t warp_threshold(const volatile uint32_t* keys, int stride, int n, uint32_t lo,
+                                                   int want, int slack) {
+  constexpr int kShift = kKeyShift<T>;
+  const int lane = threadIdx.x & 31;
+  uint32_t hi = 0;
+  lo >>= kShift;
+  int reach = 0;
+  for (int i = lane; i < n; i += 32) {
+    const uint32_t k = keys[i * stride] >> kShift;
+    hi = max(hi, k);
+    reach += k >= lo;
+  }
+  hi = __reduce_max_sync(0xffffffffu, hi) + 1;
+  reach = __reduce_add_sync(0xffffffffu, reach);
+  if (reach < want) lo = 0;
+  int kept = 0;
+  lo = raise_threshold(lo, max(hi, lo + 1), want, slack, kept, [&](uint32_t t) {
+    int c = 0;
+    for (int i = lane; i < n; i += 32) c += keys[i * stride] >> kShift >= t;
+    return static_cast<int>(__reduce_add_sync(0xffffffffu, c));
+  });
+  return lo << kShift;
+}
+
+// The value from which a threshold's unit starts; the lowest finite one where that is masked (-inf) or NaN, so
+// that what reaches a threshold is never either.
+template <typename T>
+__device__ __forceinline__ float threshold_value(uint32_t t) {
+  return t >> kKeyShift<T> <= kMaskedKey >> kKeyShift<T> || t > kInfKey ? -FLT_MAX : key_value(t);
+}
+
+// One warp: exactly the first `want` of the n candidates in `buf` (fewer where there are fewer; 0 fills places
+// without one), each handed to emit(rank, candidate) once. Keys are halved, from `lo` up, to the want-th
+// largest, and what reaches it is ranked by counting, which settles equal keys by index. Where too many are
+// equal to be kept, the index is halved first.
+template <typename T, typename F>
+__device__ __forceinline__ void select_top(const uint64_t* buf, int n, uint32_t lo, int want, TopScratch& sc, F&& emit) {
+  constexpr int kShift = kKeyShift<T>;
+  const int lane = threadIdx.x & 31;
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(buf);
+  uint64_t least = 1;  // the first candidate that is kept
   if (n > want) {
-    int kept;
-    auto count = [&](uint32_t t) {
-      int c = 0;
-      for (int i = threadIdx.x; i < n; i += kStatThreads) c += candidate_key(buf[i]) >= t;
-      return c;
-    };
-    cut = raise_threshold(0, top_key + 1, want, 0, count, sc.counts, kept);
-    cut = max(cut, 1u);
+    const uint32_t cut = max(warp_threshold<T>(words + 1, 2, n, lo, want, 0), 1u);
+    least = static_cast<uint64_t>(cut) << 32;
+    int reach = 0, above = 0;
+    for (int i = lane; i < n; i += 32) {
+      reach += candidate_key(buf[i]) >= cut;
+      above += candidate_key(buf[i]) >> kShift > cut >> kShift;
+    }
+    reach = __reduce_add_sync(0xffffffffu, reach);
+    if (reach > kKept) {
+      above = __reduce_add_sync(0xffffffffu, above);
+      auto tied = [&](uint64_t c) { return candidate_key(c) >> kShift == cut >> kShift; };
+      int kept = 0;
+      const uint32_t t = raise_threshold(0, 0xffffffffu, want - above, 0, kept, [&](uint32_t at) {
+        int c = 0;
+        for (int i = lane; i < n; i += 32) c += tied(buf[i]) && static_cast<uint32_t>(buf[i]) >= at;
+        return static_cast<int>(__reduce_add_sync(0xffffffffu, c));
+      });
+      uint32_t key = 0;  // (one unit of keys holds one value)
+      for (int i = lane; i < n; i += 32)
+        if (tied(buf[i])) key = candidate_key(buf[i]);
+      least = static_cast<uint64_t>(__reduce_max_sync(0xffffffffu, key)) << 32 | t;
+    }
   }
-  if (threadIdx.x == 0) sc.survivors = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kStatThreads) {
-    if (candidate_key(buf[i]) < cut) continue;
-    const int at = atomicAdd(&sc.survivors, 1);
-    if (at < kStatThreads) sc.kept[at] = buf[i];
+  int m = 0;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const uint64_t c = i0 + lane < n ? buf[i0 + lane] : 0;
+    const bool keep = c >= least;
+    const uint32_t mask = __ballot_sync(0xffffffffu, keep);
+    if (keep) sc.kept[m + __popc(mask & ((1u << lane) - 1u))] = c;
+    m += __popc(mask);
   }
-  __syncthreads();
-  // many equal keys at the threshold do not fit: rank against all candidates then
-  const bool fits = sc.survivors <= kStatThreads;
-  const uint64_t* from = fits ? sc.kept : buf;
-  const int m = fits ? sc.survivors : n;
-  for (int i = threadIdx.x; i < m; i += kStatThreads) {
-    const uint64_t c = from[i];
-    if (candidate_key(c) < cut) continue;
+  __syncwarp();
+  for (int i = lane; i < m; i += 32) {
+    const uint64_t c = sc.kept[i];
     int rank = 0;
-    for (int j = 0; j < m; ++j) rank += from[j] > c;
+    for (int j = 0; j < m; ++j) rank += sc.kept[j] > c;
     if (rank < want) emit(rank, c);
   }
 }
 
 // The exact way for a block's part of a row whose candidates do not fit (rows in rising order, thousands of
 // equal values): halve the value, then the index among equals, re-reading the part each time, until what is
-// left fits. Returns the number of candidates put into `buf`.
+// left fits. The whole block takes part. Returns the number of candidates put into `buf`.
 template <typename T>
 __device__ __noinline__ int collect_again(const T* row, int first, int last, int want, uint64_t* buf, TopScratch& sc) {
-  auto count_keys = [&](uint32_t t) {
+  constexpr int kShift = kKeyShift<T>;
+  auto block_count = [&](auto&& hit) {
     int c = 0;
-    for (int i = first + threadIdx.x; i < last; i += kStatThreads) c += order_key(to_float<T>(row[i])) >= t;
+    for (int i = first + threadIdx.x; i < last; i += kStatThreads) c += hit(order_key(to_float<T>(row[i])), i);
+    c = __reduce_add_sync(0xffffffffu, c);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sc.counts[threadIdx.x >> 5] = c;
+    __syncthreads();
+    c = 0;
+    for (int w = 0; w < kStatThreads / 32; ++w) c += sc.counts[w];
     return c;
   };
-  int kept;
+  int kept = 0;
   // (+inf is the largest key that counts; NaN lies above it)
-  uint32_t cut = raise_threshold(kMaskedKey, 0xff800001u, want, kCandidates - want, count_keys, sc.counts, kept);
-  __syncthreads();
-  uint32_t none_after = 0xffffffffu;  // of the elements equal to `cut`, those up to this index
-  if (cut == kMaskedKey) cut = kMaskedKey + 1;  // fewer than `want` are unmasked
-  else if (kept > kCandidates) {
-    const int above = __reduce_add_sync(0xffffffffu, count_keys(cut + 1));
-    if ((threadIdx.x & 31) == 0) sc.counts[threadIdx.x >> 5] = above;
-    __syncthreads();
-    int more = 0;
-    for (int w = 0; w < kStatThreads / 32; ++w) more += sc.counts[w];
-    __syncthreads();
-    // indices count downwards so that "at least" still means a threshold from below
-    auto count_equal = [&](uint32_t t) {
-      int c = 0;
-      for (int i = first + threadIdx.x; i < last; i += kStatThreads)
-        c += order_key(to_float<T>(row[i])) == cut && static_cast<uint32_t>(last - i) >= t;
-      return c;
-    };
-    const uint32_t t = raise_threshold(0, static_cast<uint32_t>(last - first) + 1, want - more, 0, count_equal, sc.counts, kept);
-    none_after = static_cast<uint32_t>(last) - max(t, 1u);
+  uint32_t cut = raise_threshold(kMaskedKey >> kShift, (kInfKey >> kShift) + 1, want, kCandidates - want, kept,
+                                 [&](uint32_t t) { return block_count([&](uint32_t k, int) { return k >> kShift >= t; }); });
+  int until = last;  // of the values at `cut`, those before this index
+  if (cut == kMaskedKey >> kShift) {
+    cut = (kMaskedKey >> kShift) + 1;  // fewer than `want` are unmasked
+  } else if (kept > kCandidates) {
+    const int above = block_count([&](uint32_t k, int) { return k >> kShift > cut; });
+    // (an index counts down, so that "at least" is again a threshold from below)
+    until = last - static_cast<int>(raise_threshold(0, static_cast<uint32_t>(last - first), want - above, 0, kept, [&](uint32_t t) {
+              return block_count([&](uint32_t k, int i) {
+                return k >> kShift == cut && static_cast<uint32_t>(last - 1 - i) >= t;
+              });
+            }));
   }
+  __syncthreads();
   if (threadIdx.x == 0) sc.n = 0;
   __syncthreads();
   for (int i = first + threadIdx.x; i < last; i += kStatThreads) {
     const uint32_t key = order_key(to_float<T>(row[i]));
-    if (key > cut || (key == cut && static_cast<uint32_t>(i) <= none_after)) {
-      if (key > 0xff800000u) continue;
-      const int at = atomicAdd(&sc.n, 1);
-      if (at < kCandidates) buf[at] = candidate(key, i);
-    }
+    if (key > kInfKey || key >> kShift < cut || (key >> kShift == cut && i >= until)) continue;
+    const int at = atomicAdd(&sc.n, 1);
+    if (at < kCandidates) buf[at] = candidate(key, i);
   }
   __syncthreads();
   return min(sc.n, kCandidates);
@@ -182,7 +215,7 @@ __device__ __noinline__ int collect_again(const T* row, int first, int last, int
 //
 // Alternatives: a value is a candidate when it reaches a threshold that at least `top` values of the row
 // reach. The first threshold comes from the threads' own maxima of the first batch; it is raised after 1,
-// 2, 4, ... batches from the candidates so far, so that a row of V values gives some top * log2(V / 8192)
+// 4, 8, ... batches from the candidates so far, so that a row of V values gives some top * log2(V / 8192)
 // candidates, and the common step costs one comparison for a thread's whole batch.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kStatThreads, 4)
@@ -239,33 +272,43 @@ __global__ void __launch_bounds__(kStatThreads, 4)
       if (i < v1) next[u] = load_stream(base + i);
     }
   };
-  uint32_t threshold = kMaskedKey + 1;
-  float threshold_value = -INFINITY;
+  float threshold = -FLT_MAX;
   auto push = [&](float x, int i) {
     const uint32_t key = order_key(x);
-    if (key < threshold || key > 0xff800000u) return;
     const int at = atomicAdd(&sc.n, 1);
     if (at < kCandidates) top_smem[at] = candidate(key, i);
   };
-  if (TOP && tid == 0) sc.n = 0;
+  // (one warp) the row's alternatives from n places of which `there` hold one
+  auto write_top = [&](const uint64_t* from, int n, uint32_t lo, int there, const RowStats& st) {
+    const float log2s = log2f(st.s);
+    for (int j = min(there, top) + tid; j < top; j += 32) {
+      top_ids[r * top + j] = -1;
+      top_lp[r * top + j] = -INFINITY;
+    }
+    select_top<T>(from, n, lo, top, sc, [&](int rank, uint64_t c) {
+      top_ids[r * top + rank] = 0xffffffffu - static_cast<uint32_t>(c);
+      top_lp[r * top + rank] = kLn2 * ((key_value(candidate_key(c)) - st.m) * c2 - log2s);
+    });
+  };
   load(v0);
+  if constexpr (TOP) {
+    // (a place that is taken but not yet written reads as no candidate)
+    for (int i = tid; i < kCandidates / 2; i += kStatThreads) reinterpret_cast<uint4*>(top_smem)[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) sc.n = 0, sc.threshold = -FLT_MAX;
+    __syncthreads();
+  }
   int batch = 0;
   for (int from = v0; from < v1; from += kBatch, ++batch) {
     uint4 now[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) now[u] = next[u];
-    // vectors past the end repeat the thread's first one for the maximum and are skipped in the sums
     const int mine = (v1 - from - tid + kStatThreads - 1) / kStatThreads;  // valid ones of this thread
-    float mx = -INFINITY;
-    if (mine >= kUnroll) {
-      mx = vec_max<T, kUnroll>(now);
-    } else {
+    float tops[kUnroll], mx = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (u < mine) {
-          const uint4 one[1] = {now[u]};
-          mx = fmaxf(mx, vec_max<T, 1>(one));
-        }
+    for (int u = 0; u < kUnroll; ++u) {
+      const uint4 one[1] = {now[u]};
+      tops[u] = u < mine ? vec_max<T, 1>(one) : -INFINITY;
+      mx = fmaxf(mx, tops[u]);
     }
     if (from + kBatch < v1) load(from + kBatch);
     if (mx > st.limit) st.raise(mx, c2);
@@ -279,79 +322,60 @@ __global__ void __launch_bounds__(kStatThreads, 4)
     }
     if constexpr (TOP) {
       if (batch == 0) {
-        const uint32_t own = max(order_key(mx), order_key(single));
-        const uint32_t hi = block_key_max(own, sc.maxima);
-        if (hi > kMaskedKey && hi <= 0xff800000u) {
-          int kept;
-          threshold = raise_threshold(kMaskedKey, hi + 1, top, top / 4, [&](uint32_t t) { return own >= t ? 1 : 0; },
-                                      sc.counts, kept);
-          threshold = max(threshold, kMaskedKey + 1);
+        sc.maxima[tid] = max(order_key(mx), order_key(single));
+        __syncthreads();
+        if (tid < 32) {
+          const uint32_t t = warp_threshold<T>(sc.maxima, 1, kStatThreads, kMaskedKey, top, top / 4);
+          if (tid == 0) sc.threshold = threshold_value<T>(t);
         }
-        threshold_value = key_value(threshold);
         __syncthreads();
       }
-      if (mx >= threshold_value) {
+      threshold = *const_cast<volatile float*>(&sc.threshold);
+      if (mx >= threshold) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-          if (u >= mine) break;
-          const uint4 one[1] = {now[u]};
-          if (vec_max<T, 1>(one) < threshold_value) continue;
+          if (tops[u] < threshold) continue;
           const int i0 = cut.head + (from + u * kStatThreads + tid) * kSize;
 #pragma unroll
           for (int i = 0; i < LogitVec<T>::kPairs; ++i) {
             const float2 x = unpack_pair<T>(now[u], i);
-            if (x.x >= threshold_value) push(x.x, i0 + 2 * i);
-            if (x.y >= threshold_value) push(x.y, i0 + 2 * i + 1);
+            if (x.x >= threshold) push(x.x, i0 + 2 * i);
+            if (x.y >= threshold) push(x.y, i0 + 2 * i + 1);
           }
         }
       }
-      if (((batch + 1) & batch) == 0 && from + kBatch < v1) {
-        __syncthreads();
-        const int n = min(sc.n, kCandidates);
+      // after 2, 4, 8, ... batches a warp, another each time, raises the threshold; the others go on meanwhile
+      if (batch > 0 && ((batch + 1) & batch) == 0 && from + kBatch < v1 && tid >> 5 == (__ffs(batch + 1) & 7)) {
+        const int n = min(*const_cast<volatile int*>(&sc.n), kCandidates);
         if (n > top) {
-          uint32_t hi = 0;
-          for (int i = tid; i < n; i += kStatThreads) hi = max(hi, candidate_key(top_smem[i]));
-          hi = block_key_max(hi, sc.maxima);
-          int kept;
-          auto count = [&](uint32_t t) {
-            int c = 0;
-            for (int i = tid; i < n; i += kStatThreads) c += candidate_key(top_smem[i]) >= t;
-            return c;
-          };
-          threshold = raise_threshold(threshold, hi + 1, top, top / 4, count, sc.counts, kept);
-          threshold_value = key_value(threshold);
+          const uint32_t* keys = reinterpret_cast<const uint32_t*>(top_smem) + 1;
+          const uint32_t t = warp_threshold<T>(keys, 2, n, order_key(threshold), top, top / 4);
+          if ((tid & 31) == 0 && t > order_key(threshold)) *const_cast<volatile float*>(&sc.threshold) = threshold_value<T>(t);
         }
-        __syncthreads();
       }
     }
   }
   RowStats all = block_merge(st.total(), c2, scratch);
   if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   if constexpr (TOP) {
-    if (single > -INFINITY && single >= threshold_value) push(single, single_at);
+    if (single >= threshold) push(single, single_at);
     __syncthreads();
     int n = sc.n;
+    uint32_t lo = order_key(sc.threshold);
     __syncthreads();
     if (n > kCandidates) {
+      lo = 0;
       const int first = part == 0 ? 0 : cut.head + v0 * kSize;
       const int last = part == blocks - 1 ? v : cut.head + v1 * kSize;
       n = collect_again(row, first, last, top, top_smem, sc);
     }
-    if (blocks > 1) {
+    if (blocks > 1 && tid < 32) {
       // this block's first `top`, at its place in the leader's shared memory
       uint64_t* lead = cluster.map_shared_rank(top_smem, 0) + kCandidates + part * top;
-      for (int j = min(n, top) + tid; j < top; j += kStatThreads) lead[j] = 0;
-      select_top(top_smem, n, top, sc, [&](int rank, uint64_t c) { lead[rank] = c; });
-    } else {
-      const float log2s = log2f(all.s);
-      for (int j = min(n, top) + tid; j < top; j += kStatThreads) {
-        top_ids[r * top + j] = -1;
-        top_lp[r * top + j] = -INFINITY;
-      }
-      select_top(top_smem, n, top, sc, [&](int rank, uint64_t c) {
-        top_ids[r * top + rank] = 0xffffffffu - static_cast<uint32_t>(c);
-        top_lp[r * top + rank] = kLn2 * ((key_value(candidate_key(c)) - all.m) * c2 - log2s);
-      });
+      for (int j = min(n, top) + tid; j < top; j += 32) lead[j] = 0;
+      select_top<T>(top_smem, n, lo, top, sc, [&](int rank, uint64_t c) { lead[rank] = c; });
+    } else if (tid < 32) {
+      write_top(top_smem, n, lo, n, all);
     }
   }
   if (blocks > 1) {
@@ -361,24 +385,12 @@ __global__ void __launch_bounds__(kStatThreads, 4)
     all = parts[0];
     for (int b = 1; b < blocks; ++b) all.merge(parts[b], c2);
     if constexpr (TOP) {
-      const float log2s = log2f(all.s);
-      const uint64_t* gathered = top_smem + kCandidates;
-      int there = 0;
-      for (int j = tid; j < blocks * top; j += kStatThreads) there += gathered[j] != 0;
-      there = __reduce_add_sync(0xffffffffu, there);
-      if ((tid & 31) == 0) sc.counts[tid >> 5] = there;
-      __syncthreads();
-      int n = 0;
-      for (int w = 0; w < kStatThreads / 32; ++w) n += sc.counts[w];
-      __syncthreads();
-      for (int j = min(n, top) + tid; j < top; j += kStatThreads) {
-        top_ids[r * top + j] = -1;
-        top_lp[r * top + j] = -INFINITY;
+      if (tid < 32) {
+        const uint64_t* gathered = top_smem + kCandidates;
+        int there = 0;
+        for (int j = tid; j < blocks * top; j += 32) there += gathered[j] != 0;
+        write_top(gathered, blocks * top, 0, __reduce_add_sync(0xffffffffu, there), all);
       }
-      select_top(gathered, blocks * top, top, sc, [&](int rank, uint64_t c) {
-        top_ids[r * top + rank] = 0xffffffffu - static_cast<uint32_t>(c);
-        top_lp[r * top + rank] = kLn2 * ((key_value(candidate_key(c)) - all.m) * c2 - log2s);
-      });
     }
   }
   if (tid == 0) {
