@@ -86,7 +86,7 @@ at::Tensor token_logprob_bwd(const at::Tensor& logits, const at::Tensor& targets
 std::vector<at::Tensor> token_stats_fwd(const at::Tensor& logits, const c10::optional<at::Tensor>& targets,
                                         double temperature, int64_t top, int64_t ignore_index, bool save);
 at::Tensor token_stats_bwd(const at::Tensor& logits, const c10::optional<at::Tensor>& targets,
-                           const at::Tensor& top_ids, const at::Tensor& saved, double temperature,
+                           const c10::optional<at::Tensor>& top_ids, const at::Tensor& saved, double temperature,
                            const c10::optional<at::Tensor>& g_log_probs, const c10::optional<at::Tensor>& g_entropy,
                            const c10::optional<at::Tensor>& g_top);
 // lm_head.cu

@@ -286,6 +286,15 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
   }
 }
 
+// total = sum of x, in an order that depends on n alone.
+__global__ void __launch_bounds__(1024) sum_kernel(const float* __restrict__ x, int64_t n, float* __restrict__ total) {
+  __shared__ float scratch[32];
+  float s = 0.f;
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) s += x[i];
+  s = block_sum(s, scratch);
+  if (threadIdx.x == 0) *total = s;
+}
+
 // x *= *factor, unless it is one: the gradient was written for an upstream gradient of one. x is an
 // allocation's start, so its vectors are aligned.
 template <typename T>
@@ -325,15 +334,16 @@ int blocks_per_row(int64_t rows, int64_t vocab, int64_t item, bool grad) {
 
 }  // namespace
 
-// (total [], rows [R], dlogits like logits, or empty where no gradient is asked for).
+// (total [], the rows' divergences, the gradient like logits, or undefined where it is not asked for).
 std::vector<at::Tensor> distill_fwd(const at::Tensor& logits_in, const at::Tensor& ids, const at::Tensor& teacher,
                                     const c10::optional<at::Tensor>& weights, double temperature, bool tail, bool grad) {
   check_logits(logits_in, "distillation_loss");
   const int64_t vocab = logits_in.size(-1), rows = logits_in.numel() / vocab;
   check_cuda_tensor(ids, "teacher_ids");
   check_cuda_tensor(teacher, "teacher_log_probs");
-  TDSV_CHECK(ids.dim() == 2 && ids.size(0) == rows && ids.size(1) >= 1 && ids.size(1) <= kMaxAlternatives,
-             "distillation_loss: teacher_ids must be [rows, 1 .. ", kMaxAlternatives, "]");
+  TDSV_CHECK(ids.dim() == logits_in.dim() && ids.size(-1) >= 1 && ids.size(-1) <= kMaxAlternatives &&
+                 ids.numel() == rows * ids.size(-1),
+             "distillation_loss: teacher_ids must be [..., 1 .. ", kMaxAlternatives, "]");
   TDSV_CHECK(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, "distillation_loss: int32 or int64 teacher_ids");
   TDSV_CHECK(teacher.sizes() == ids.sizes() && teacher.scalar_type() == at::kFloat,
              "distillation_loss: fp32 teacher_log_probs of the ids' shape");
@@ -351,12 +361,13 @@ std::vector<at::Tensor> distill_fwd(const at::Tensor& logits_in, const at::Tenso
     TDSV_CHECK(row_layout(logits, layout), "distillation_loss: logits layout");
   }
   const auto f32 = logits.options().dtype(at::kFloat);
-  auto row_loss = at::empty({rows}, f32);
-  auto weighted = at::empty({rows}, f32);
+  auto row_loss = at::empty(logits.sizes().slice(0, logits.dim() - 1), f32);
+  auto weighted = at::empty({rows + 1}, f32);  // each row's share of the total, and the total
+  auto total = weighted.select(0, rows);
   auto dlogits = grad ? at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous))
-                      : at::empty({0}, logits.options());
-  if (rows == 0) return {weighted.sum(), row_loss, dlogits};
-  const int k = static_cast<int>(ids.size(1));
+                      : at::Tensor();
+  if (rows == 0) return {total.zero_(), row_loss, dlogits};
+  const int k = static_cast<int>(ids.size(-1));
   const int item = static_cast<int>(logits.element_size());
   const int blocks = blocks_per_row(rows, vocab, item, grad);
   // the largest stretch of a block: its vectors, one ahead and one after, and a bit for each value
@@ -401,7 +412,11 @@ std::vector<at::Tensor> distill_fwd(const at::Tensor& logits_in, const at::Tenso
     else with_ids(static_cast<int32_t*>(nullptr));
   });
   TDSV_LAUNCH_CHECK();
-  return {weighted.sum(), row_loss, dlogits};
+  const float* shares = weighted.data_ptr<float>();
+  sum_kernel<<<1, static_cast<unsigned>(std::min<int64_t>(1024, (rows + 31) / 32 * 32)), 0, stream()>>>(
+      shares, rows, weighted.data_ptr<float>() + rows);
+  TDSV_LAUNCH_CHECK();
+  return {total, row_loss, dlogits};
 }
 
 // dlogits *= factor (a device scalar), in place; nothing is touched where it is one.

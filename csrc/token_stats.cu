@@ -68,43 +68,76 @@ __device__ __forceinline__ uint32_t raise_threshold(uint32_t lo, uint32_t hi, in
   }
   return lo;
 }
+// The same in quarters: count3(a, b, c) gives three numbers, 10 bits each, so a step takes two halvings.
+template <typename F>
+__device__ __forceinline__ uint32_t raise_threshold_by4(uint32_t lo, uint32_t hi, int want, int slack, int& kept,
+                                                        F&& count3) {
+  while (hi - lo > 1) {
+    const uint32_t d = hi - lo, a = lo + max(d / 4, 1u), b = max(lo + d / 2, a), c = max(lo + d / 4 * 3, b);
+    const uint32_t all = count3(a, b, c);
+    const int na = all & 1023u, nb = all >> 10 & 1023u, nc = all >> 20;
+    if (nc >= want) lo = c, kept = nc;
+    else if (nb >= want) lo = b, hi = c, kept = nb;
+    else if (na >= want) lo = a, hi = b, kept = na;
+    else hi = a;
+    if (kept >= want && kept <= want + slack) break;
+  }
+  return lo;
+}
 
 constexpr int kKept = kMaxTop + 64;
 struct TopScratch {
   uint64_t kept[kKept];          // the selected candidates, before they are ranked
   uint32_t maxima[kStatThreads]; // of each thread's first batch
   int counts[16];
-  int n;
+  int n, kept_n, gathered;
   float threshold;
 };
 
 // One warp's threshold over n keys, `stride` words apart, from `lo` up (or from below, should fewer than `want`
-// reach it). A selection is a chain of short steps: one warp takes it through without a block barrier, at an
-// eighth of the instructions that eight warps would issue. The keys may still be arriving: a threshold
-// that enough of them reach only gets easier to reach.
-template <typename T>
+// reach it); `kept` keys reach the result. A selection is a chain of short steps: one warp takes it through
+// without a block barrier, its keys in registers (32 kRegs of them; more are read again each step). The keys
+// may still be arriving: a threshold that enough of them reach only gets easier to reach.
+template <typename T, int kRegs>
 __device__ __forceinline__ uint32_t warp_threshold(const volatile uint32_t* keys, int stride, int n, uint32_t lo,
-                                                   int want, int slack) {
+                                                   int want, int slack, int& kept) {
   constexpr int kShift = kKeyShift<T>;
   const int lane = threadIdx.x & 31;
-  uint32_t hi = 0;
   lo >>= kShift;
-  int reach = 0;
-  for (int i = lane; i < n; i += 32) {
-    const uint32_t k = keys[i * stride] >> kShift;
-    hi = max(hi, k);
-    reach += k >= lo;
+  uint32_t k[kRegs], hi = 0, least = 0xffffffffu;
+#pragma unroll
+  for (int j = 0; j < kRegs; ++j) {
+    // (places beyond n hold 0, which reaches no threshold above 0)
+    k[j] = j * 32 + lane < n ? keys[(j * 32 + lane) * stride] >> kShift : 0;
+    hi = max(hi, k[j]);
+    if (j * 32 + lane < n) least = min(least, k[j]);
+  }
+  for (int i = kRegs * 32 + lane; i < n; i += 32) {
+    hi = max(hi, keys[i * stride] >> kShift);
+    least = 0;
   }
   hi = __reduce_max_sync(0xffffffffu, hi) + 1;
-  reach = __reduce_add_sync(0xffffffffu, reach);
-  if (reach < want) lo = 0;
-  int kept = 0;
-  lo = raise_threshold(lo, max(hi, lo + 1), want, slack, kept, [&](uint32_t t) {
+  lo = max(lo, __reduce_min_sync(0xffffffffu, least));  // all n reach the least
+  auto count = [&](uint32_t t) {
     int c = 0;
-    for (int i = lane; i < n; i += 32) c += keys[i * stride] >> kShift >= t;
+#pragma unroll
+    for (int j = 0; j < kRegs; ++j) c += k[j] >= t;
+    for (int i = kRegs * 32 + lane; i < n; i += 32) c += keys[i * stride] >> kShift >= t;
     return static_cast<int>(__reduce_add_sync(0xffffffffu, c));
-  });
-  return lo << kShift;
+  };
+  kept = count(lo);
+  if (kept < want) {
+    lo = 0;
+    kept = n;
+  }
+  if (kept <= want + slack) return lo << kShift;
+  if (n > kRegs * 32) return raise_threshold(lo, max(hi, lo + 1), want, slack, kept, count) << kShift;
+  return raise_threshold_by4(lo, max(hi, lo + 1), want, slack, kept, [&](uint32_t ta, uint32_t tb, uint32_t tc) {
+    uint32_t ca = 0, cb = 0, cc = 0;
+#pragma unroll
+    for (int j = 0; j < kRegs; ++j) ca += k[j] >= ta, cb += k[j] >= tb, cc += k[j] >= tc;
+    return __reduce_add_sync(0xffffffffu, ca | cb << 10 | cc << 20);
+  }) << kShift;
 }
 
 // The value from which a threshold's unit starts; the lowest finite one where that is masked (-inf) or NaN, so
@@ -114,54 +147,63 @@ __device__ __forceinline__ float threshold_value(uint32_t t) {
   return t >> kKeyShift<T> <= kMaskedKey >> kKeyShift<T> || t > kInfKey ? -FLT_MAX : key_value(t);
 }
 
-// One warp: exactly the first `want` of the n candidates in `buf` (fewer where there are fewer; 0 fills places
-// without one), each handed to emit(rank, candidate) once. Keys are halved, from `lo` up, to the want-th
-// largest, and what reaches it is ranked by counting, which settles equal keys by index. Where too many are
-// equal to be kept, the index is halved first.
-template <typename T, typename F>
-__device__ __forceinline__ void select_top(const uint64_t* buf, int n, uint32_t lo, int want, TopScratch& sc, F&& emit) {
+// One warp: the first `want` of the n candidates in `buf` (all where there are fewer; 0 fills places without one)
+// go to sc.kept, in any order, and their number is returned; at most kKept when more are equal at the end of
+// the list. Keys are raised, from `lo` up, to the want-th largest; where too many are equal to be kept, the
+// lower indices are found by halving in turn.
+template <typename T>
+__device__ __forceinline__ int select_top(const uint64_t* buf, int n, uint32_t lo, int want, TopScratch& sc) {
   constexpr int kShift = kKeyShift<T>;
   const int lane = threadIdx.x & 31;
-  const uint32_t* words = reinterpret_cast<const uint32_t*>(buf);
   uint64_t least = 1;  // the first candidate that is kept
   if (n > want) {
-    const uint32_t cut = max(warp_threshold<T>(words + 1, 2, n, lo, want, 0), 1u);
+    int kept = 0;
+    const uint32_t cut = max(warp_threshold<T, 16>(reinterpret_cast<const uint32_t*>(buf) + 1, 2, n, lo, want, 0, kept), 1u);
     least = static_cast<uint64_t>(cut) << 32;
-    int reach = 0, above = 0;
-    for (int i = lane; i < n; i += 32) {
-      reach += candidate_key(buf[i]) >= cut;
-      above += candidate_key(buf[i]) >> kShift > cut >> kShift;
-    }
-    reach = __reduce_add_sync(0xffffffffu, reach);
-    if (reach > kKept) {
-      above = __reduce_add_sync(0xffffffffu, above);
+    if (kept > kKept && cut >> kShift != 0) {
       auto tied = [&](uint64_t c) { return candidate_key(c) >> kShift == cut >> kShift; };
-      int kept = 0;
+      int above = 0;
+      uint32_t key = 0;  // (one unit of keys holds one value)
+      for (int i = lane; i < n; i += 32) {
+        above += candidate_key(buf[i]) >> kShift > cut >> kShift;
+        if (tied(buf[i])) key = candidate_key(buf[i]);
+      }
+      above = __reduce_add_sync(0xffffffffu, above);
       const uint32_t t = raise_threshold(0, 0xffffffffu, want - above, 0, kept, [&](uint32_t at) {
         int c = 0;
         for (int i = lane; i < n; i += 32) c += tied(buf[i]) && static_cast<uint32_t>(buf[i]) >= at;
         return static_cast<int>(__reduce_add_sync(0xffffffffu, c));
       });
-      uint32_t key = 0;  // (one unit of keys holds one value)
-      for (int i = lane; i < n; i += 32)
-        if (tied(buf[i])) key = candidate_key(buf[i]);
       least = static_cast<uint64_t>(__reduce_max_sync(0xffffffffu, key)) << 32 | t;
     }
   }
   int m = 0;
+#pragma unroll 4
   for (int i0 = 0; i0 < n; i0 += 32) {
     const uint64_t c = i0 + lane < n ? buf[i0 + lane] : 0;
     const bool keep = c >= least;
     const uint32_t mask = __ballot_sync(0xffffffffu, keep);
-    if (keep) sc.kept[m + __popc(mask & ((1u << lane) - 1u))] = c;
+    const int at = m + __popc(mask & ((1u << lane) - 1u));
+    if (keep && at < kKept) sc.kept[at] = c;
     m += __popc(mask);
   }
   __syncwarp();
-  for (int i = lane; i < m; i += 32) {
-    const uint64_t c = sc.kept[i];
+  return min(m, kKept);
+}
+
+// The block: ranks the m kept candidates by counting, four threads to each; emit(rank, candidate) once each.
+template <typename F>
+__device__ __forceinline__ void rank_kept(const TopScratch& sc, int m, F&& emit) {
+  const int quarter = threadIdx.x & 3;
+  for (int i0 = 0; i0 < m; i0 += kStatThreads / 4) {
+    const int i = i0 + static_cast<int>(threadIdx.x >> 2);
+    const uint64_t c = i < m ? sc.kept[i] : 0;
     int rank = 0;
-    for (int j = 0; j < m; ++j) rank += sc.kept[j] > c;
-    if (rank < want) emit(rank, c);
+#pragma unroll 4
+    for (int j = quarter; j < m; j += 4) rank += sc.kept[j] > c;
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    if (quarter == 0 && i < m) emit(rank, c);
   }
 }
 
@@ -225,7 +267,7 @@ __global__ void __launch_bounds__(kStatThreads, 4)
                      float4* __restrict__ saved, int* status) {
   namespace cg = cooperative_groups;
   constexpr int kSize = LogitVec<T>::kSize;
-  extern __shared__ uint64_t top_smem[];  // [kCandidates], then [blocks of the cluster][top]
+  extern __shared__ uint64_t top_smem[];  // [kCandidates], then [blocks of the cluster][kKept]
   __shared__ RowStats scratch[33];
   __shared__ RowStats parts[kMaxCluster];
   __shared__ TopScratch sc;
@@ -248,7 +290,10 @@ __global__ void __launch_bounds__(kStatThreads, 4)
     return;
   }
   // every block of the cluster runs before another writes to its shared memory (waited for below)
-  if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (blocks > 1) {
+    if (TOP && tid == 0) sc.gathered = 0;
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  }
   const T* row = logits + layout.offset(r);
   const RowCut cut = cut_row(row, v);
   const int per = (cut.vecs + blocks - 1) / blocks;
@@ -277,18 +322,6 @@ __global__ void __launch_bounds__(kStatThreads, 4)
     const uint32_t key = order_key(x);
     const int at = atomicAdd(&sc.n, 1);
     if (at < kCandidates) top_smem[at] = candidate(key, i);
-  };
-  // (one warp) the row's alternatives from n places of which `there` hold one
-  auto write_top = [&](const uint64_t* from, int n, uint32_t lo, int there, const RowStats& st) {
-    const float log2s = log2f(st.s);
-    for (int j = min(there, top) + tid; j < top; j += 32) {
-      top_ids[r * top + j] = -1;
-      top_lp[r * top + j] = -INFINITY;
-    }
-    select_top<T>(from, n, lo, top, sc, [&](int rank, uint64_t c) {
-      top_ids[r * top + rank] = 0xffffffffu - static_cast<uint32_t>(c);
-      top_lp[r * top + rank] = kLn2 * ((key_value(candidate_key(c)) - st.m) * c2 - log2s);
-    });
   };
   load(v0);
   if constexpr (TOP) {
@@ -325,7 +358,8 @@ __global__ void __launch_bounds__(kStatThreads, 4)
         sc.maxima[tid] = max(order_key(mx), order_key(single));
         __syncthreads();
         if (tid < 32) {
-          const uint32_t t = warp_threshold<T>(sc.maxima, 1, kStatThreads, kMaskedKey, top, top / 4);
+          int kept;
+          const uint32_t t = warp_threshold<T, kStatThreads / 32>(sc.maxima, 1, kStatThreads, 0, top, top / 4, kept);
           if (tid == 0) sc.threshold = threshold_value<T>(t);
         }
         __syncthreads();
@@ -345,18 +379,22 @@ __global__ void __launch_bounds__(kStatThreads, 4)
         }
       }
       // after 2, 4, 8, ... batches a warp, another each time, raises the threshold; the others go on meanwhile
-      if (batch > 0 && ((batch + 1) & batch) == 0 && from + kBatch < v1 && tid >> 5 == (__ffs(batch + 1) & 7)) {
+      if (batch > 0 && ((batch + 1) & batch) == 0 && from + 2 * kBatch < v1 && tid >> 5 == (__ffs(batch + 1) & 7)) {
         const int n = min(*const_cast<volatile int*>(&sc.n), kCandidates);
         if (n > top) {
           const uint32_t* keys = reinterpret_cast<const uint32_t*>(top_smem) + 1;
-          const uint32_t t = warp_threshold<T>(keys, 2, n, order_key(threshold), top, top / 4);
+          int kept;
+          const uint32_t t = warp_threshold<T, 8>(keys, 2, n, order_key(threshold), top, top / 4, kept);
           if ((tid & 31) == 0 && t > order_key(threshold)) *const_cast<volatile float*>(&sc.threshold) = threshold_value<T>(t);
         }
       }
     }
   }
   RowStats all = block_merge(st.total(), c2, scratch);
-  if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if (blocks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  // the candidates of the row: this block's, or what every block of the cluster sends to the first one
+  int from_n = 0;
+  uint32_t from_lo = 0;
   if constexpr (TOP) {
     if (single >= threshold) push(single, single_at);
     __syncthreads();
@@ -369,14 +407,19 @@ __global__ void __launch_bounds__(kStatThreads, 4)
       const int last = part == blocks - 1 ? v : cut.head + v1 * kSize;
       n = collect_again(row, first, last, top, top_smem, sc);
     }
-    if (blocks > 1 && tid < 32) {
-      // this block's first `top`, at its place in the leader's shared memory
-      uint64_t* lead = cluster.map_shared_rank(top_smem, 0) + kCandidates + part * top;
-      for (int j = min(n, top) + tid; j < top; j += 32) lead[j] = 0;
-      select_top<T>(top_smem, n, lo, top, sc, [&](int rank, uint64_t c) { lead[rank] = c; });
-    } else if (tid < 32) {
-      write_top(top_smem, n, lo, n, all);
+    if (blocks > 1) {
+      // this block's first `top`, in any order, behind the other blocks' in the leader's shared memory
+      if (tid < 32) {
+        const int m = select_top<T>(top_smem, n, lo, top, sc);
+        int first = 0;
+        if (tid == 0) first = atomicAdd(cluster.map_shared_rank(&sc.gathered, 0), m);
+        first = __shfl_sync(0xffffffffu, first, 0);
+        uint64_t* lead = cluster.map_shared_rank(top_smem, 0) + kCandidates + first;
+        for (int j = tid; j < m; j += 32) lead[j] = sc.kept[j];
+      }
     }
+    from_n = n;
+    from_lo = lo;
   }
   if (blocks > 1) {
     if (tid == 0) *cluster.map_shared_rank(&parts[part], 0) = all;
@@ -384,14 +427,25 @@ __global__ void __launch_bounds__(kStatThreads, 4)
     if (part != 0) return;
     all = parts[0];
     for (int b = 1; b < blocks; ++b) all.merge(parts[b], c2);
-    if constexpr (TOP) {
-      if (tid < 32) {
-        const uint64_t* gathered = top_smem + kCandidates;
-        int there = 0;
-        for (int j = tid; j < blocks * top; j += 32) there += gathered[j] != 0;
-        write_top(gathered, blocks * top, 0, __reduce_add_sync(0xffffffffu, there), all);
-      }
+    if (TOP) from_n = sc.gathered;
+  }
+  if constexpr (TOP) {
+    if (tid < 32) {
+      const int m = select_top<T>(top_smem + (blocks > 1 ? kCandidates : 0), from_n, from_lo, top, sc);
+      if (tid == 0) sc.kept_n = m;
     }
+    __syncthreads();
+    const int m = sc.kept_n;
+    const float log2s = log2f(all.s);
+    for (int j = min(m, top) + tid; j < top; j += kStatThreads) {
+      top_ids[r * top + j] = -1;
+      top_lp[r * top + j] = -INFINITY;
+    }
+    rank_kept(sc, m, [&](int rank, uint64_t c) {
+      if (rank >= top) return;
+      top_ids[r * top + rank] = 0xffffffffu - static_cast<uint32_t>(c);
+      top_lp[r * top + rank] = kLn2 * ((key_value(candidate_key(c)) - all.m) * c2 - log2s);
+    });
   }
   if (tid == 0) {
     const float log2s = log2f(all.s);
@@ -484,7 +538,8 @@ int blocks_per_row(int64_t rows, int64_t vocab, int64_t item) {
 
 }  // namespace
 
-// (log_probs, entropy, top_ids, top_log_probs, saved): flat over the rows of logits [..., V].
+// (log_probs, entropy, top_ids, top_log_probs, saved) over the rows of logits [..., V]; what is not asked for is
+// undefined (None).
 std::vector<at::Tensor> token_stats_fwd(const at::Tensor& logits_in, const c10::optional<at::Tensor>& targets,
                                         double temperature, int64_t top, int64_t ignore_index, bool save) {
   check_logits(logits_in, "token_statistics");
@@ -505,11 +560,17 @@ std::vector<at::Tensor> token_stats_fwd(const at::Tensor& logits_in, const c10::
     TDSV_CHECK(targets->scalar_type() == at::kLong && targets->numel() == rows, "token_statistics: int64 targets, one per row");
   }
   const auto f32 = logits.options().dtype(at::kFloat);
-  auto log_probs = at::empty({has_target ? rows : 0}, f32);
-  auto entropy = at::empty({rows}, f32);
-  auto top_ids = at::empty({top > 0 ? rows : 0, top}, logits.options().dtype(at::kLong));
-  auto top_lp = at::empty({top > 0 ? rows : 0, top}, f32);
-  auto saved = at::empty({save ? rows : 0, 4}, f32);
+  const auto shape = logits.sizes().slice(0, logits.dim() - 1);
+  at::Tensor log_probs, top_ids, top_lp, saved;
+  if (has_target) log_probs = at::empty(shape, f32);
+  auto entropy = at::empty(shape, f32);
+  if (top > 0) {
+    auto wide = shape.vec();
+    wide.push_back(top);
+    top_ids = at::empty(wide, f32.dtype(at::kLong));
+    top_lp = at::empty(wide, f32);
+  }
+  if (save) saved = at::empty({rows, 4}, f32);
   if (rows == 0) return {log_probs, entropy, top_ids, top_lp, saved};
   const float c2 = static_cast<float>(1.4426950408889634 / temperature);
   const int blocks = blocks_per_row(rows, vocab, logits.element_size());
@@ -534,7 +595,7 @@ std::vector<at::Tensor> token_stats_fwd(const at::Tensor& logits_in, const c10::
           top ? top_ids.data_ptr<int64_t>() : nullptr, top ? top_lp.data_ptr<float>() : nullptr,
           save ? reinterpret_cast<float4*>(saved.data_ptr<float>()) : nullptr, status_word_ptr()));
     };
-    if (top > 0) launch(stats_fwd_kernel<T, true>, (kCandidates + (blocks > 1 ? blocks * top : 0)) * sizeof(uint64_t));
+    if (top > 0) launch(stats_fwd_kernel<T, true>, (kCandidates + (blocks > 1 ? blocks * kKept : 0)) * sizeof(uint64_t));
     else launch(stats_fwd_kernel<T, false>, 0);
   });
   TDSV_LAUNCH_CHECK();
@@ -543,7 +604,7 @@ std::vector<at::Tensor> token_stats_fwd(const at::Tensor& logits_in, const c10::
 
 // Contiguous gradient of the logits, in their shape and type.
 at::Tensor token_stats_bwd(const at::Tensor& logits_in, const c10::optional<at::Tensor>& targets,
-                           const at::Tensor& top_ids, const at::Tensor& saved, double temperature,
+                           const c10::optional<at::Tensor>& top_ids, const at::Tensor& saved, double temperature,
                            const c10::optional<at::Tensor>& g_log_probs, const c10::optional<at::Tensor>& g_entropy,
                            const c10::optional<at::Tensor>& g_top) {
   check_logits(logits_in, "token_statistics");
@@ -558,7 +619,13 @@ at::Tensor token_stats_bwd(const at::Tensor& logits_in, const c10::optional<at::
   auto dlogits = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
   if (rows == 0) return dlogits;
   check_cuda_tensor(saved, "saved");
-  check_cuda_tensor(top_ids, "top_ids");
+  const bool has_top = top_ids.has_value() && top_ids->defined();
+  if (has_top) {
+    check_cuda_tensor(*top_ids, "top_ids");
+    TDSV_CHECK(top_ids->scalar_type() == at::kLong && top_ids->dim() >= 1 && top_ids->size(-1) <= kMaxTop &&
+                   top_ids->numel() == rows * top_ids->size(-1),
+               "token_statistics: top_ids");
+  }
   TDSV_CHECK(saved.scalar_type() == at::kFloat && saved.numel() == 4 * rows, "token_statistics: saved row statistics");
   auto pointer = [&](const c10::optional<at::Tensor>& t, int64_t count) -> const float* {
     if (!t.has_value() || !t->defined()) return nullptr;
@@ -571,8 +638,7 @@ at::Tensor token_stats_bwd(const at::Tensor& logits_in, const c10::optional<at::
     check_cuda_tensor(*targets, "targets");
     TDSV_CHECK(targets->scalar_type() == at::kLong && targets->numel() == rows, "token_statistics: int64 targets, one per row");
   }
-  const int top = static_cast<int>(top_ids.size(1));
-  TDSV_CHECK(top <= kMaxTop, "token_statistics: too many alternatives");
+  const int top = has_top ? static_cast<int>(top_ids->size(-1)) : 0;
   const float *g_lp = pointer(g_log_probs, rows), *g_ent = pointer(g_entropy, rows), *g_alt = pointer(g_top, rows * top);
   const float c2 = static_cast<float>(1.4426950408889634 / temperature), inv_t = static_cast<float>(1.0 / temperature);
   const int64_t stretch = kStretchBytes / logits.element_size(), parts = (vocab + stretch - 1) / stretch;
@@ -582,7 +648,7 @@ at::Tensor token_stats_bwd(const at::Tensor& logits_in, const c10::optional<at::
     stats_bwd_kernel<T><<<static_cast<unsigned>(rows * parts), kStatThreads, 0, stream()>>>(
         static_cast<const T*>(logits.data_ptr()), layout, static_cast<int>(vocab), static_cast<int>(parts),
         has_target ? targets->data_ptr<int64_t>() : nullptr, c2, inv_t, top,
-        top ? top_ids.data_ptr<int64_t>() : nullptr, reinterpret_cast<const float4*>(saved.data_ptr<float>()), g_lp,
+        top ? top_ids->data_ptr<int64_t>() : nullptr, reinterpret_cast<const float4*>(saved.data_ptr<float>()), g_lp,
         g_ent, top ? g_alt : nullptr, static_cast<T*>(dlogits.data_ptr()));
   });
   TDSV_LAUNCH_CHECK();

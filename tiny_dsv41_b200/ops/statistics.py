@@ -130,7 +130,8 @@ class _TokenStatistics(torch.autograd.Function):
         lp, entropy, ids, values, saved = ext().token_stats_fwd(logits, targets, temperature, top, IGNORE_INDEX, True)
         ctx.save_for_backward(logits, targets, ids, saved)
         ctx.temperature = temperature
-        ctx.mark_non_differentiable(ids)
+        if ids is not None:
+            ctx.mark_non_differentiable(ids)
         ctx.set_materialize_grads(False)
         return lp, entropy, ids, values
 
@@ -138,7 +139,7 @@ class _TokenStatistics(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_lp, g_entropy, _g_ids, g_values):
         logits, targets, ids, saved = ctx.saved_tensors
-        plain = lambda g: None if g is None else g.float().contiguous()  # noqa: E731
+        plain = lambda g: None if g is None else g.contiguous()  # noqa: E731
         return ext().token_stats_bwd(logits, targets, ids, saved, ctx.temperature, plain(g_lp), plain(g_entropy),
                                      plain(g_values)), None, None, None
 
@@ -161,16 +162,14 @@ def token_statistics(logits: torch.Tensor, targets: torch.Tensor | None = None, 
         raise ValueError(f"top must be a whole number in [0, min({MAX_TOP}, vocabulary)]")
     if targets is not None:
         _check_targets(targets, shape, logits.device)
-    if not on_gpu(logits):
+    if not logits.is_cuda:
         return _scores_reference(logits, targets, temperature, top)
     if targets is not None:
         targets = targets.contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        lp, entropy, ids, values = _TokenStatistics.apply(logits, targets, temperature, top)
-    else:
-        lp, entropy, ids, values, _ = ext().token_stats_fwd(logits, targets, temperature, top, IGNORE_INDEX, False)
-    return TokenStatistics(None if targets is None else lp.view(shape), entropy.view(shape),
-                           ids.view(*shape, top) if top else None, values.view(*shape, top) if top else None)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenStatistics(*_TokenStatistics.apply(logits, targets, temperature, top))
+    lp, entropy, ids, values, _ = ext().token_stats_fwd(logits, targets, temperature, top, IGNORE_INDEX, False)
+    return TokenStatistics(lp, entropy, ids, values)
 
 
 # -- statistics of the LM head's product ------------------------------------------------------------
@@ -258,7 +257,7 @@ class _Distillation(torch.autograd.Function):
         if dlogits is None:
             raise RuntimeError("distillation_loss: the gradient was handed out by an earlier backward; call the "
                                "operator again")
-        ext().distill_scale(dlogits, g_total.float().contiguous())
+        ext().distill_scale(dlogits, g_total.contiguous())
         return dlogits, None, None, None, None, None
 
 
@@ -289,19 +288,20 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
         raise ValueError(f"a teacher records 1 to {MAX_TOP} alternatives")
     if weights is not None and weights.shape != shape:
         raise ValueError("weights must hold one value per row")
-    if any(t is not None and t.device != logits.device for t in (teacher_ids, teacher_log_probs, weights)):
+    device = logits.device
+    if teacher_ids.device != device or teacher_log_probs.device != device or (
+            weights is not None and weights.device != device):
         raise ValueError("teacher and weights must be on the logits' device")
-    if not on_gpu(logits):
+    if not logits.is_cuda:
         return _distillation_reference(logits, teacher_ids, teacher_log_probs.detach(),
                                        None if weights is None else weights.detach(), temperature, tail)
-    ids = teacher_ids.reshape(-1, k).contiguous()
-    teacher = teacher_log_probs.detach().float().reshape(-1, k).contiguous()
-    weights = None if weights is None else weights.detach().float().reshape(-1).contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
+    ids, teacher = teacher_ids.contiguous(), teacher_log_probs.detach().float().contiguous()
+    weights = None if weights is None else weights.detach().float().contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
         total, rows = _Distillation.apply(logits, ids, teacher, weights, temperature, tail)
     else:
         total, rows, _ = ext().distill_fwd(logits, ids, teacher, weights, temperature, tail, False)
-    return DistillationLoss(total, rows.view(shape))
+    return DistillationLoss(total, rows)
 
 
 __all__ = ["DistillationLoss", "TokenStatistics", "distillation_loss", "linear_token_statistics",
