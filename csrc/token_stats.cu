@@ -27,7 +27,7 @@ constexpr int kStatThreads = 256;
 constexpr int kMaxTop = 128;
 constexpr int kUnroll = 4;          // vectors a thread has in flight
 constexpr int kBatch = kStatThreads * kUnroll;
-constexpr int kCandidates = 2048;   // candidates for the alternatives that a block can hold
+constexpr int kCandidates = 2176;   // candidates for the alternatives that a block can hold: kKept vectors' values too
 constexpr int kMaxCluster = 8;
 
 // Floats as whole numbers of the same order (both zeros are one value), and back.
@@ -85,13 +85,14 @@ __device__ __forceinline__ uint32_t raise_threshold_by4(uint32_t lo, uint32_t hi
   return lo;
 }
 
-constexpr int kKept = kMaxTop + 64;
+constexpr int kKept = 2 * kMaxTop;
+static_assert(kCandidates >= 8 * kKept + 2 * 7, "the values of the kept vectors fit");
 struct TopScratch {
   uint64_t kept[kKept];          // the selected candidates, before they are ranked
   uint32_t maxima[kStatThreads]; // of each thread's first batch
   int counts[16];
   int n, kept_n, gathered;
-  float threshold;
+  float first, threshold;
 };
 
 // One warp's threshold over n keys, `stride` words apart, from `lo` up (or from below, should fewer than `want`
@@ -147,10 +148,9 @@ __device__ __forceinline__ float threshold_value(uint32_t t) {
   return t >> kKeyShift<T> <= kMaskedKey >> kKeyShift<T> || t > kInfKey ? -FLT_MAX : key_value(t);
 }
 
-// One warp: the first `want` of the n candidates in `buf` (all where there are fewer; 0 fills places without one)
-// go to sc.kept, in any order, and their number is returned; at most kKept when more are equal at the end of
-// the list. Keys are raised, from `lo` up, to the want-th largest; where too many are equal to be kept, the
-// lower indices are found by halving in turn.
+// One warp: the candidates among the n in `buf` whose key reaches the want-th largest (all where there are
+// fewer; 0 fills places without one) go to sc.kept, in any order, and their number is returned. Where more are
+// equal at the end than fit, those above and the `want` lowest indices of the equal ones go.
 template <typename T>
 __device__ __forceinline__ int select_top(const uint64_t* buf, int n, uint32_t lo, int want, TopScratch& sc) {
   constexpr int kShift = kKeyShift<T>;
@@ -169,7 +169,7 @@ __device__ __forceinline__ int select_top(const uint64_t* buf, int n, uint32_t l
         if (tied(buf[i])) key = candidate_key(buf[i]);
       }
       above = __reduce_add_sync(0xffffffffu, above);
-      const uint32_t t = raise_threshold(0, 0xffffffffu, want - above, 0, kept, [&](uint32_t at) {
+      const uint32_t t = raise_threshold(0, 0xffffffffu, want, kKept - want - above, kept, [&](uint32_t at) {
         int c = 0;
         for (int i = lane; i < n; i += 32) c += tied(buf[i]) && static_cast<uint32_t>(buf[i]) >= at;
         return static_cast<int>(__reduce_add_sync(0xffffffffu, c));
@@ -255,10 +255,13 @@ __device__ __noinline__ int collect_again(const T* row, int first, int last, int
 
 // A block (or a cluster of blocks, each on a stretch of the row) reads a row once in 16-byte vectors.
 //
-// Alternatives: a value is a candidate when it reaches a threshold that at least `top` values of the row
-// reach. The first threshold comes from the threads' own maxima of the first batch; it is raised after 1,
-// 4, 8, ... batches from the candidates so far, so that a row of V values gives some top * log2(V / 8192)
-// candidates, and the common step costs one comparison for a thread's whole batch.
+// Alternatives are found by whole vectors first: a vector is a candidate when its maximum reaches a threshold
+// that the maxima of at least `top` vectors reach. The first threshold comes from the threads' maxima of the
+// first batch; later vectors have to pass it (equal values there lose by their index), and it is raised after 2,
+// 4, 8, ... batches, so that a row gives some top * log2 of its batches candidates. The common step costs one
+// comparison for a thread's batch, a candidate some 20 instructions (by single values it was 67, and 4096 rows
+// with 64 alternatives took 546 us). At the end the `top` first vectors hold all of the `top` first values: they
+// are read once more, value by value.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kStatThreads, 4)
     stats_fwd_kernel(const T* __restrict__ logits, RowLayout layout, int v, const int64_t* __restrict__ targets,
@@ -317,12 +320,6 @@ __global__ void __launch_bounds__(kStatThreads, 4)
       if (i < v1) next[u] = load_stream(base + i);
     }
   };
-  float threshold = -FLT_MAX;
-  auto push = [&](float x, int i) {
-    const uint32_t key = order_key(x);
-    const int at = atomicAdd(&sc.n, 1);
-    if (at < kCandidates) top_smem[at] = candidate(key, i);
-  };
   load(v0);
   if constexpr (TOP) {
     // (a place that is taken but not yet written reads as no candidate)
@@ -331,52 +328,54 @@ __global__ void __launch_bounds__(kStatThreads, 4)
     __syncthreads();
   }
   int batch = 0;
-  for (int from = v0; from < v1; from += kBatch, ++batch) {
+  // a batch of which every thread has all vectors, or the last one
+  auto step = [&](auto whole, int from) {
     uint4 now[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) now[u] = next[u];
-    const int mine = (v1 - from - tid + kStatThreads - 1) / kStatThreads;  // valid ones of this thread
     float tops[kUnroll], mx = -INFINITY;
+    const int mine = decltype(whole)::value ? kUnroll : (v1 - from - tid + kStatThreads - 1) / kStatThreads;
+    if constexpr (TOP) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const uint4 one[1] = {now[u]};
-      tops[u] = u < mine ? vec_max<T, 1>(one) : -INFINITY;
-      mx = fmaxf(mx, tops[u]);
+      for (int u = 0; u < kUnroll; ++u) {
+        now[u] = next[u];
+        const uint4 one[1] = {now[u]};
+        tops[u] = u < mine ? vec_max<T, 1>(one) : -INFINITY;
+        mx = fmaxf(mx, tops[u]);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) now[u] = u == 0 || u < mine ? next[u] : now[0];
+      if (mine > 0) mx = vec_max<T, kUnroll>(now);
     }
     if (from + kBatch < v1) load(from + kBatch);
     if (mx > st.limit) st.raise(mx, c2);
-    if (mine >= kUnroll) {
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) st.add_vec<T>(now[u], c2);
-    } else {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (u < mine) st.add_vec<T>(now[u], c2);
-    }
+    for (int u = 0; u < kUnroll; ++u)
+      if (u < mine) st.add_vec<T>(now[u], c2);
     if constexpr (TOP) {
+      float threshold;
       if (batch == 0) {
-        sc.maxima[tid] = max(order_key(mx), order_key(single));
+        sc.maxima[tid] = order_key(mx);
         __syncthreads();
         if (tid < 32) {
           int kept;
           const uint32_t t = warp_threshold<T, kStatThreads / 32>(sc.maxima, 1, kStatThreads, 0, top, top / 4, kept);
-          if (tid == 0) sc.threshold = threshold_value<T>(t);
-        }
-        __syncthreads();
-      }
-      threshold = *const_cast<volatile float*>(&sc.threshold);
-      if (mx >= threshold) {
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          if (tops[u] < threshold) continue;
-          const int i0 = cut.head + (from + u * kStatThreads + tid) * kSize;
-#pragma unroll
-          for (int i = 0; i < LogitVec<T>::kPairs; ++i) {
-            const float2 x = unpack_pair<T>(now[u], i);
-            if (x.x >= threshold) push(x.x, i0 + 2 * i);
-            if (x.y >= threshold) push(x.y, i0 + 2 * i + 1);
+          if (tid == 0) {
+            sc.first = threshold_value<T>(t);
+            sc.threshold = threshold_value<T>(max(t, kMaskedKey) + (1u << kKeyShift<T>));
           }
         }
+        __syncthreads();
+        threshold = sc.first;
+      } else {
+        threshold = *const_cast<volatile float*>(&sc.threshold);
+      }
+      if (mx >= threshold) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          if (tops[u] >= threshold) {
+            const int at = atomicAdd(&sc.n, 1);
+            if (at < kCandidates) top_smem[at] = candidate(order_key(tops[u]), from + u * kStatThreads + tid);
+          }
       }
       // after 2, 4, 8, ... batches a warp, another each time, raises the threshold; the others go on meanwhile
       if (batch > 0 && ((batch + 1) & batch) == 0 && from + 2 * kBatch < v1 && tid >> 5 == (__ffs(batch + 1) & 7)) {
@@ -388,29 +387,53 @@ __global__ void __launch_bounds__(kStatThreads, 4)
           if ((tid & 31) == 0 && t > order_key(threshold)) *const_cast<volatile float*>(&sc.threshold) = threshold_value<T>(t);
         }
       }
+      ++batch;
     }
-  }
+  };
+  int from = v0;
+  for (; from + kBatch <= v1; from += kBatch) step(std::true_type{}, from);
+  if (from < v1) step(std::false_type{}, from);
   RowStats all = block_merge(st.total(), c2, scratch);
   if (blocks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  // the candidates of the row: this block's, or what every block of the cluster sends to the first one
-  int from_n = 0;
-  uint32_t from_lo = 0;
+  // the row's candidates: this block's, or what every block of the cluster sends to the first one
+  int row_n = 0;
   if constexpr (TOP) {
-    if (single >= threshold) push(single, single_at);
     __syncthreads();
-    int n = sc.n;
-    uint32_t lo = order_key(sc.threshold);
+    const int n = sc.n;
+    const uint32_t lo = order_key(sc.threshold);
     __syncthreads();
     if (n > kCandidates) {
-      lo = 0;
       const int first = part == 0 ? 0 : cut.head + v0 * kSize;
       const int last = part == blocks - 1 ? v : cut.head + v1 * kSize;
-      n = collect_again(row, first, last, top, top_smem, sc);
+      row_n = collect_again(row, first, last, top, top_smem, sc);
+    } else {
+      if (tid < 32) {
+        const int m = select_top<T>(top_smem, n, lo, top, sc);
+        // the least maximum of `top` vectors, from which a value can be among the first
+        uint32_t least = 0xffffffffu;
+        for (int j = tid; j < m; j += 32) least = min(least, candidate_key(sc.kept[j]));
+        least = __reduce_min_sync(0xffffffffu, least);
+        if (tid == 0) sc.kept_n = m, sc.n = 0, sc.first = m < top ? -FLT_MAX : key_value(least);
+      }
+      __syncthreads();
+      const int m = sc.kept_n;
+      const float least = sc.first;
+      auto push = [&](float x, int i) {
+        if (!(x >= least)) return;
+        top_smem[atomicAdd(&sc.n, 1)] = candidate(order_key(x), i);  // (kKept vectors fit, and the single values)
+      };
+      for (int j = tid; j < m * kSize; j += kStatThreads) {
+        const int i = cut.head + static_cast<int>(0xffffffffu - static_cast<uint32_t>(sc.kept[j / kSize])) * kSize + j % kSize;
+        push(to_float<T>(row[i]), i);
+      }
+      push(single, single_at);
+      __syncthreads();
+      row_n = sc.n;
     }
     if (blocks > 1) {
       // this block's first `top`, in any order, behind the other blocks' in the leader's shared memory
       if (tid < 32) {
-        const int m = select_top<T>(top_smem, n, lo, top, sc);
+        const int m = select_top<T>(top_smem, row_n, 0, top, sc);
         int first = 0;
         if (tid == 0) first = atomicAdd(cluster.map_shared_rank(&sc.gathered, 0), m);
         first = __shfl_sync(0xffffffffu, first, 0);
@@ -418,8 +441,6 @@ __global__ void __launch_bounds__(kStatThreads, 4)
         for (int j = tid; j < m; j += 32) lead[j] = sc.kept[j];
       }
     }
-    from_n = n;
-    from_lo = lo;
   }
   if (blocks > 1) {
     if (tid == 0) *cluster.map_shared_rank(&parts[part], 0) = all;
@@ -427,11 +448,11 @@ __global__ void __launch_bounds__(kStatThreads, 4)
     if (part != 0) return;
     all = parts[0];
     for (int b = 1; b < blocks; ++b) all.merge(parts[b], c2);
-    if (TOP) from_n = sc.gathered;
+    if (TOP) row_n = sc.gathered;
   }
   if constexpr (TOP) {
     if (tid < 32) {
-      const int m = select_top<T>(top_smem + (blocks > 1 ? kCandidates : 0), from_n, from_lo, top, sc);
+      const int m = select_top<T>(top_smem + (blocks > 1 ? kCandidates : 0), row_n, 0, top, sc);
       if (tid == 0) sc.kept_n = m;
     }
     __syncthreads();
