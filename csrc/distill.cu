@@ -37,10 +37,21 @@ constexpr int kMaxCluster = 16;  // above 8 the kernel is allowed it explicitly
 
 // What one warp works out for a row and the block then uses.
 struct RowPlan {
-  int read;       // whether the row is read at all
-  float base;     // reference of the pass that writes the gradient
-  float outside;  // A above
+  int read;                             // whether the row is read at all
+  int bad;                              // an id beyond the vocabulary
+  float q_sum, q_rest, q_log_q, q_y;    // sums over the alternatives: q, the rest, q ln q, q y
+  float chosen_m, chosen_s;             // the student's sum over the alternatives
+  float base;                           // reference of the pass that writes the gradient
+  float outside;                        // A above
 };
+
+// Warp 0 says that its part of the block's state is ready (and goes on); the other warps wait for it.
+__device__ __forceinline__ void named_barrier_arrive() {
+  asm volatile("bar.arrive 1, %0;" ::"n"(kDistillThreads) : "memory");
+}
+__device__ __forceinline__ void named_barrier_wait() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kDistillThreads) : "memory");
+}
 
 // A cluster of blocks takes a row, each block a stretch of it. The block's stretch is read from memory once:
 // it is summed as it arrives and kept in shared memory, from where the gradient is formed after the cluster
@@ -58,12 +69,12 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
   namespace cg = cooperative_groups;
   constexpr int kSize = LogitVec<T>::kSize;
   extern __shared__ uint4 smem[];  // GRAD: the stretch (one vector ahead of it, one after); then its bitmap
-  __shared__ RowStats scratch[33];
+  __shared__ JoinScratch<kDistillThreads> scratch;
   __shared__ RowStats parts[kMaxCluster];
   __shared__ int repeats[kMaxCluster];  // whether a block met an id twice
   __shared__ int at[kMaxAlternatives];
   __shared__ float q_s[kMaxAlternatives];
-  __shared__ float d_s[kMaxAlternatives];
+  __shared__ float e_s[kMaxAlternatives];  // 2^y of an alternative; then its gradient
   __shared__ RowPlan plan;
   const cg::cluster_group cluster = cg::this_cluster();
   const int blocks = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
@@ -105,13 +116,11 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
   __syncthreads();
 
   // ---- the teacher's distribution and the student at its tokens (warp 0)
-  int id[kPerLane];
-  float t[kPerLane], x[kPerLane], q[kPerLane], log_q[kPerLane];
-  float shift = 0.f, q_sum = 0.f, q_rest = 0.f;
-  bool any_bad = false;
   if (tid < 32) {
+    int id[kPerLane];
+    float t[kPerLane], x[kPerLane];
     bool bad = false, nan = false, repeated = false;
-    float top = -INFINITY;
+    float shift = -INFINITY;
     int found = 0;
 #pragma unroll
     for (int j = 0; j < kPerLane; ++j) {
@@ -121,12 +130,12 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
         const int64_t raw = static_cast<int64_t>(ids[r * k + a]);
         bad |= raw >= v;
         if (raw >= 0 && raw < v) id[j] = static_cast<int>(raw), t[j] = teacher[r * k + a];
-        at[a] = id[j];
       }
+      at[a] = id[j];
       if (id[j] >= 0) {
         ++found;
         nan |= t[j] != t[j];
-        top = fmaxf(top, t[j]);
+        shift = fmaxf(shift, t[j]);
         x[j] = to_float<T>(row[id[j]]);
         if (id[j] >= first && id[j] < last) {
           const int bit = id[j] - e_vec + 32;
@@ -134,40 +143,61 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
         }
       }
     }
-    any_bad = __any_sync(0xffffffffu, bad);
+    bad = __any_sync(0xffffffffu, bad);
     nan = __any_sync(0xffffffffu, nan);
     found = __reduce_add_sync(0xffffffffu, found);
     repeated = __any_sync(0xffffffffu, repeated);
-    shift = warp_max(top);
+    shift = warp_max(shift);
     if (lane == 0) {
-      plan.read = any_bad || nan || (found > 0 && (tail || shift != -INFINITY));
+      plan.read = bad || nan || (found > 0 && (tail || shift != -INFINITY));
+      plan.bad = bad;
       repeats[part] = repeated;
+      if (bad && part == 0) report_status(status, kOutOfBounds);
     }
-    if (bad && part == 0) report_status(status, kOutOfBounds);
+    named_barrier_arrive();
+    // what of the loss and the gradient does not need the other tokens, while the other warps go on
+    if (tail) shift = 0.f;
+    float q[kPerLane], q_sum = 0.f, q_log_q = 0.f, q_y = 0.f;
+    RowStats chosen;
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) {
+      q[j] = t[j] == -INFINITY ? 0.f : expf(t[j] - shift);
+      q_sum += q[j];
+      if (id[j] >= 0) chosen.m = fmaxf(chosen.m, x[j]);
+    }
+    q_sum = warp_sum(q_sum);
+    chosen.m = warp_max(chosen.m);
+    if (chosen.m == -INFINITY) chosen.m = 0.f;
+    const float log_sum = tail ? 0.f : logf(q_sum);
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) {
+      if (!tail) q[j] /= q_sum;
+      const float y = (x[j] - chosen.m) * c2, e = exp2_fast(y);
+      if (id[j] >= 0) chosen.s += e;
+      if (q[j] != 0.f) q_log_q += q[j] * (t[j] - shift - log_sum), q_y += q[j] * y;
+      q_s[j * 32 + lane] = q[j];
+      e_s[j * 32 + lane] = e;
+    }
+    q_log_q = warp_sum(q_log_q);
+    q_y = warp_sum(q_y);
+    chosen.s = warp_sum(chosen.s);
+    if (lane == 0) {
+      plan.q_sum = tail ? q_sum : 1.f;
+      plan.q_rest = tail ? fmaxf(0.f, 1.f - q_sum) : 0.f;
+      plan.q_log_q = q_log_q;
+      plan.q_y = q_y;
+      plan.chosen_m = chosen.m;
+      plan.chosen_s = chosen.s;
+    }
+    __syncwarp();
+  } else {
+    named_barrier_wait();
   }
-  __syncthreads();
   if (!plan.read) {  // the same for the whole cluster
     if (tid == 0 && part == 0) rows_out[r] = 0.f, weighted[r] = 0.f;
     if (GRAD) write_zeros<T, kDistillThreads>(dlogits + r * v + first, last - first);
     if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     return;
-  }
-  if (tid < 32) {
-    if (tail) shift = 0.f;
-#pragma unroll
-    for (int j = 0; j < kPerLane; ++j) {
-      q[j] = t[j] == -INFINITY ? 0.f : expf(t[j] - shift);
-      q_sum += q[j];
-    }
-    q_sum = warp_sum(q_sum);
-    if (tail) q_rest = fmaxf(0.f, 1.f - q_sum);
-    const float log_sum = tail ? 0.f : logf(q_sum);
-#pragma unroll
-    for (int j = 0; j < kPerLane; ++j) {
-      log_q[j] = t[j] - shift - log_sum;
-      if (!tail) q[j] /= q_sum;
-      q_s[j * 32 + lane] = q[j];
-    }
   }
 
   // ---- the student outside the alternatives: one pass
@@ -212,7 +242,7 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
     const int bit = single_at - e_vec + 32;
     if (!(bitmap[bit >> 5] >> (bit & 31) & 1u)) st.add_one(single, c2);
   }
-  RowStats rest = block_merge(st.total(), c2, scratch);
+  RowStats rest = block_join<kDistillThreads>(st.total(), c2, scratch);
   if (blocks > 1) {
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (tid < blocks) {
@@ -220,69 +250,63 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
       if (tid != part) *cluster.map_shared_rank(&repeats[part], tid) = repeats[part];
     }
     cluster.sync();
-    rest = parts[0];
-    for (int b = 1; b < blocks; ++b) rest.merge(parts[b], c2);
   }
 
   // ---- the row's loss and constants (warp 0 of every block, the same everywhere)
-  const float w = weights != nullptr ? weights[r] : 1.f;
   if (tid < 32) {
-    // repeated ids: the first place of each counts, with the mass of all
-    const bool repeated = __any_sync(0xffffffffu, lane < blocks && repeats[lane] != 0);
+    if (blocks > 1) rest = warp_merge(lane < blocks ? parts[lane] : RowStats(), c2);
     RowStats chosen;
-#pragma unroll
-    for (int j = 0; j < kPerLane; ++j) {
-      bool counts = id[j] >= 0;
-      float mass = q[j];
-      if (repeated) {
-        for (int i = 0; i < j * 32 + lane && counts; ++i) counts = at[i] != id[j];
-        mass = 0.f;
-        for (int i = 0; i < k; ++i) mass += at[i] == id[j] ? q_s[i] : 0.f;
+    chosen.m = plan.chosen_m, chosen.s = plan.chosen_s;
+    const bool repeated = __any_sync(0xffffffffu, lane < blocks && repeats[lane] != 0);
+    if (repeated) {  // the first place of an id counts
+      chosen.s = 0.f;
+      for (int a = lane; a < k; a += 32) {
+        bool counts = at[a] >= 0;
+        for (int i = 0; i < a && counts; ++i) counts = at[i] != at[a];
+        if (counts) chosen.s += e_s[a];
       }
-      d_s[j * 32 + lane] = mass;
-      if (counts) chosen.add(x[j], c2);
+      chosen.s = warp_sum(chosen.s);
     }
-    chosen = warp_merge(chosen, c2);
     RowStats all = chosen;
     all.merge(rest, c2);
-    const float log2s = log2f(all.s);
-    if (rest.s == 0.f) q_rest = 0.f;
-    float loss = 0.f;
-#pragma unroll
-    for (int j = 0; j < kPerLane; ++j)
-      if (q[j] != 0.f) loss += q[j] * (log_q[j] - kLn2 * ((x[j] - all.m) * c2 - log2s));
-    loss = warp_sum(loss);
+    const float log2s = log2f(all.s), q_sum = plan.q_sum, q_rest = rest.s == 0.f ? 0.f : plan.q_rest;
+    // - ln p_k = ln 2 (log2 S + (m - m_a) c2 - y_k)
+    float loss = plan.q_log_q - kLn2 * (plan.q_y + q_sum * ((chosen.m - all.m) * c2 - log2s));
     if (q_rest > 0.f) loss += q_rest * (logf(q_rest) - kLn2 * ((rest.m - all.m) * c2 + log2f(rest.s) - log2s));
     const bool empty = all.s == 0.f;  // every logit is masked: no distribution, no gradient
     if (empty) loss = INFINITY;
-    if (any_bad) loss = NAN;
-    const float mass = tail ? q_sum : 1.f, whole = mass + q_rest, scale = w * inv_t;
+    if (plan.bad) loss = NAN;
+    const float w = weights != nullptr ? weights[r] : 1.f;
+    const float scale = w * inv_t, whole = q_sum + q_rest;
+    const float to_p = chosen.s == 0.f ? 0.f : exp2_fast((chosen.m - all.m) * c2) / all.s;
     float outside = 0.f;
     if (rest.s != 0.f) {
       const float p_rest = exp2_fast((rest.m - all.m) * c2) * rest.s / all.s;
-      const float p_chosen = chosen.s == 0.f ? 0.f : exp2_fast((chosen.m - all.m) * c2) * chosen.s / all.s;
-      outside = scale * (mass * p_rest - q_rest * p_chosen) / rest.s;
+      outside = scale * (q_sum * p_rest - q_rest * (chosen.s * to_p)) / rest.s;
     }
     if (GRAD) {
-#pragma unroll
-      for (int j = 0; j < kPerLane; ++j) {
-        const int a = j * 32 + lane;
-        const float d = empty ? 0.f : scale * (whole * exp2_fast((x[j] - all.m) * c2 - log2s) - d_s[a]);
-        d_s[a] = any_bad ? NAN : d;
+      for (int a = lane; a < k; a += 32) {
+        float mass = q_s[a];
+        if (repeated) {  // ... with the mass of all of its places
+          mass = 0.f;
+          for (int i = 0; i < k; ++i) mass += at[i] == at[a] ? q_s[i] : 0.f;
+        }
+        const float d = empty ? 0.f : scale * (whole * (e_s[a] * to_p) - mass);
+        e_s[a] = plan.bad ? NAN : d;
       }
     }
     if (lane == 0) {
-      plan.base = rest.s == 0.f ? 0.f : rest.m;  // (every other logit is -inf there)
-      plan.outside = any_bad ? NAN : outside;
       if (part == 0) rows_out[r] = loss, weighted[r] = w * loss;
+      plan.base = rest.s == 0.f ? 0.f : rest.m;  // (every other logit is -inf there)
+      plan.outside = plan.bad ? NAN : outside;
     }
   }
   if constexpr (GRAD) {
     __syncthreads();
     T* out = dlogits + r * v;
-    write_gradient<T, kDistillThreads>(kept_values, out + first, last - first, plan.base, c2, plan.outside, 0.f);
+    write_gradient<T, kDistillThreads, true>(kept_values, out + first, last - first, plan.base, c2, plan.outside, 0.f);
     __syncthreads();
-    if (tid < k && at[tid] >= first && at[tid] < last) out[at[tid]] = from_float<T>(d_s[tid]);
+    if (tid < k && at[tid] >= first && at[tid] < last) out[at[tid]] = from_float<T>(e_s[tid]);
   }
 }
 

@@ -95,21 +95,32 @@ __device__ __forceinline__ RowStats warp_merge(RowStats v, float c2) {
   return v;
 }
 
-// Block-wide merge in a fixed order; every thread gets the result. `scratch` holds 33 entries.
-__device__ __forceinline__ RowStats block_merge(RowStats v, float c2, RowStats* scratch) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
-  v = warp_merge(v, c2);
+// Joins the statistics of THREADS threads in a fixed order; every thread gets the result. The maximum first, so
+// that each thread moves its reference once (a tree of pairwise merges costs six times the instructions).
+template <int THREADS>
+struct JoinScratch {
+  float m[THREADS / 32], s[THREADS / 32], w[THREADS / 32];
+};
+template <int THREADS>
+__device__ __forceinline__ RowStats block_join(const RowStats& v, float c2, JoinScratch<THREADS>& sc) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool some = v.s != 0.f;  // (NaN is something)
+  float m = warp_max(some ? v.m : -INFINITY);
+  if (lane == 0) sc.m[warp] = m;
   __syncthreads();
-  if (lane == 0) scratch[warp] = v;
+  m = sc.m[0];
+#pragma unroll
+  for (int i = 1; i < THREADS / 32; ++i) m = fmaxf(m, sc.m[i]);
+  const float d = (v.m - m) * c2, f = exp2_fast(d);
+  const float s = warp_sum(some ? v.s * f : 0.f);
+  const float w = warp_sum(some ? (v.w + v.s * fmaxf(d, kMinExponent)) * f : 0.f);
+  if (lane == 0) sc.s[warp] = s, sc.w[warp] = w;
   __syncthreads();
-  if (warp == 0) {
-    RowStats t;
-    if (lane < warps) t = scratch[lane];
-    t = warp_merge(t, c2);
-    if (lane == 0) scratch[32] = t;
-  }
-  __syncthreads();
-  return scratch[32];
+  RowStats r;
+  r.m = m;
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; ++i) r.s += sc.s[i], r.w += sc.w[i];
+  return r;
 }
 
 // ---- vectors of logits: 16 bytes, 8 or 4 values -----------------------------------------------------
@@ -303,8 +314,8 @@ __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
   }
 }
 
-// (the one rounding of the gradient to the logits' type)
-template <typename T>
+// (the one rounding of the gradient to the logits' type; PLAIN: b is zero)
+template <typename T, bool PLAIN>
 __device__ __forceinline__ uint4 gradient_vec(const uint4& v, float m, float c2, float a, float b) {
   const F2 neg = pair(-m, -m), c = pair(c2, c2), aa = pair(a, a), bb = pair(b, b);
   F2 d[LogitVec<T>::kPairs];
@@ -313,8 +324,12 @@ __device__ __forceinline__ uint4 gradient_vec(const uint4& v, float m, float c2,
     F2 x;
     x.f = unpack_pair<T>(v, i);
     F2 y = mul2(add2(x, neg), c);
-    y = pair(fmaxf(y.f.x, kMinExponent), fmaxf(y.f.y, kMinExponent));
-    d[i] = mul2(pair(exp2_fast(y.f.x), exp2_fast(y.f.y)), fma2(bb, y, aa));
+    if (PLAIN) {
+      d[i] = mul2(pair(exp2_fast(y.f.x), exp2_fast(y.f.y)), aa);
+    } else {
+      y = pair(fmaxf(y.f.x, kMinExponent), fmaxf(y.f.y, kMinExponent));
+      d[i] = mul2(pair(exp2_fast(y.f.x), exp2_fast(y.f.y)), fma2(bb, y, aa));
+    }
   }
   uint4 o;
   if constexpr (sizeof(T) == 2) {
@@ -357,7 +372,7 @@ __device__ __forceinline__ uint4 shift_vec(const uint4& lo, const uint4& hi, int
 // logits may lie at another offset in their 16 bytes: two of their vectors are then joined by a shift, so
 // that both sides move 16 bytes a thread whatever the vocabulary and the pitch are. `row` is in global or
 // shared memory; nothing outside [0, n) is read.
-template <typename T, int THREADS>
+template <typename T, int THREADS, bool PLAIN>
 __device__ __forceinline__ void write_gradient(const T* row, T* out, int n, float m, float c2, float a, float b) {
   constexpr int kSize = LogitVec<T>::kSize, kAhead = 4;
   const RowCut cut = cut_row(out, n);
@@ -379,7 +394,7 @@ __device__ __forceinline__ void write_gradient(const T* row, T* out, int n, floa
         if (i + u * THREADS < cut.vecs) v[u] = x[i + u * THREADS];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        if (i + u * THREADS < cut.vecs) to[i + u * THREADS] = gradient_vec<T>(v[u], m, c2, a, b);
+        if (i + u * THREADS < cut.vecs) to[i + u * THREADS] = gradient_vec<T, PLAIN>(v[u], m, c2, a, b);
     }
     return;
   }
@@ -395,7 +410,7 @@ __device__ __forceinline__ void write_gradient(const T* row, T* out, int n, floa
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
       if (i + u * THREADS < last)
-        to[i + u * THREADS] = gradient_vec<T>(shift_vec(lo[u], hi[u], off * static_cast<int>(sizeof(T))), m, c2, a, b);
+        to[i + u * THREADS] = gradient_vec<T, PLAIN>(shift_vec(lo[u], hi[u], off * static_cast<int>(sizeof(T))), m, c2, a, b);
   }
   // (two vectors at most, one value a thread)
   if (tid < 2 * kSize && cut.vecs > 0) {

@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kStatThreads, 4)
   namespace cg = cooperative_groups;
   constexpr int kSize = LogitVec<T>::kSize;
   extern __shared__ uint64_t top_smem[];  // [kCandidates], then [blocks of the cluster][kKept]
-  __shared__ RowStats scratch[33];
+  __shared__ JoinScratch<kStatThreads> scratch;
   __shared__ RowStats parts[kMaxCluster];
   __shared__ TopScratch sc;
   const cg::cluster_group cluster = cg::this_cluster();
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(kStatThreads, 4)
   int from = v0;
   for (; from + kBatch <= v1; from += kBatch) step(std::true_type{}, from);
   if (from < v1) step(std::false_type{}, from);
-  RowStats all = block_merge(st.total(), c2, scratch);
+  RowStats all = block_join<kStatThreads>(st.total(), c2, scratch);
   if (blocks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   // the row's candidates: this block's, or what every block of the cluster sends to the first one
   int row_n = 0;
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(kStatThreads)
   // T dx_i = 2^y_i (a + b y_i) / S + (d_i terms),  y_i = (x_i - m) c2
   const float a = -(g - h * s.z), b = -h;
   const float scale = inv_t * s.y;
-  write_gradient<T, kStatThreads>(row + first, out + first, n, s.x, c2, scale * a, scale * b);
+  write_gradient<T, kStatThreads, false>(row + first, out + first, n, s.x, c2, scale * a, scale * b);
   __syncthreads();
   // (u and a cancel where p = 1: they are added before anything is scaled)
   auto special = [&](int i, float u) {
