@@ -39,11 +39,18 @@ constexpr int kMaxCluster = 16;  // above 8 the kernel is allowed it explicitly
 struct RowPlan {
   int read;                             // whether the row is read at all
   int bad;                              // an id beyond the vocabulary
+  int copied;                           // whether the bulk copy was started
   float q_sum, q_rest, q_log_q, q_y;    // sums over the alternatives: q, the rest, q ln q, q y
   float chosen_m, chosen_s;             // the student's sum over the alternatives
   float base;                           // reference of the pass that writes the gradient
   float outside;                        // A above
 };
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 
 // Warp 0 says that its part of the block's state is ready (and goes on); the other warps wait for it.
 __device__ __forceinline__ void named_barrier_arrive() {
@@ -53,15 +60,16 @@ __device__ __forceinline__ void named_barrier_wait() {
   asm volatile("bar.sync 1, %0;" ::"n"(kDistillThreads) : "memory");
 }
 
-// A cluster of blocks takes a row, each block a stretch of it. The block's stretch is read from memory once:
-// it is summed as it arrives and kept in shared memory, from where the gradient is formed after the cluster
-// has joined its sums. So a row costs one read and one write, whatever its length (up to the shared memory
-// of 16 blocks). Several blocks on an SM are in different phases, which keeps loads, sums and stores going
-// at once.
+// A cluster of blocks takes a row, each block a stretch of it. With the gradient, the stretch is copied to
+// shared memory by one bulk copy that starts as soon as the row is known to have alternatives; it is summed
+// there, and the gradient is formed there after the cluster has joined its sums. So a row costs one read and
+// one write, whatever its length (up to the shared memory of 16 blocks). Five blocks on an SM are in
+// different phases, which keeps copies, sums and stores going at once: the phases of one block alone are a chain
+// of latencies. Without the gradient a stretch passes through registers.
 //
 // One warp deals with the alternatives, up to four a lane, without block barriers.
 template <typename T, typename I, bool GRAD>
-__global__ void __launch_bounds__(kDistillThreads, 4)
+__global__ void __launch_bounds__(kDistillThreads, 5)
     distill_kernel(const T* __restrict__ logits, RowLayout layout, int v, const I* __restrict__ ids,
                    const float* __restrict__ teacher, int k, const float* __restrict__ weights, float c2, float inv_t,
                    bool tail, float* __restrict__ rows_out, float* __restrict__ weighted, T* __restrict__ dlogits,
@@ -76,6 +84,7 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
   __shared__ float q_s[kMaxAlternatives];
   __shared__ float e_s[kMaxAlternatives];  // 2^y of an alternative; then its gradient
   __shared__ RowPlan plan;
+  __shared__ uint64_t arrived;  // mbarrier of the bulk copy
   const cg::cluster_group cluster = cg::this_cluster();
   const int blocks = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
   if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -102,7 +111,14 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
       if (i < vecs) next[u] = load_stream(base + i);
     }
   };
-  load(0);
+  if (GRAD) {
+    if (tid == 0) {
+      mbar_init(&arrived, 1);
+      fence_barrier_init();
+    }
+  } else {
+    load(0);
+  }
   float single = -INFINITY;
   int single_at = -1;
   if (tid < e_vec - first) single_at = first + tid;
@@ -128,12 +144,25 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
       id[j] = -1, t[j] = -INFINITY, x[j] = -INFINITY;
       if (a < k) {
         const int64_t raw = static_cast<int64_t>(ids[r * k + a]);
+        t[j] = teacher[r * k + a];
         bad |= raw >= v;
-        if (raw >= 0 && raw < v) id[j] = static_cast<int>(raw), t[j] = teacher[r * k + a];
+        if (raw >= 0 && raw < v) id[j] = static_cast<int>(raw);
       }
       at[a] = id[j];
+      found += id[j] >= 0;
+    }
+    if (GRAD) {
+      const bool copy = vecs > 0 && __any_sync(0xffffffffu, found > 0 || bad);
+      if (lane == 0 && copy) {
+        mbar_arrive_expect_tx(&arrived, static_cast<uint32_t>(vecs) * 16);
+        bulk_load(kept, base, static_cast<uint32_t>(vecs) * 16, &arrived);
+      }
+      if (lane == 0) plan.copied = copy;
+    }
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) {
+      if (id[j] < 0) t[j] = -INFINITY;
       if (id[j] >= 0) {
-        ++found;
         nan |= t[j] != t[j];
         shift = fmaxf(shift, t[j]);
         x[j] = to_float<T>(row[id[j]]);
@@ -195,7 +224,10 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
   }
   if (!plan.read) {  // the same for the whole cluster
     if (tid == 0 && part == 0) rows_out[r] = 0.f, weighted[r] = 0.f;
-    if (GRAD) write_zeros<T, kDistillThreads>(dlogits + r * v + first, last - first);
+    if (GRAD) {
+      if (plan.copied) mbar_wait(&arrived, 0, status, kTimeoutFull);
+      write_zeros<T, kDistillThreads>(dlogits + r * v + first, last - first);
+    }
     if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     return;
   }
@@ -203,41 +235,48 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
   // ---- the student outside the alternatives: one pass
   VecSum st;
   const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bitmap);
-  for (int from = 0; from < vecs; from += kDistillThreads * kAhead) {
-    uint4 now[kAhead];
+  auto without_chosen = [&](uint4& x, int i) {
+    const uint32_t chosen = sizeof(T) == 2 ? bytes[i + 4] : bytes[(i >> 1) + 4] >> (4 * (i & 1)) & 15u;
+    if (chosen == 0) return;
+    uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) now[u] = next[u];
-    if (from + kDistillThreads * kAhead < vecs) load(from + kDistillThreads * kAhead);
-    float mx = -INFINITY;
+    for (int e = 0; e < kSize; ++e) {
+      if (!(chosen >> e & 1u)) continue;
+      if constexpr (sizeof(T) == 4) {
+        w[e] = 0xff800000u;
+      } else {
+        const uint32_t masked = std::is_same_v<T, __half> ? 0xfc00u : 0xff80u;
+        w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | masked << 16 : (w[e >> 1] & 0xffff0000u) | masked;
+      }
+    }
+    x = make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  if (GRAD && plan.copied) mbar_wait(&arrived, 0, status, kTimeoutFull);
+  auto step = [&](auto whole, int from) {
+    uint4 now[kAhead];
+    const int mine = decltype(whole)::value ? kAhead : (vecs - from - tid + kDistillThreads - 1) / kDistillThreads;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int i = from + u * kDistillThreads + tid;
-      if (i < vecs) {
-        if (GRAD) kept[i] = now[u];
-        const uint32_t chosen = sizeof(T) == 2 ? bytes[i + 4] : bytes[(i >> 1) + 4] >> (4 * (i & 1)) & 15u;
-        if (chosen != 0) {
-          uint32_t w[4] = {now[u].x, now[u].y, now[u].z, now[u].w};
+      if (!GRAD) now[u] = next[u];
+      else if (u < mine) now[u] = kept[from + u * kDistillThreads + tid];
+    }
+    if (!GRAD && from + kDistillThreads * kAhead < vecs) load(from + kDistillThreads * kAhead);
+    float mx = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < kSize; ++e) {
-            if (!(chosen >> e & 1u)) continue;
-            if constexpr (sizeof(T) == 4) {
-              w[e] = 0xff800000u;
-            } else {
-              const uint32_t masked = std::is_same_v<T, __half> ? 0xfc00u : 0xff80u;
-              w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | masked << 16 : (w[e >> 1] & 0xffff0000u) | masked;
-            }
-          }
-          now[u] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+    for (int u = 0; u < kAhead; ++u)
+      if (u < mine) {
+        without_chosen(now[u], from + u * kDistillThreads + tid);
         const uint4 one[1] = {now[u]};
         mx = fmaxf(mx, vec_max<T, 1>(one));
       }
-    }
     if (mx > st.limit) st.raise(mx, c2);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (from + u * kDistillThreads + tid < vecs) st.add_vec<T>(now[u], c2);
-  }
+      if (u < mine) st.add_vec<T>(now[u], c2);
+  };
+  int from = 0;
+  for (; from + kDistillThreads * kAhead <= vecs; from += kDistillThreads * kAhead) step(std::true_type{}, from);
+  if (from < vecs) step(std::false_type{}, from);
   if (single_at >= 0) {
     const int bit = single_at - e_vec + 32;
     if (!(bitmap[bit >> 5] >> (bit & 31) & 1u)) st.add_one(single, c2);
