@@ -52,6 +52,9 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
+constexpr int kRowsAhead = 128;  // 148 SMs with five blocks hold 92 rows of eight blocks
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // Warp 0 says that its part of the block's state is ready (and goes on); the other warps wait for it.
 __device__ __forceinline__ void named_barrier_arrive() {
   asm volatile("bar.arrive 1, %0;" ::"n"(kDistillThreads) : "memory");
@@ -89,8 +92,8 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
   const int blocks = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
   if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31;
-  const int64_t r = blockIdx.x / blocks;
-  const T* row = logits + layout.offset(r);
+  const int64_t r = blockIdx.x / static_cast<unsigned>(blocks);
+  const T* row = logits + layout.offset(static_cast<uint32_t>(r));
 
   // this block's stretch: vectors [v0, v1) of the row, and the single values at the row's ends
   const RowCut cut = cut_row(row, v);
@@ -111,37 +114,24 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
       if (i < vecs) next[u] = load_stream(base + i);
     }
   };
-  if (GRAD) {
-    if (tid == 0) {
-      mbar_init(&arrived, 1);
-      fence_barrier_init();
-    }
-  } else {
-    load(0);
-  }
+  if (!GRAD) load(0);
   float single = -INFINITY;
   int single_at = -1;
   if (tid < e_vec - first) single_at = first + tid;
   const int after = last - e_vec - vecs * kSize;
   if (tid >= 32 && tid < 32 + after) single_at = last - after + tid - 32;
-  if (single_at >= 0) single = to_float<T>(row[single_at]);
-  if (GRAD && single_at >= 0) kept_values[single_at - first] = row[single_at];
 
-  const int words = (vecs * kSize + kSize + 31) / 32 + 1;
-  for (int i = tid; i < words; i += kDistillThreads) bitmap[i] = 0;
-  __syncthreads();
-
-  // ---- the teacher's distribution and the student at its tokens (warp 0)
+  // ---- the alternatives (warp 0), while the other warps clear the bitmap
+  int id[kPerLane];
+  float t[kPerLane], w = 1.f;
+  bool bad = false;
+  int found = 0;
   if (tid < 32) {
-    int id[kPerLane];
-    float t[kPerLane], x[kPerLane];
-    bool bad = false, nan = false, repeated = false;
-    float shift = -INFINITY;
-    int found = 0;
+    if (weights != nullptr) w = weights[r];
 #pragma unroll
     for (int j = 0; j < kPerLane; ++j) {
       const int a = j * 32 + lane;
-      id[j] = -1, t[j] = -INFINITY, x[j] = -INFINITY;
+      id[j] = -1, t[j] = -INFINITY;
       if (a < k) {
         const int64_t raw = static_cast<int64_t>(ids[r * k + a]);
         t[j] = teacher[r * k + a];
@@ -153,14 +143,38 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
     }
     if (GRAD) {
       const bool copy = vecs > 0 && __any_sync(0xffffffffu, found > 0 || bad);
+      if (lane == 0) {
+        mbar_init(&arrived, 1);
+        fence_barrier_init();
+        fence_proxy_async_smem();
+      }
       if (lane == 0 && copy) {
         mbar_arrive_expect_tx(&arrived, static_cast<uint32_t>(vecs) * 16);
         bulk_load(kept, base, static_cast<uint32_t>(vecs) * 16, &arrived);
       }
       if (lane == 0) plan.copied = copy;
     }
+  } else {
+    const int words = (vecs * kSize + kSize + 31) / 32 + 1;
+    for (int i = tid - 32; i < words; i += kDistillThreads - 32) bitmap[i] = 0;
+    // The alternatives of a row that will start about when this one ends: from memory they would hold up the
+    // row's copy behind all the others' (start to known alternatives: 8100 of a block's 25300 cycles).
+    const int64_t later = r + kRowsAhead;
+    if (part == 0 && tid >= kDistillThreads - 32 && later * blocks < gridDim.x) {
+      if (lane * 16 < k) prefetch_l2(ids + later * k + lane * 16);  // 64 or 128 bytes of ids a lane
+      if (lane * 32 < k) prefetch_l2(teacher + later * k + lane * 32);
+    }
+  }
+  if (single_at >= 0) single = to_float<T>(row[single_at]);
+  if (GRAD && single_at >= 0) kept_values[single_at - first] = row[single_at];
+  __syncthreads();
+
+  if (tid < 32) {
+    float x[kPerLane], shift = -INFINITY;
+    bool nan = false, repeated = false;
 #pragma unroll
     for (int j = 0; j < kPerLane; ++j) {
+      x[j] = -INFINITY;
       if (id[j] < 0) t[j] = -INFINITY;
       if (id[j] >= 0) {
         nan |= t[j] != t[j];
@@ -233,7 +247,7 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
   }
 
   // ---- the student outside the alternatives: one pass
-  VecSum st;
+  VecStats<false> st;
   const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bitmap);
   auto without_chosen = [&](uint4& x, int i) {
     const uint32_t chosen = sizeof(T) == 2 ? bytes[i + 4] : bytes[(i >> 1) + 4] >> (4 * (i & 1)) & 15u;
@@ -252,31 +266,48 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
     x = make_uint4(w[0], w[1], w[2], w[3]);
   };
   if (GRAD && plan.copied) mbar_wait(&arrived, 0, status, kTimeoutFull);
-  auto step = [&](auto whole, int from) {
-    uint4 now[kAhead];
-    const int mine = decltype(whole)::value ? kAhead : (vecs - from - tid + kDistillThreads - 1) / kDistillThreads;
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (!GRAD) now[u] = next[u];
-      else if (u < mine) now[u] = kept[from + u * kDistillThreads + tid];
-    }
-    if (!GRAD && from + kDistillThreads * kAhead < vecs) load(from + kDistillThreads * kAhead);
+  if constexpr (GRAD) {
+    // (the reference is a value of the rest: an alternative far above all of it would round it away)
+    // Warp 0, which has the alternatives to see to, takes no part.
+    uint4 one[1];
     float mx = -INFINITY;
+    const int i0 = tid >= 32 ? tid - 32 : vecs;
+    if (i0 < vecs) {
+      one[0] = kept[i0];
+      without_chosen(one[0], i0);
+      mx = vec_max<T, 1>(one);
+    }
+    st.start(warp_max(mx), c2);
+#pragma unroll 2
+    for (int i = i0; i < vecs; i += kDistillThreads - 32) {
+      one[0] = kept[i];
+      without_chosen(one[0], i);
+      mx = vec_max<T, 1>(one);
+      if (mx > st.limit) st.raise(mx, c2);
+      st.add_vec<T>(one[0], c2);
+    }
+  } else {
+    for (int from = 0; from < vecs; from += kDistillThreads * kAhead) {
+      uint4 now[kAhead];
+      const int mine = (vecs - from - tid + kDistillThreads - 1) / kDistillThreads;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (u < mine) {
-        without_chosen(now[u], from + u * kDistillThreads + tid);
-        const uint4 one[1] = {now[u]};
-        mx = fmaxf(mx, vec_max<T, 1>(one));
-      }
-    if (mx > st.limit) st.raise(mx, c2);
+      for (int u = 0; u < kAhead; ++u) now[u] = next[u];
+      if (from + kDistillThreads * kAhead < vecs) load(from + kDistillThreads * kAhead);
+      float mx = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (u < mine) st.add_vec<T>(now[u], c2);
-  };
-  int from = 0;
-  for (; from + kDistillThreads * kAhead <= vecs; from += kDistillThreads * kAhead) step(std::true_type{}, from);
-  if (from < vecs) step(std::false_type{}, from);
+      for (int u = 0; u < kAhead; ++u)
+        if (u < mine) {
+          without_chosen(now[u], from + u * kDistillThreads + tid);
+          const uint4 one[1] = {now[u]};
+          mx = fmaxf(mx, vec_max<T, 1>(one));
+        }
+      if (from == 0) st.start(warp_max(mx), c2);
+      if (mx > st.limit) st.raise(mx, c2);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (u < mine) st.add_vec<T>(now[u], c2);
+    }
+  }
   if (single_at >= 0) {
     const int bit = single_at - e_vec + 32;
     if (!(bitmap[bit >> 5] >> (bit & 31) & 1u)) st.add_one(single, c2);
@@ -315,7 +346,6 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
     const bool empty = all.s == 0.f;  // every logit is masked: no distribution, no gradient
     if (empty) loss = INFINITY;
     if (plan.bad) loss = NAN;
-    const float w = weights != nullptr ? weights[r] : 1.f;
     const float scale = w * inv_t, whole = q_sum + q_rest;
     const float to_p = chosen.s == 0.f ? 0.f : exp2_fast((chosen.m - all.m) * c2) / all.s;
     float outside = 0.f;
@@ -343,7 +373,7 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
   if constexpr (GRAD) {
     __syncthreads();
     T* out = dlogits + r * v;
-    write_gradient<T, kDistillThreads, true>(kept_values, out + first, last - first, plan.base, c2, plan.outside, 0.f);
+    write_gradient<T, kDistillThreads, true, 1>(kept_values, out + first, last - first, plan.base, c2, plan.outside, 0.f);
     __syncthreads();
     if (tid < k && at[tid] >= first && at[tid] < last) out[at[tid]] = from_float<T>(e_s[tid]);
   }
@@ -384,14 +414,15 @@ __global__ void scale_kernel(T* __restrict__ x, int64_t n, const float* __restri
 
 constexpr int kMostShared = 200 * 1024;
 
-// A row is split so that a block's stretch takes at most about 40 KB (with the gradient: five blocks' worth
-// of shared memory on an SM) or, where rows are few, until every SM holds four blocks; a stretch stays
-// several vectors a thread.
+// A row is split so that a block's stretch takes at most about 40 KB (with the gradient: five blocks' worth of
+// shared memory on an SM) or, where rows are few, until every SM holds four blocks; a stretch stays several
+// vectors a thread. (Without the gradient a finer split costs more, by each block's own start, than the fuller
+// last round of blocks gives: 152 us against 129 for 2000 rows of 151936.)
 int blocks_per_row(int64_t rows, int64_t vocab, int64_t item, bool grad) {
+  const int64_t round = 4 * num_sms(), bytes = vocab * item;
   int blocks = 1;
-  while (grad && blocks < kMaxCluster && vocab * item > 40960 * blocks) blocks *= 2;
-  while (blocks < 8 && rows * blocks * 2 <= 4 * num_sms() && vocab * item / (blocks * 2) >= kDistillThreads * 16)
-    blocks *= 2;
+  while (grad && blocks < kMaxCluster && bytes > 40960 * blocks) blocks *= 2;
+  while (blocks < 8 && rows * blocks * 2 <= round && bytes / (blocks * 2) >= kDistillThreads * 16) blocks *= 2;
   return blocks;
 }
 

@@ -2,7 +2,7 @@
 // score tokens (token_stats.cu) and distil from a teacher's alternatives (distill.cu).
 //
 // With y = x / T every kernel works in base 2: c2 = log2(e) / T, and a row is summarised by
-//     m  the maximum (of the part of the row that was summed)
+//     m  the maximum of what was summed, or a value little below or above it
 //     S  = sum 2^((x - m) c2)
 //     W  = sum 2^((x - m) c2) (x - m) c2
 // so that  ln sum e^y = m / T + ln S  and the entropy is  ln S - ln 2 * W / S. x - m is formed first
@@ -25,11 +25,12 @@ constexpr float kMinExponent = -1.0e4f;
 // One row of a logits tensor whose leading dimensions collapse to two strides (in elements): a slice
 // such as logits[:, :-1] or a padded vocabulary cut to size is read in place.
 struct RowLayout {
-  int64_t inner;     // rows of the inner leading dimension
+  uint32_t inner;  // rows of the inner leading dimension (a 64-bit division would cost a block some 200 cycles)
   int64_t outer_stride;
   int64_t inner_stride;
-  __device__ __forceinline__ int64_t offset(int64_t r) const {
-    return (r / inner) * outer_stride + (r % inner) * inner_stride;
+  __device__ __forceinline__ int64_t offset(uint32_t r) const {
+    const uint32_t o = r / inner;
+    return o * outer_stride + (r - o * inner) * inner_stride;
   }
 };
 
@@ -207,24 +208,36 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   return r;
 }
 
-// A thread's running statistics over batches of vectors, whose maximum is taken first: the reference
-// moves at most once a batch, and inside it a value costs half a subtraction, a product, one exponential,
-// half a sum and half a multiply-add. Every exponent is <= 0, so w only ever adds terms of one sign. (A
-// reference that may lie below the maximum saves the moves, 7 % of the instructions, but then w cancels
-// where one token has nearly all of the mass.) Pairs are summed apart, which also halves the rounding of a
-// long sum.
+// A thread's running statistics over vectors, whose maximum is taken first. The reference m starts at the
+// maximum of the warp's first vectors and moves only when a value passes it by more than 2^kHeadroom, so the
+// common step has no running maximum to carry and, for a value, half a subtraction, half a product, one
+// exponential, half a sum and half a multiply-add. W then has positive terms of at most kHeadroom, beside
+// which it can only be small where the largest weight is 2^kHeadroom times all others': its relative error
+// stays within 2^kHeadroom roundings, 1e-6. (Moving m with every maximum costs some lane of a warp its
+// moves in nine of ten steps, 20 instructions each.) Pairs are summed apart, which also halves the rounding of
+// a long sum.
+constexpr float kHeadroom = 4.f;
+
+template <bool ENTROPY>
 struct VecStats {
-  float m = 0.f, limit = -INFINITY;  // limit = m once a value was seen
+  float m = 0.f, limit = -INFINITY;  // nothing seen: any value sets the reference
   F2 s = pair(0.f, 0.f), w = pair(0.f, 0.f);
 
   __device__ __forceinline__ void raise(float to, float c2) {
     const float d = limit == -INFINITY ? 0.f : (m - to) * c2;
     const float f = exp2_fast(d), dc = fmaxf(d, kMinExponent);
-    w.f.x = (w.f.x + s.f.x * dc) * f;
-    w.f.y = (w.f.y + s.f.y * dc) * f;
+    if (ENTROPY) {
+      w.f.x = (w.f.x + s.f.x * dc) * f;
+      w.f.y = (w.f.y + s.f.y * dc) * f;
+    }
     s.f.x *= f;
     s.f.y *= f;
-    m = limit = to;
+    m = to;
+    limit = to + kHeadroom / c2;
+  }
+  // Before the first values: a reference that is one of the warp's values (none where all are masked).
+  __device__ __forceinline__ void start(float warps_max, float c2) {
+    if (warps_max > limit) raise(warps_max, c2);
   }
   template <typename T>
   __device__ __forceinline__ void add_vec(const uint4& v, float c2) {
@@ -236,54 +249,20 @@ struct VecStats {
       const F2 y = mul2(add2(x, neg), c);
       const F2 e = pair(exp2_fast(y.f.x), exp2_fast(y.f.y));
       s = add2(s, e);
-      w = fma2(e, pair(fmaxf(y.f.x, kMinExponent), fmaxf(y.f.y, kMinExponent)), w);
+      if (ENTROPY) w = fma2(e, pair(fmaxf(y.f.x, kMinExponent), fmaxf(y.f.y, kMinExponent)), w);
     }
   }
   __device__ __forceinline__ void add_one(float x, float c2) {
     if (x > limit) raise(x, c2);
     const float y = (x - m) * c2, e = exp2_fast(y);
     s.f.x += e;
-    w.f.x += e * fmaxf(y, kMinExponent);
+    if (ENTROPY) w.f.x += e * fmaxf(y, kMinExponent);
   }
   __device__ __forceinline__ RowStats total() const {
     RowStats r;
     r.m = m;
     r.s = s.f.x + s.f.y;
     r.w = w.f.x + w.f.y;
-    return r;
-  }
-};
-
-// The same without W.
-struct VecSum {
-  float m = 0.f, limit = -INFINITY;
-  F2 s = pair(0.f, 0.f);
-
-  __device__ __forceinline__ void raise(float to, float c2) {
-    const float f = exp2_fast(limit == -INFINITY ? 0.f : (m - to) * c2);
-    s.f.x *= f;
-    s.f.y *= f;
-    m = limit = to;
-  }
-  template <typename T>
-  __device__ __forceinline__ void add_vec(const uint4& v, float c2) {
-    const F2 neg = pair(-m, -m), c = pair(c2, c2);
-#pragma unroll
-    for (int i = 0; i < LogitVec<T>::kPairs; ++i) {
-      F2 x;
-      x.f = unpack_pair<T>(v, i);
-      const F2 y = mul2(add2(x, neg), c);
-      s = add2(s, pair(exp2_fast(y.f.x), exp2_fast(y.f.y)));
-    }
-  }
-  __device__ __forceinline__ void add_one(float x, float c2) {
-    if (x > limit) raise(x, c2);
-    s.f.x += exp2_fast((x - m) * c2);
-  }
-  __device__ __forceinline__ RowStats total() const {
-    RowStats r;
-    r.m = m;
-    r.s = s.f.x + s.f.y;
     return r;
   }
 };
@@ -371,10 +350,10 @@ __device__ __forceinline__ uint4 shift_vec(const uint4& lo, const uint4& hi, int
 // out[0, n) = gradient of row[0, n), by the threads of one block in vectors that are aligned at `out`. The
 // logits may lie at another offset in their 16 bytes: two of their vectors are then joined by a shift, so
 // that both sides move 16 bytes a thread whatever the vocabulary and the pitch are. `row` is in global or
-// shared memory; nothing outside [0, n) is read.
-template <typename T, int THREADS, bool PLAIN>
+// shared memory, kAhead vectors a thread are loaded at once; nothing outside [0, n) is read.
+template <typename T, int THREADS, bool PLAIN, int kAhead>
 __device__ __forceinline__ void write_gradient(const T* row, T* out, int n, float m, float c2, float a, float b) {
-  constexpr int kSize = LogitVec<T>::kSize, kAhead = 4;
+  constexpr int kSize = LogitVec<T>::kSize;
   const RowCut cut = cut_row(out, n);
   const int tid = threadIdx.x;
   if (tid < cut.head) out[tid] = from_float<T>(gradient_one(to_float<T>(row[tid]), m, c2, a, b));
@@ -441,7 +420,9 @@ inline bool row_layout(const at::Tensor& t, RowLayout& out) {
     else dims.push_back({t.size(i), t.stride(i)});
   }
   if (dims.size() > 2) return false;
-  out.inner = dims.empty() ? 1 : dims.back().first;
+  const int64_t inner = dims.empty() ? 1 : dims.back().first;
+  if (inner > 0x7fffffff) return false;
+  out.inner = static_cast<uint32_t>(std::max<int64_t>(inner, 1));
   out.inner_stride = dims.empty() ? 0 : dims.back().second;
   out.outer_stride = dims.size() == 2 ? dims[0].second : 0;
   return true;

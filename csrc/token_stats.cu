@@ -277,7 +277,21 @@ __global__ void __launch_bounds__(kStatThreads, 4)
   const cg::cluster_group cluster = cg::this_cluster();
   const int blocks = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x;
-  const int64_t r = blockIdx.x / blocks;
+  const int64_t r = blockIdx.x / static_cast<unsigned>(blocks);
+  const T* row = logits + layout.offset(static_cast<uint32_t>(r));
+  const RowCut cut = cut_row(row, v);
+  const int per = (cut.vecs + blocks - 1) / blocks;
+  const int v0 = min(cut.vecs, part * per), v1 = min(cut.vecs, v0 + per);
+  const uint4* base = reinterpret_cast<const uint4*>(row + cut.head);
+  uint4 next[kUnroll];  // on its way while the batch before is summed
+  auto load = [&](int from) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = from + u * kStatThreads + tid;
+      if (i < v1) next[u] = load_stream(base + i);
+    }
+  };
+  load(v0);  // (before the target is known: it arrives at the same time)
   const int64_t target = targets != nullptr ? targets[r] : 0;
   if (targets != nullptr && target == ignore_index) {  // (the whole cluster leaves)
     if (part != 0) return;
@@ -297,30 +311,14 @@ __global__ void __launch_bounds__(kStatThreads, 4)
     if (TOP && tid == 0) sc.gathered = 0;
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   }
-  const T* row = logits + layout.offset(r);
-  const RowCut cut = cut_row(row, v);
-  const int per = (cut.vecs + blocks - 1) / blocks;
-  const int v0 = min(cut.vecs, part * per), v1 = min(cut.vecs, v0 + per);
-  const uint4* base = reinterpret_cast<const uint4*>(row + cut.head);
-
   // the values before the first vector and after the last: one per thread, of two warps
   float single = -INFINITY;
   int single_at = 0;
   if (part == 0 && tid < cut.head) single_at = tid, single = to_float<T>(row[tid]);
   if (part == blocks - 1 && tid >= 32 && tid < 32 + cut.tail)
     single_at = v - cut.tail + tid - 32, single = to_float<T>(row[single_at]);
-  VecStats st;
-  if (single != -INFINITY) st.add_one(single, c2);
+  VecStats<true> st;
 
-  uint4 next[kUnroll];
-  auto load = [&](int from) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int i = from + u * kStatThreads + tid;
-      if (i < v1) next[u] = load_stream(base + i);
-    }
-  };
-  load(v0);
   if constexpr (TOP) {
     // (a place that is taken but not yet written reads as no candidate)
     for (int i = tid; i < kCandidates / 2; i += kStatThreads) reinterpret_cast<uint4*>(top_smem)[i] = make_uint4(0, 0, 0, 0);
@@ -331,22 +329,22 @@ __global__ void __launch_bounds__(kStatThreads, 4)
   // a batch of which every thread has all vectors, or the last one
   auto step = [&](auto whole, int from) {
     uint4 now[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) now[u] = next[u];
     float tops[kUnroll], mx = -INFINITY;
     const int mine = decltype(whole)::value ? kUnroll : (v1 - from - tid + kStatThreads - 1) / kStatThreads;
-    if constexpr (TOP) {
+    if constexpr (TOP || !decltype(whole)::value) {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        now[u] = next[u];
         const uint4 one[1] = {now[u]};
         tops[u] = u < mine ? vec_max<T, 1>(one) : -INFINITY;
         mx = fmaxf(mx, tops[u]);
       }
     } else {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) now[u] = u == 0 || u < mine ? next[u] : now[0];
-      if (mine > 0) mx = vec_max<T, kUnroll>(now);
+      mx = vec_max<T, kUnroll>(now);
     }
     if (from + kBatch < v1) load(from + kBatch);
+    if (batch == 0) st.start(warp_max(mx), c2);
     if (mx > st.limit) st.raise(mx, c2);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
@@ -387,12 +385,13 @@ __global__ void __launch_bounds__(kStatThreads, 4)
           if ((tid & 31) == 0 && t > order_key(threshold)) *const_cast<volatile float*>(&sc.threshold) = threshold_value<T>(t);
         }
       }
-      ++batch;
     }
+    ++batch;
   };
   int from = v0;
   for (; from + kBatch <= v1; from += kBatch) step(std::true_type{}, from);
   if (from < v1) step(std::false_type{}, from);
+  if (single != -INFINITY) st.add_one(single, c2);
   RowStats all = block_join<kStatThreads>(st.total(), c2, scratch);
   if (blocks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   // the row's candidates: this block's, or what every block of the cluster sends to the first one
@@ -500,9 +499,9 @@ __global__ void __launch_bounds__(kStatThreads)
   __shared__ float grad[kMaxTop + 1];
   __shared__ float scratch[32];
   constexpr int kStretch = kStretchBytes / static_cast<int>(sizeof(T));
-  const int64_t r = blockIdx.x / parts;
-  const int first = static_cast<int>(blockIdx.x % parts) * kStretch, n = min(kStretch, v - first);
-  const T* row = logits + layout.offset(r);
+  const int64_t r = blockIdx.x / static_cast<unsigned>(parts);
+  const int first = static_cast<int>(blockIdx.x - static_cast<unsigned>(r) * static_cast<unsigned>(parts)) * kStretch, n = min(kStretch, v - first);
+  const T* row = logits + layout.offset(static_cast<uint32_t>(r));
   T* out = dlogits + r * v;
   const float4 s = saved[r];
   if (s.y == 0.f) {  // ignored, or nothing unmasked
@@ -529,7 +528,7 @@ __global__ void __launch_bounds__(kStatThreads)
   // T dx_i = 2^y_i (a + b y_i) / S + (d_i terms),  y_i = (x_i - m) c2
   const float a = -(g - h * s.z), b = -h;
   const float scale = inv_t * s.y;
-  write_gradient<T, kStatThreads, false>(row + first, out + first, n, s.x, c2, scale * a, scale * b);
+  write_gradient<T, kStatThreads, false, 4>(row + first, out + first, n, s.x, c2, scale * a, scale * b);
   __syncthreads();
   // (u and a cancel where p = 1: they are added before anything is scaled)
   auto special = [&](int i, float u) {
@@ -548,11 +547,15 @@ __global__ void __launch_bounds__(kStatThreads)
   }
 }
 
-// A row is split over a cluster while there are too few rows for every SM to hold four blocks, and while
-// each part is still several batches of loads.
-int blocks_per_row(int64_t rows, int64_t vocab, int64_t item) {
+// A row is split over a cluster while there are too few rows for every SM to hold four blocks and each part is
+// still several batches of loads. Without alternatives, whose parts have to be gathered, it is split further
+// until the blocks come to eight rounds of the SMs, so that a last round that is not full costs little (2001
+// rows of 151936: 3.4 rounds, 122 us; in halves 6.8).
+int blocks_per_row(int64_t rows, int64_t vocab, int64_t item, bool top) {
+  const int64_t round = 4 * num_sms(), bytes = vocab * item;
   int blocks = 1;
-  while (blocks < kMaxCluster && rows * blocks * 2 <= 4 * num_sms() && vocab * item / (blocks * 2) >= kStatThreads * 16)
+  while (blocks < kMaxCluster && ((rows * blocks * 2 <= round && bytes / (blocks * 2) >= kStatThreads * 16) ||
+                                  (!top && rows * blocks < 8 * round && bytes / (blocks * 2) >= 16 * kBatch)))
     blocks *= 2;
   return blocks;
 }
@@ -594,7 +597,7 @@ std::vector<at::Tensor> token_stats_fwd(const at::Tensor& logits_in, const c10::
   if (save) saved = at::empty({rows, 4}, f32);
   if (rows == 0) return {log_probs, entropy, top_ids, top_lp, saved};
   const float c2 = static_cast<float>(1.4426950408889634 / temperature);
-  const int blocks = blocks_per_row(rows, vocab, logits.element_size());
+  const int blocks = blocks_per_row(rows, vocab, logits.element_size(), top > 0);
   with_logit_type(logits.scalar_type(), [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     auto launch = [&](auto kern, size_t smem) {
