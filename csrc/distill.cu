@@ -174,12 +174,10 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
     bool nan = false, repeated = false;
 #pragma unroll
     for (int j = 0; j < kPerLane; ++j) {
-      x[j] = -INFINITY;
       if (id[j] < 0) t[j] = -INFINITY;
       if (id[j] >= 0) {
         nan |= t[j] != t[j];
         shift = fmaxf(shift, t[j]);
-        x[j] = to_float<T>(row[id[j]]);
         if (id[j] >= first && id[j] < last) {
           const int bit = id[j] - e_vec + 32;
           repeated |= (atomicOr(&bitmap[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u) != 0;
@@ -197,8 +195,11 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
       repeats[part] = repeated;
       if (bad && part == 0) report_status(status, kOutOfBounds);
     }
+    __syncwarp();
     named_barrier_arrive();
     // what of the loss and the gradient does not need the other tokens, while the other warps go on
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) x[j] = id[j] >= 0 ? to_float<T>(row[id[j]]) : -INFINITY;
     if (tail) shift = 0.f;
     float q[kPerLane], q_sum = 0.f, q_log_q = 0.f, q_y = 0.f;
     RowStats chosen;
@@ -324,7 +325,7 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
 
   // ---- the row's loss and constants (warp 0 of every block, the same everywhere)
   if (tid < 32) {
-    if (blocks > 1) rest = warp_merge(lane < blocks ? parts[lane] : RowStats(), c2);
+    if (blocks > 1) rest = warp_join(lane < blocks ? parts[lane] : RowStats(), c2);
     RowStats chosen;
     chosen.m = plan.chosen_m, chosen.s = plan.chosen_s;
     const bool repeated = __any_sync(0xffffffffu, lane < blocks && repeats[lane] != 0);

@@ -84,20 +84,19 @@ __device__ __forceinline__ float4 saved_stats(const RowStats& st) {
   return make_float4(st.m, 1.f / st.s, st.w / st.s, 0.f);
 }
 
-__device__ __forceinline__ RowStats warp_merge(RowStats v, float c2) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    RowStats u;
-    u.m = __shfl_xor_sync(0xffffffffu, v.m, o);
-    u.s = __shfl_xor_sync(0xffffffffu, v.s, o);
-    u.w = __shfl_xor_sync(0xffffffffu, v.w, o);
-    v.merge(u, c2);
-  }
-  return v;
+// Joins 32 statistics: the maximum first, so that each moves its reference once (a tree of pairwise merges is a
+// chain of 1700 cycles).
+__device__ __forceinline__ RowStats warp_join(const RowStats& v, float c2) {
+  const bool some = v.s != 0.f;  // (NaN is something)
+  RowStats r;
+  r.m = warp_max(some ? v.m : -INFINITY);
+  const float d = (v.m - r.m) * c2, f = exp2_fast(d);
+  r.s = warp_sum(some ? v.s * f : 0.f);
+  r.w = warp_sum(some ? (v.w + v.s * fmaxf(d, kMinExponent)) * f : 0.f);
+  return r;
 }
 
-// Joins the statistics of THREADS threads in a fixed order; every thread gets the result. The maximum first, so
-// that each thread moves its reference once (a tree of pairwise merges costs six times the instructions).
+// The same for THREADS threads; every thread gets the result.
 template <int THREADS>
 struct JoinScratch {
   float m[THREADS / 32], s[THREADS / 32], w[THREADS / 32];

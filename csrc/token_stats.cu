@@ -445,8 +445,7 @@ __global__ void __launch_bounds__(kStatThreads, 4)
     if (tid == 0) *cluster.map_shared_rank(&parts[part], 0) = all;
     cluster.sync();
     if (part != 0) return;
-    all = parts[0];
-    for (int b = 1; b < blocks; ++b) all.merge(parts[b], c2);
+    all = warp_join((tid & 31) < blocks ? parts[tid & 31] : RowStats(), c2);
     if (TOP) row_n = sc.gathered;
   }
   if constexpr (TOP) {
