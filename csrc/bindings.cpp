@@ -91,10 +91,11 @@ at::Tensor token_stats_bwd(const at::Tensor& logits, const c10::optional<at::Ten
                            const c10::optional<at::Tensor>& g_top);
 // lm_head.cu
 std::vector<at::Tensor> lm_head_stats_fwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
-                                          double temperature, int64_t ignore_index);
+                                          double temperature, int64_t ignore_index, bool save, bool keep);
 at::Tensor lm_head_stats_bwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
-                             const at::Tensor& saved, double temperature, int64_t ignore_index,
-                             const c10::optional<at::Tensor>& g_log_probs, const c10::optional<at::Tensor>& g_entropy);
+                             const at::Tensor& saved, const c10::optional<at::Tensor>& logits, double temperature,
+                             int64_t ignore_index, const c10::optional<at::Tensor>& g_log_probs,
+                             const c10::optional<at::Tensor>& g_entropy);
 // distill.cu
 std::vector<at::Tensor> distill_fwd(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher,
                                     const c10::optional<at::Tensor>& weights, double temperature, bool tail, bool grad);
@@ -109,6 +110,7 @@ void sgd_step(at::Tensor& param, const at::Tensor& grad, const c10::optional<at:
 at::Tensor grad_sq_norm(const at::Tensor& g);
 // gemm_tc.cu
 void gemm(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, bool a_mn, bool b_mn, bool accumulate);
+void gemm_split_k(const at::Tensor& a, const at::Tensor& b, at::Tensor& out);
 void grouped_gemm_m(const at::Tensor& a, const at::Tensor& b, const at::Tensor& group_off,
                     const at::Tensor& group_rows, at::Tensor& out, bool b_mn, int64_t max_rows);
 void grouped_gemm_k(const at::Tensor& a, const at::Tensor& b, const at::Tensor& group_off,
@@ -235,6 +237,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sgd_step", &tdsv::sgd_step);
   m.def("grad_sq_norm", &tdsv::grad_sq_norm);
   m.def("gemm", &tdsv::gemm);
+  m.def("gemm_split_k", &tdsv::gemm_split_k, "a [M, K] b [K, N] with K cut into slices that fill the SMs evenly");
   m.def("grouped_gemm_m", &tdsv::grouped_gemm_m);
   m.def("grouped_gemm_k", &tdsv::grouped_gemm_k);
   m.def("mhc_sinkhorn_fwd", &tdsv::mhc_sinkhorn_fwd);

@@ -19,6 +19,8 @@
 //            of A and C (rows_g a multiple of 128) and uses B[g] of a [G, N, K] (or [G, K, N]) tensor
 //   kGroupK  expert-grouped along K (MoE weight gradients): C[g] = A_g^T B_g where A_g, B_g are rows
 //            [off_g, off_g + rows_g) of [R, M] and [R, N] tensors (both MN-major).
+//   kSplitK  one problem whose K extent is cut into slices of whole k-blocks: C[s] = A[:, slice s] B[:, slice s]^T,
+//            for products with fewer output tiles than SMs can share evenly (gemm_split_k adds the slices)
 // Group sizes live on the device, so no host synchronisation is needed between routing and GEMMs.
 //
 // Every mbarrier wait is bounded (see common.cuh); a timeout records a status code and the CTA
@@ -36,12 +38,13 @@ constexpr int BK = 64;  // 64 bf16 = 128 bytes = one swizzle atom row
 constexpr int kThreads = 192;
 constexpr int kMaxGroups = 512;
 
-enum Mode : int { kDense = 0, kGroupM = 1, kGroupK = 2 };
+enum Mode : int { kDense = 0, kGroupM = 1, kGroupK = 2, kSplitK = 3 };
 enum Epi : int { kStoreBF16 = 0, kStoreF32 = 1, kAccumF32 = 2 };
 
 struct Params {
   int M, N, K;           // dense problem (kGroupM: N, K used; kGroupK: M, N used)
-  int num_groups;
+  int num_groups;        // (kSplitK: slices)
+  int slice_k;           // kSplitK: K extent of a slice, a multiple of BK
   const int* group_off;  // [G] start row of each group
   const int* group_rows; // [G] rows of each group (kGroupM: multiple of 128; kGroupK: multiple of 64)
   void* C;
@@ -110,6 +113,18 @@ __device__ __forceinline__ bool tile_info(const Params& p, const int* prefix, in
     ti.k_begin = 0;
     ti.k_len = p.K;
     ti.m_limit = p.group_off[g] + p.group_rows[g];
+  } else if (MODE == kSplitK) {
+    const int m_blocks = (p.M + BM - 1) / BM;
+    const int per_slice = m_blocks * n_blocks;
+    const int s = tile / per_slice, local = tile % per_slice;
+    const int mb = m_blocks <= n_blocks ? local % m_blocks : local / n_blocks;
+    const int nb = m_blocks <= n_blocks ? local / m_blocks : local % n_blocks;
+    ti.group = s;
+    ti.m0 = mb * BM;
+    ti.n0 = nb * BN;
+    ti.k_begin = s * p.slice_k;
+    ti.k_len = min(p.slice_k, p.K - ti.k_begin);
+    ti.m_limit = p.M;
   } else {
     const int m_blocks = (p.M + BM - 1) / BM;
     const int per_group = m_blocks * n_blocks;
@@ -179,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (threadIdx.x == 32) {
     const int n_blocks = (p.N + BN - 1) / BN;
     const int m_blocks = (p.M + BM - 1) / BM;
-    *total_tiles_s = MODE == kDense ? m_blocks * n_blocks : m_blocks * n_blocks * p.num_groups;
+    *total_tiles_s = MODE == kDense ? m_blocks * n_blocks : m_blocks * n_blocks * p.num_groups;  // (or slices)
   }
   tc_fence_before();
   __syncthreads();
@@ -317,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0 && ti.n0 + c0 < p.N && row0 < ti.m_limit) {
           const int x = ti.n0 + c0;
-          if (MODE == kGroupK) {
+          if (MODE == kGroupK || MODE == kSplitK) {
             if (p.epi == kAccumF32) tma_reduce_add_3d(&tma_c, stage_u32, x, row0, ti.group);
             else tma_store_3d(&tma_c, stage_u32, x, row0, ti.group);
           } else {
@@ -462,6 +477,8 @@ void dispatch(bool a_mn, bool b_mn, int bn, const CUtensorMap& ma, const CUtenso
     TDSV_GEMM_CASE(true, true, 128)
     TDSV_GEMM_CASE(true, false, 256)
     TDSV_GEMM_CASE(true, false, 128)
+  } else if constexpr (MODE == kSplitK) {
+    TDSV_GEMM_CASE(false, true, 256)
   } else if constexpr (MODE == kGroupM) {
     TDSV_GEMM_CASE(false, false, 256)
     TDSV_GEMM_CASE(false, false, 128)
@@ -520,6 +537,66 @@ void gemm(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, bool a_mn, 
   }
   const int tiles = ((M + BM - 1) / BM) * ((N + bn - 1) / bn);
   dispatch<kDense>(a_mn, b_mn, bn, ma, mb, mc, p, tiles);
+}
+
+namespace {
+
+// out = the slices' sum, in slice order, rounded once.
+__global__ void add_slices_kernel(const float4* __restrict__ part, int slices, int64_t n, uint2* __restrict__ out) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  float4 s = part[i];
+  for (int k = 1; k < slices; ++k) {
+    const float4 v = part[k * n + i];
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(s.x, s.y), hi = __floats2bfloat162_rn(s.z, s.w);
+  out[i] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+
+}  // namespace
+
+// out[M, N] = A[M, K] B[K, N], bf16, where K is long and the output tiles are few: K is cut so that the tiles of all
+// slices fill the SMs evenly, the slices are accumulated apart in fp32 and added in order. (1023 x 5120 x 129280,
+// the hidden states' gradient of an LM head: 160 tiles take two rounds of 148 SMs, 1805 us.)
+void gemm_split_k(const at::Tensor& a, const at::Tensor& b, at::Tensor& out) {
+  check_operand(a, "a");
+  check_cuda_tensor(b, "b");
+  check_cuda_tensor(out, "out");
+  TDSV_CHECK(a.dim() == 2 && b.dim() == 2 && out.dim() == 2 && a.size(1) == b.size(0) && out.size(0) == a.size(0) &&
+                 out.size(1) == b.size(1),
+             "gemm_split_k: a [M, K], b [K, N], out [M, N]");
+  TDSV_CHECK(out.scalar_type() == at::kBFloat16 && out.size(1) % 8 == 0, "gemm_split_k: bf16 out, N a multiple of 8");
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(1);
+  if (M == 0) return;
+  // the rounds of a slice's tiles over the SMs, against writing and reading its sums
+  const int64_t tiles = ((M + BM - 1) / BM) * ((N + 255) / 256), sms = num_sms();
+  const double round_us = 2.0 * BM * 256 * K * sms / 1.4e9, slice_us = M * N * 8 / 6.5e6;
+  int slices = 1;
+  double best = 1e30;
+  for (int s = 1; s <= 16 && K / s >= 16 * BK; ++s) {
+    const double us = static_cast<double>((tiles * s + sms - 1) / sms) * round_us / s + (s > 1 ? s * slice_us + 5.0 : 0.0);
+    if (us < best) best = us, slices = s;
+  }
+  if (slices == 1 || N < 256) return gemm(a, b, out, false, true, false);
+  c10::cuda::CUDAGuard guard(a.device());
+  const int64_t slice_k = ((K + slices - 1) / slices + BK - 1) / BK * BK;
+  slices = static_cast<int>((K + slice_k - 1) / slice_k);
+  auto part = at::empty({slices, M, N}, out.options().dtype(at::kFloat));
+  const CUtensorMap ma = make_map(a, BM), mb = make_map(b, BK), mc = make_out_map(part);
+  Params p{};
+  p.M = static_cast<int>(M);
+  p.N = static_cast<int>(N);
+  p.K = static_cast<int>(K);
+  p.num_groups = slices;
+  p.slice_k = static_cast<int>(slice_k);
+  p.epi = kStoreF32;
+  p.status = status_word_ptr();
+  dispatch<kSplitK>(false, true, 256, ma, mb, mc, p, static_cast<int>(tiles * slices));
+  const int64_t n = M * N / 4;
+  add_slices_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream()>>>(
+      reinterpret_cast<const float4*>(part.data_ptr<float>()), slices, n, static_cast<uint2*>(out.data_ptr()));
+  TDSV_LAUNCH_CHECK();
 }
 
 // Expert-grouped along M: out[off_g : off_g + rows_g] = A[off_g : ...] * B[g]^T.

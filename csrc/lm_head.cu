@@ -8,6 +8,13 @@
 //               from the fp32 accumulators and a, b from the saved row statistics (logits rounded to bf16 first
 //               would put an error of 2^-9 |x| into ln p). dX feeds the plain GEMMs of dhidden and dweight.
 //
+// Where a backward will follow and the fp32 logits fit the caller's budget, the statistics' epilogue stores them
+// as well (behind the MMAs, which are what the kernel waits for), and the gradient is one pass over them: for
+// 1023 x 5120 x 129280 that replaces a product of 1010 us.
+//
+// When only scores are wanted, rows without a target are left out: the others are gathered first and their
+// number stays on the device.
+//
 // Roles inside a CTA (192 threads, one CTA per SM): warp 0 feeds a ring of 128B-swizzled stages by TMA,
 // one thread of warp 1 issues the MMAs into a double-buffered accumulator, warps 2-5 are the epilogue. A
 // thread of the epilogue owns one row (its TMEM lane), so the reduction needs no shuffles. Every wait is
@@ -30,8 +37,12 @@ constexpr int kStageB = BN * BK * 2;
 constexpr int kStageC = 32 * 128;
 constexpr int kSmemBytes = kStages * (kStageA + kStageB) + 4 * kStageC + 1024 /*align*/ + 256 /*barriers*/;
 
+enum Epilogue : int { kStats = 0, kStatsKeep = 1, kGrad = 2 };
+
 struct HeadParams {
   int M, N, K;
+  int bn;                  // columns of a tile (kStats: any multiple of 16 up to BN, to share few tiles evenly)
+  const int* rows;         // device: the rows that are there, or null: M
   float c2, inv_t;
   const int64_t* targets;  // [M]
   // statistics
@@ -48,16 +59,16 @@ struct HeadParams {
 struct HeadTile {
   int m0, n0, nb;
 };
-__device__ __forceinline__ bool head_tile(const HeadParams& p, int tile, HeadTile& t) {
-  const int m_blocks = (p.M + BM - 1) / BM, n_blocks = (p.N + BN - 1) / BN;
+__device__ __forceinline__ bool head_tile(const HeadParams& p, int rows, int tile, HeadTile& t) {
+  const int m_blocks = (rows + BM - 1) / BM, n_blocks = (p.N + p.bn - 1) / p.bn;
   if (tile >= m_blocks * n_blocks) return false;
   t.nb = tile / m_blocks;
   t.m0 = (tile % m_blocks) * BM;
-  t.n0 = t.nb * BN;
+  t.n0 = t.nb * p.bn;
   return true;
 }
 
-template <bool GRAD>
+template <int EPI>
 __global__ void __launch_bounds__(kThreads, 1)
     lm_head_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                    const __grid_constant__ CUtensorMap tma_c, const HeadParams p) {
@@ -74,6 +85,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* aborted = reinterpret_cast<int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rows = p.rows != nullptr ? min(*p.rows, p.M) : p.M;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
@@ -102,13 +114,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       tma_prefetch_desc(&tma_b);
       uint32_t it = 0;
       HeadTile t;
-      for (int tile = blockIdx.x; head_tile(p, tile, t); tile += gridDim.x) {
+      for (int tile = blockIdx.x; head_tile(p, rows, tile, t); tile += gridDim.x) {
         for (int kb = 0; kb < kb_count; ++kb, ++it) {
           const int s = it % kStages;
           const uint32_t ph = (it / kStages) & 1;
           if (!mbar_wait(&empty[s], ph ^ 1, p.status, kTimeoutEmpty)) { *aborted = 1; break; }
           if (*(volatile int*)aborted) break;
-          mbar_arrive_expect_tx(&full[s], kStageA + kStageB);
+          mbar_arrive_expect_tx(&full[s], kStageA + p.bn * BK * 2);
           tma_load_2d(smem_a + s * kStageA, &tma_a, &full[s], kb * BK, t.m0);
           tma_load_2d(smem_b + s * kStageB, &tma_b, &full[s], kb * BK, t.n0);
         }
@@ -117,10 +129,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t idesc = make_idesc_bf16(BM, BN, false, false);
+      const uint32_t idesc = make_idesc_bf16(BM, p.bn, false, false);
       uint32_t it = 0, tcount = 0;
       HeadTile t;
-      for (int tile = blockIdx.x; head_tile(p, tile, t); tile += gridDim.x, ++tcount) {
+      for (int tile = blockIdx.x; head_tile(p, rows, tile, t); tile += gridDim.x, ++tcount) {
         const int buf = tcount & 1;
         if (!mbar_wait(&tempty[buf], ((tcount >> 1) & 1) ^ 1, p.status, kTimeoutAccumFree)) { *aborted = 1; break; }
         tc_fence_after();
@@ -146,17 +158,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* stage = smem_c + quarter * kStageC;
     uint32_t tcount = 0;
     HeadTile t;
-    for (int tile = blockIdx.x; head_tile(p, tile, t); tile += gridDim.x, ++tcount) {
+    for (int tile = blockIdx.x; head_tile(p, rows, tile, t); tile += gridDim.x, ++tcount) {
       const int buf = tcount & 1;
       const int row = t.m0 + quarter * 32 + lane;
-      const bool live = row < p.M;
+      const bool live = row < rows;
       const int64_t target = live ? p.targets[row] : -1;
       // the target's column inside this tile, or a column no chunk has
       const int64_t rel = target - t.n0;
-      const int hit = rel >= 0 && rel < BN && target < p.N ? static_cast<int>(rel) : -1;
+      const int hit = rel >= 0 && rel < p.bn && target < p.N ? static_cast<int>(rel) : -1;
       // dx = 2^y (a + b y) with 1 / (S T) inside a and b; a row without a gradient has y = -inf throughout
       float m = INFINITY, a = 0.f, b = 0.f, bonus = 0.f;
-      if (GRAD && live && target != p.ignore_index) {
+      if (EPI == kGrad && live && target != p.ignore_index) {
         const float4 sv = p.saved[row];
         if (sv.y != 0.f) {
           const float g = p.g != nullptr && target >= 0 && target < p.N ? p.g[row] : 0.f;
@@ -165,21 +177,36 @@ __global__ void __launch_bounds__(kThreads, 1)
           m = sv.x;
           a = -scale * (g - h * sv.z);
           b = -scale * h;
-          bonus = p.inv_t * g;
+          bonus = __fmul_rn(p.inv_t, g);  // (rounded as in a: the two cancel where p = 1)
         }
       }
       if (!mbar_wait(&tfull[buf], (tcount >> 1) & 1, p.status, kTimeoutAccum)) { *aborted = 1; break; }
       tc_fence_after();
       const uint32_t t_addr = tmem_base + buf * BN + (static_cast<uint32_t>(quarter * 32) << 16);
-      if (!GRAD) {
+      if (EPI != kGrad) {
         RowStats st;
 #pragma unroll 1
         for (int c0 = 0; c0 < BN; c0 += 32) {
-          const int left = p.N - t.n0 - c0;  // columns of this chunk inside the vocabulary
+          const int left = min(p.N - t.n0, p.bn) - c0;  // columns of this chunk inside the tile
           if (left <= 0) break;
           uint32_t raw[32];
           tmem_ld_32x32b_x32(t_addr + c0, raw);
           tmem_ld_wait();
+          if (EPI == kStatsKeep) {
+            if (lane == 0) bulk_wait_group_read0();  // the last chunk's store has read the staging buffer
+            __syncwarp();
+            uint8_t* my_row = stage + lane * 128;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              *reinterpret_cast<uint4*>(my_row + ((q ^ (lane & 7)) << 4)) =
+                  make_uint4(raw[4 * q], raw[4 * q + 1], raw[4 * q + 2], raw[4 * q + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && t.m0 + quarter * 32 < p.M) {
+              tma_store_2d(&tma_c, smem_u32(stage), t.n0 + c0, t.m0 + quarter * 32);
+              bulk_commit_group();
+            }
+          }
           float top = -INFINITY;
           if (left < 32) {
 #pragma unroll
@@ -255,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty[buf]);
     }
-    if (GRAD && lane == 0) bulk_wait_group0();
+    if (EPI != kStats && lane == 0) bulk_wait_group0();
     __syncwarp();
   }
   tc_fence_before();
@@ -266,57 +293,156 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the column tiles of each row: 32 rows a block, 16 slices of the tiles, merged in slice order.
-constexpr int kJoinSlices = 16;
-__global__ void __launch_bounds__(32 * kJoinSlices)
-    lm_head_join_kernel(const float* __restrict__ part_m, const float* __restrict__ part_s,
-                        const float* __restrict__ part_w, const float* __restrict__ target_logit,
-                        const int64_t* __restrict__ targets, int64_t ignore_index, int rows, int vocab, int tiles,
-                        float c2, float* __restrict__ log_probs, float* __restrict__ entropy,
-                        float4* __restrict__ saved, int* status) {
-  __shared__ RowStats part[kJoinSlices][32];
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const int r = blockIdx.x * 32 + lane;
-  RowStats st;
-  if (r < rows) {
+// Joins the column tiles of each row: 8 rows a block, 64 slices of the tiles. The largest reference first, so that
+// no term waits for the one before; slices are added in slice order.
+constexpr int kJoinRows = 8, kJoinSlices = 64;
+__global__ void __launch_bounds__(kJoinRows * kJoinSlices)
+    lm_head_join_kernel(const HeadParams p, const int* __restrict__ where, int tiles, float* __restrict__ log_probs,
+                        float* __restrict__ entropy, float4* __restrict__ saved) {
+  __shared__ float part[2][kJoinSlices][kJoinRows];
+  const int lane = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows;
+  const int i = blockIdx.x * kJoinRows + lane;
+  const bool live = i < (p.rows != nullptr ? min(*p.rows, p.M) : p.M);
+  float m = -INFINITY;
+  if (live)
     for (int t = slice; t < tiles; t += kJoinSlices) {
-      const int64_t o = static_cast<int64_t>(t) * rows + r;
-      RowStats u;
-      u.m = part_m[o], u.s = part_s[o], u.w = part_w[o];
-      st.merge(u, c2);
+      const int64_t o = static_cast<int64_t>(t) * p.M + i;
+      if (p.part_s[o] != 0.f) m = fmaxf(m, p.part_m[o]);
     }
-  }
-  part[slice][lane] = st;
+  part[0][slice][lane] = m;
   __syncthreads();
-  if (slice != 0 || r >= rows) return;
-  for (int s = 1; s < kJoinSlices; ++s) st.merge(part[s][lane], c2);
-  const int64_t target = targets[r];
+  for (int s = 0; s < kJoinSlices; ++s) m = fmaxf(m, part[0][s][lane]);
+  __syncthreads();
+  float sum = 0.f, w = 0.f;
+  if (live)
+    for (int t = slice; t < tiles; t += kJoinSlices) {
+      const int64_t o = static_cast<int64_t>(t) * p.M + i;
+      const float s = p.part_s[o];
+      if (s == 0.f) continue;
+      const float d = (p.part_m[o] - m) * p.c2, f = exp2_fast(d);
+      sum += s * f;
+      w += (p.part_w[o] + s * fmaxf(d, kMinExponent)) * f;
+    }
+  part[0][slice][lane] = sum;
+  part[1][slice][lane] = w;
+  __syncthreads();
+  if (slice != 0 || !live) return;
+  RowStats st;
+  st.m = m;
+  for (int s = 0; s < kJoinSlices; ++s) st.s += part[0][s][lane], st.w += part[1][s][lane];
+  const int64_t target = p.targets[i];
+  const int r = where != nullptr ? where[i] : i;
   float lp = 0.f, ent = 0.f;
-  if (target != ignore_index) {
+  if (target != p.ignore_index) {
     const float log2s = log2f(st.s);
     ent = st.s == 0.f ? 0.f : kLn2 * (log2s - st.w / st.s);
-    if (target >= 0 && target < vocab) {
-      lp = st.s == 0.f ? -INFINITY : kLn2 * ((target_logit[r] - st.m) * c2 - log2s);
+    if (target >= 0 && target < p.N) {
+      lp = st.s == 0.f ? -INFINITY : kLn2 * ((p.target_logit[i] - st.m) * p.c2 - log2s);
     } else {
       lp = NAN;
-      report_status(status, kOutOfBounds);
+      report_status(p.status, kOutOfBounds);
     }
   }
   log_probs[r] = lp;
   entropy[r] = ent;
-  saved[r] = saved_stats(st);
+  if (saved != nullptr) saved[r] = saved_stats(st);
+}
+
+// The rows with a target, in order: where[i] is row i's place, with its target; the others' results are zeros.
+__global__ void __launch_bounds__(1024)
+    lm_head_rows_kernel(const int64_t* __restrict__ targets, int rows, int64_t ignore_index, int* __restrict__ where,
+                        int64_t* __restrict__ kept_targets, int* __restrict__ count, float* __restrict__ log_probs,
+                        float* __restrict__ entropy) {
+  __shared__ int sums[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int base = 0;
+  for (int r0 = 0; r0 < rows; r0 += 1024) {
+    const int r = r0 + static_cast<int>(threadIdx.x);
+    const int64_t t = r < rows ? targets[r] : ignore_index;
+    const bool keep = t != ignore_index;
+    const uint32_t mask = __ballot_sync(0xffffffffu, keep);
+    if (lane == 0) sums[warp] = __popc(mask);
+    __syncthreads();
+    int before = base, all = 0;
+    for (int w = 0; w < 32; ++w) {
+      if (w < warp) before += sums[w];
+      all += sums[w];
+    }
+    if (keep) {
+      const int at = before + __popc(mask & ((1u << lane) - 1u));
+      where[at] = r;
+      kept_targets[at] = t;
+    } else if (r < rows) {
+      log_probs[r] = 0.f;
+      entropy[r] = 0.f;
+    }
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *count = base;
+}
+__global__ void lm_head_gather_kernel(const uint4* __restrict__ hidden, const int* __restrict__ where,
+                                      const int* __restrict__ count, int vecs, uint4* __restrict__ out) {
+  const int i = blockIdx.x;
+  if (i >= *count) return;
+  const int64_t from = static_cast<int64_t>(where[i]) * vecs, to = static_cast<int64_t>(i) * vecs;
+  for (int j = threadIdx.x; j < vecs; j += blockDim.x) out[to + j] = hidden[from + j];
+}
+
+// The gradient from kept logits: 8 values a thread, rows of both padded to 8 values.
+constexpr int kKeptThreads = 256, kKeptVecs = 4;
+__global__ void __launch_bounds__(kKeptThreads)
+    lm_head_kept_kernel(const float4* __restrict__ logits, const HeadParams p, int parts, int vecs,
+                        uint4* __restrict__ dlogits) {
+  const int r = static_cast<int>(blockIdx.x / static_cast<unsigned>(parts));
+  const int first = static_cast<int>(blockIdx.x - static_cast<unsigned>(r) * static_cast<unsigned>(parts)) * kKeptThreads *
+                    kKeptVecs;
+  const int64_t target = p.targets[r];
+  const float4 sv = p.saved[r];
+  uint4* out = dlogits + static_cast<int64_t>(r) * vecs;
+  const float4* row = logits + static_cast<int64_t>(r) * vecs * 2;
+  const bool live = target != p.ignore_index && sv.y != 0.f;
+  const bool has_target = target >= 0 && target < p.N;
+  const float g = live && has_target && p.g != nullptr ? p.g[r] : 0.f, h = live && p.h != nullptr ? p.h[r] * kLn2 : 0.f;
+  const float scale = p.inv_t * sv.y, a = -scale * (g - h * sv.z), b = -scale * h;
+  const float bonus = __fmul_rn(p.inv_t, g);  // (rounded as in a: the two cancel where p = 1)
+#pragma unroll
+  for (int u = 0; u < kKeptVecs; ++u) {
+    const int i = first + u * kKeptThreads + static_cast<int>(threadIdx.x);
+    if (i >= vecs) return;
+    uint4 o = make_uint4(0, 0, 0, 0);
+    if (live) {
+      const float4 lo = row[2 * i], hi = row[2 * i + 1];
+      float d[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = gradient_one(d[e], sv.x, p.c2, a, b);
+      const int64_t hit = has_target ? target - 8 * static_cast<int64_t>(i) : -1;
+      if (hit >= 0 && hit < 8) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e == hit) d[e] += bonus;
+      }
+      o.x = pack_pair<__nv_bfloat16>(d[0], d[1]);
+      o.y = pack_pair<__nv_bfloat16>(d[2], d[3]);
+      o.z = pack_pair<__nv_bfloat16>(d[4], d[5]);
+      o.w = pack_pair<__nv_bfloat16>(d[6], d[7]);
+    }
+    out[i] = o;
+  }
 }
 
 CUtensorMap head_map(const at::Tensor& t, int64_t row_stride, int box_rows) {
   bind_primary_context();
-  TDSV_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (row_stride * 2) % 16 == 0,
+  const bool bf16 = t.scalar_type() == at::kBFloat16;
+  const int item = bf16 ? 2 : 4;
+  TDSV_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (row_stride * item) % 16 == 0,
              "linear_token_statistics: rows must start on 16-byte boundaries");
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(t.size(1)), static_cast<cuuint64_t>(t.size(0))};
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_stride) * 2};
-  cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_stride) * item};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / item), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
   CUtensorMap map;
-  const CUresult r = encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, t.data_ptr(), dims, strides, box, estr,
+  const CUresult r = encode_fn()(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, t.data_ptr(), dims, strides, box, estr,
                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", static_cast<int>(r));
@@ -338,19 +464,34 @@ void check_head(const at::Tensor& hidden, const at::Tensor& weight, const at::Te
              "linear_token_statistics: size");
 }
 
-template <bool GRAD>
+// Columns of a tile: 256, unless the tiles are so few that their last round over the SMs would be mostly empty
+// (one row block of 151936 columns: 594 tiles are 4.01 rounds of 148; of 208 columns 731 are 4.94).
+int tile_columns(int64_t rows, int64_t vocab) {
+  const int64_t m_blocks = (rows + BM - 1) / BM, sms = num_sms();
+  if (m_blocks * ((vocab + BN - 1) / BN) >= 8 * sms) return BN;
+  int best = BN;
+  int64_t least = INT64_MAX;
+  for (int bn = BN; bn >= 96; bn -= 16) {
+    const int64_t columns = (m_blocks * ((vocab + bn - 1) / bn) + sms - 1) / sms * bn;
+    if (columns < least) least = columns, best = bn;
+  }
+  return best;
+}
+
+template <int EPI>
 void launch_head(const at::Tensor& hidden, const at::Tensor& weight, const CUtensorMap& mc, HeadParams& p) {
-  auto kern = lm_head_kernel<GRAD>;
+  auto kern = lm_head_kernel<EPI>;
   static std::once_flag once;
   std::call_once(once, [&] {
     TDSV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
   });
-  const CUtensorMap ma = head_map(hidden, hidden.size(1), BM), mb = head_map(weight, weight.size(1), BN);
   p.M = static_cast<int>(hidden.size(0));
   p.N = static_cast<int>(weight.size(0));
   p.K = static_cast<int>(hidden.size(1));
+  p.bn = EPI == kStats ? tile_columns(p.M, p.N) : BN;
   p.status = status_word_ptr();
-  const int64_t tiles = static_cast<int64_t>((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
+  const CUtensorMap ma = head_map(hidden, hidden.size(1), BM), mb = head_map(weight, weight.size(1), p.bn);
+  const int64_t tiles = static_cast<int64_t>((p.M + BM - 1) / BM) * ((p.N + p.bn - 1) / p.bn);
   TDSV_CHECK(tiles < (int64_t(1) << 30), "linear_token_statistics: too many tiles");
   const int grid = static_cast<int>(std::min<int64_t>(num_sms(), tiles));
   void* args[] = {const_cast<CUtensorMap*>(&ma), const_cast<CUtensorMap*>(&mb), const_cast<CUtensorMap*>(&mc), &p};
@@ -360,40 +501,61 @@ void launch_head(const at::Tensor& hidden, const at::Tensor& weight, const CUten
 
 }  // namespace
 
-// (log_probs [M], entropy [M], saved [M, 4])
-std::vector<at::Tensor> lm_head_stats_fwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
-                                          double temperature, int64_t ignore_index) {
-  check_head(hidden, weight, targets);
-  const int64_t rows = hidden.size(0), vocab = weight.size(0);
-  c10::cuda::CUDAGuard guard(hidden.device());
-  const auto f32 = hidden.options().dtype(at::kFloat);
-  auto log_probs = at::empty({rows}, f32), entropy = at::empty({rows}, f32), saved = at::empty({rows, 4}, f32);
-  if (rows == 0) return {log_probs, entropy, saved};
-  const int64_t tiles = (vocab + BN - 1) / BN;
-  auto part = at::empty({3, tiles, rows}, f32);
-  auto target_logit = at::empty({rows}, f32);
+// (log_probs [M], entropy [M], saved [M, 4], fp32 logits [M, V] in rows padded to 32 bytes). `saved` is undefined
+// without `save`, the logits unless `keep` asks for them.
+std::vector<at::Tensor> lm_head_stats_fwd(const at::Tensor& hidden_in, const at::Tensor& weight, const at::Tensor& targets,
+                                          double temperature, int64_t ignore_index, bool save, bool keep) {
+  check_head(hidden_in, weight, targets);
+  const int64_t rows = hidden_in.size(0), vocab = weight.size(0);
+  c10::cuda::CUDAGuard guard(hidden_in.device());
+  const auto f32 = hidden_in.options().dtype(at::kFloat);
+  auto log_probs = at::empty({rows}, f32), entropy = at::empty({rows}, f32);
+  at::Tensor saved, logits, hidden = hidden_in, where, kept_targets;
+  if (save) saved = at::empty({rows, 4}, f32);
+  if (keep) logits = at::empty({rows, (vocab + 7) / 8 * 8}, f32).narrow(1, 0, vocab);
+  if (rows == 0) return {log_probs, entropy, saved, logits};
   HeadParams p{};
   p.c2 = static_cast<float>(1.4426950408889634 / temperature);
   p.targets = targets.data_ptr<int64_t>();
+  p.ignore_index = ignore_index;
+  if (!save && rows > 2 * BM) {  // (fewer would hardly save a row block)
+    where = at::empty({rows + 1}, f32.dtype(at::kInt));
+    kept_targets = at::empty({rows}, targets.options());
+    hidden = at::empty_like(hidden_in);
+    int* count = where.data_ptr<int>() + rows;
+    lm_head_rows_kernel<<<1, 1024, 0, stream()>>>(p.targets, static_cast<int>(rows), ignore_index, where.data_ptr<int>(),
+                                                  kept_targets.data_ptr<int64_t>(), count, log_probs.data_ptr<float>(),
+                                                  entropy.data_ptr<float>());
+    const int vecs = static_cast<int>(hidden.size(1) / 8);
+    lm_head_gather_kernel<<<static_cast<unsigned>(rows), 128, 0, stream()>>>(
+        static_cast<const uint4*>(hidden_in.data_ptr()), where.data_ptr<int>(), count, vecs,
+        static_cast<uint4*>(hidden.data_ptr()));
+    TDSV_LAUNCH_CHECK();
+    p.rows = count;
+    p.targets = kept_targets.data_ptr<int64_t>();
+  }
+  const int64_t tiles = (vocab + (keep ? BN : tile_columns(rows, vocab)) - 1) / (keep ? BN : tile_columns(rows, vocab));
+  auto part = at::empty({3 * tiles + 1, rows}, f32);
   p.part_m = part.data_ptr<float>();
   p.part_s = p.part_m + tiles * rows;
   p.part_w = p.part_s + tiles * rows;
-  p.target_logit = target_logit.data_ptr<float>();
-  p.ignore_index = ignore_index;
+  p.target_logit = p.part_w + tiles * rows;
   const CUtensorMap unused{};
-  launch_head<false>(hidden, weight, unused, p);
-  lm_head_join_kernel<<<static_cast<unsigned>((rows + 31) / 32), 32 * kJoinSlices, 0, stream()>>>(
-      p.part_m, p.part_s, p.part_w, p.target_logit, p.targets, ignore_index, static_cast<int>(rows),
-      static_cast<int>(vocab), static_cast<int>(tiles), p.c2, log_probs.data_ptr<float>(), entropy.data_ptr<float>(),
-      reinterpret_cast<float4*>(saved.data_ptr<float>()), p.status);
+  if (keep) launch_head<kStatsKeep>(hidden, weight, head_map(logits, (vocab + 7) / 8 * 8, 32), p);
+  else launch_head<kStats>(hidden, weight, unused, p);
+  lm_head_join_kernel<<<static_cast<unsigned>((rows + kJoinRows - 1) / kJoinRows), kJoinRows * kJoinSlices, 0, stream()>>>(
+      p, where.defined() ? where.data_ptr<int>() : nullptr, static_cast<int>(tiles), log_probs.data_ptr<float>(),
+      entropy.data_ptr<float>(), save ? reinterpret_cast<float4*>(saved.data_ptr<float>()) : nullptr);
   TDSV_LAUNCH_CHECK();
-  return {log_probs, entropy, saved};
+  return {log_probs, entropy, saved, logits};
 }
 
-// bf16 gradient of the logits, [M, V] with rows padded to 16 bytes.
+// bf16 gradient of the logits, [M, V] with rows padded to 16 bytes, from the logits that were kept or else from the
+// product again.
 at::Tensor lm_head_stats_bwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
-                             const at::Tensor& saved, double temperature, int64_t ignore_index,
-                             const c10::optional<at::Tensor>& g_log_probs, const c10::optional<at::Tensor>& g_entropy) {
+                             const at::Tensor& saved, const c10::optional<at::Tensor>& logits, double temperature,
+                             int64_t ignore_index, const c10::optional<at::Tensor>& g_log_probs,
+                             const c10::optional<at::Tensor>& g_entropy) {
   check_head(hidden, weight, targets);
   const int64_t rows = hidden.size(0), vocab = weight.size(0), pitch = (vocab + 7) / 8 * 8;
   c10::cuda::CUDAGuard guard(hidden.device());
@@ -415,8 +577,20 @@ at::Tensor lm_head_stats_bwd(const at::Tensor& hidden, const at::Tensor& weight,
   p.g = pointer(g_log_probs);
   p.h = pointer(g_entropy);
   p.ignore_index = ignore_index;
-  const CUtensorMap mc = head_map(dlogits, pitch, 32);
-  launch_head<true>(hidden, weight, mc, p);
+  if (logits.has_value() && logits->defined()) {
+    TDSV_CHECK(logits->is_cuda() && logits->scalar_type() == at::kFloat && logits->dim() == 2 && logits->size(0) == rows &&
+                   logits->size(1) == vocab && (rows == 1 || logits->stride(0) == pitch),
+               "linear_token_statistics: kept logits");
+    p.M = static_cast<int>(rows);
+    p.N = static_cast<int>(vocab);
+    const int vecs = static_cast<int>(pitch / 8), parts = (vecs + kKeptThreads * kKeptVecs - 1) / (kKeptThreads * kKeptVecs);
+    TDSV_CHECK(rows * parts < (int64_t(1) << 31), "linear_token_statistics: too many rows");
+    lm_head_kept_kernel<<<static_cast<unsigned>(rows * parts), kKeptThreads, 0, stream()>>>(
+        reinterpret_cast<const float4*>(logits->data_ptr<float>()), p, parts, vecs, static_cast<uint4*>(dlogits.data_ptr()));
+    TDSV_LAUNCH_CHECK();
+    return dlogits;
+  }
+  launch_head<kGrad>(hidden, weight, head_map(dlogits, pitch, 32), p);
   return dlogits;
 }
 

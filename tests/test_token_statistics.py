@@ -459,6 +459,54 @@ def test_linear_statistics_in_row_blocks(monkeypatch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,hidden,vocab", [(5, 64, 300), (260, 512, 20011), (129, 1024, 9000)])
+def test_linear_statistics_recomputed(monkeypatch, rows, hidden, vocab):
+    """The backward without kept logits: the same fp32 values, so the same gradients to their bf16 rounding."""
+    h, w, t = _head(rows, hidden, vocab, "cuda", torch.bfloat16, 50)
+    g, e = torch.randn(rows, device="cuda"), torch.randn(rows, device="cuda")
+    grads = []
+    for kept in (S.KEPT_BYTES, 0):
+        monkeypatch.setattr(S, "KEPT_BYTES", kept)
+        hh, ww = h.clone().requires_grad_(), w.clone().requires_grad_()
+        got = ops.linear_token_statistics(hh, ww, t)
+        torch.autograd.backward((got.log_probs, got.entropy), (g, e))
+        grads.append((hh.grad.float(), ww.grad.float()))
+    for a, b in zip(*grads):
+        assert (a - b).norm() <= 2.0 ** -8 * a.norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 256, 2048), (300, 512, 40000), (129, 264, 20011), (128, 2048, 5000)])
+def test_gemm_split_k(m, n, k):
+    gen = _generator(60)
+    pitch = (k + 7) // 8 * 8
+    a = torch.randn(m, pitch, generator=gen).bfloat16().cuda()[:, :k]
+    b = torch.randn(k, n, generator=gen).bfloat16().cuda()
+    out = torch.full((m, n), float("nan"), device="cuda", dtype=torch.bfloat16)
+    ops.ext().gemm_split_k(a, b, out)
+    want = a.double() @ b.double()
+    # one rounding to bf16 of each value, and fp32 sums that are off by 1e-5 of the products' size
+    assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5 * k).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,ignored", [(300, 0), (300, 1), (300, 299), (300, 300), (2500, 1100)])
+def test_linear_statistics_leaves_ignored_rows_out(rows, ignored):
+    h, w, t = _head(rows, 128, 2003, "cuda", torch.bfloat16, 70)
+    t[1] = 7
+    t[torch.randperm(rows, generator=_generator(71))[:ignored].cuda()] = -100
+    h[t == -100] = float("nan")
+    got = ops.linear_token_statistics(h, w, t)
+    kept = t != -100
+    want = _statistics((h[kept].double() @ w.double().t()).cpu(), t[kept].cpu(), 1.0, 0)
+    _close_rows(got.log_probs[kept], want["log_probs"], 3e-5, 1e-5)
+    _close_rows(got.entropy[kept], want["entropy"], 3e-4)
+    assert bool((got.log_probs[~kept] == 0).all()) and bool((got.entropy[~kept] == 0).all())
+    again = ops.linear_token_statistics(h, w, t)
+    assert torch.equal(got.log_probs, again.log_probs) and torch.equal(got.entropy, again.entropy)
+
+
+@pytest.mark.gpu
 def test_linear_statistics_other_types_and_views():
     h, w, t = _head(12, 60, 333, "cuda", torch.bfloat16, 40)  # H is no multiple of 8: the product is written
     want = _statistics((h @ w.t()).cpu(), t.cpu(), 1.0, 0)

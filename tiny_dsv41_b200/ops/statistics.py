@@ -24,6 +24,7 @@ from .loss import IGNORE_INDEX
 
 MAX_TOP = 128  # alternatives of one row
 GRADIENT_BYTES = 4 * 2 ** 30  # of the logits' gradient that linear_token_statistics holds at a time
+KEPT_BYTES = 4 * 2 ** 30  # of fp32 logits that it keeps for its backward; larger ones are recomputed
 _LOGIT_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -176,8 +177,10 @@ def token_statistics(logits: torch.Tensor, targets: torch.Tensor | None = None, 
 class _LinearTokenStatistics(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, temperature):
-        lp, entropy, saved = ext().lm_head_stats_fwd(hidden, weight, targets, temperature, IGNORE_INDEX)
-        ctx.save_for_backward(hidden, weight, targets, saved)
+        ctx.keep = hidden.shape[0] * weight.shape[0] * 4 <= KEPT_BYTES
+        lp, entropy, saved, logits = ext().lm_head_stats_fwd(hidden, weight, targets, temperature, IGNORE_INDEX, True,
+                                                             ctx.keep)
+        ctx.save_for_backward(hidden, weight, targets, saved, logits)
         ctx.temperature = temperature
         ctx.set_materialize_grads(False)
         return lp, entropy
@@ -186,11 +189,11 @@ class _LinearTokenStatistics(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_lp, g_entropy):
         C = ext()
-        hidden, weight, targets, saved = ctx.saved_tensors
+        hidden, weight, targets, saved, logits = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[:2]
         if g_lp is None and g_entropy is None:
             return None, None, None, None
-        g_lp, g_entropy = (None if g is None else g.float().contiguous() for g in (g_lp, g_entropy))
+        g_lp, g_entropy = (None if g is None else g.contiguous() for g in (g_lp, g_entropy))
         rows, vocab = hidden.shape[0], weight.shape[0]
         if rows == 0:
             return hidden.new_zeros(hidden.shape), weight.new_zeros(weight.shape), None, None
@@ -202,11 +205,11 @@ class _LinearTokenStatistics(torch.autograd.Function):
                                                                             device=weight.device)
         for start in range(0, rows, chunk):
             part = slice(start, min(rows, start + chunk))
-            dlogits = C.lm_head_stats_bwd(hidden[part], weight, targets[part], saved[part], ctx.temperature,
-                                          IGNORE_INDEX, None if g_lp is None else g_lp[part],
-                                          None if g_entropy is None else g_entropy[part])
+            pick = lambda x: None if x is None else x[part]  # noqa: E731
+            dlogits = C.lm_head_stats_bwd(hidden[part], weight, targets[part], saved[part], pick(logits),
+                                          ctx.temperature, IGNORE_INDEX, pick(g_lp), pick(g_entropy))
             if need_dx:
-                C.gemm(dlogits, weight, dx[part], False, True, False)
+                C.gemm_split_k(dlogits, weight, dx[part])
             if need_dw:
                 C.gemm(dlogits, hidden[part], dw, True, True, chunk < rows)
             del dlogits
@@ -219,9 +222,10 @@ def linear_token_statistics(hidden: torch.Tensor, weight: torch.Tensor, targets:
     ``targets`` and entropy of each row of ``hidden`` [..., H] under the LM head ``weight`` [V, H].
 
     The reduction runs in the epilogue of the tensor-core product on its fp32 accumulators, so no
-    logit is rounded to bf16; backward recomputes the product, writes the logits' bf16 gradient (in
-    row blocks of at most 4 GiB) and multiplies it into ``hidden`` and ``weight``. Rows with target -100 give 0 and
-    take no gradient. bf16 operands with H a multiple of 8; on a GPU other types go through the product
+    logit is rounded to bf16. Without a backward no logit is written, and rows with target -100, whose
+    results are 0, take no part in the product. For a backward the fp32 logits are kept while they take at
+    most ``KEPT_BYTES`` (4 GiB), else their product is repeated; the logits' bf16 gradient, in row blocks of
+    at most 4 GiB, is multiplied into ``hidden`` and ``weight``. bf16 operands with H a multiple of 8; on a GPU other types go through the product
     and :func:`token_statistics`, where the logits exist in ``hidden``'s type."""
     temperature = _check_temperature(temperature)
     if hidden.ndim < 1 or weight.ndim != 2 or hidden.shape[-1] != weight.shape[1] or weight.shape[0] < 1:
@@ -238,7 +242,7 @@ def linear_token_statistics(hidden: torch.Tensor, weight: torch.Tensor, targets:
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         lp, entropy = _LinearTokenStatistics.apply(flat, weight, targets, temperature)
     else:
-        lp, entropy, _ = ext().lm_head_stats_fwd(flat, weight, targets, temperature, IGNORE_INDEX)
+        lp, entropy, _, _ = ext().lm_head_stats_fwd(flat, weight, targets, temperature, IGNORE_INDEX, False, False)
     return TokenStatistics(lp.view(shape), entropy.view(shape))
 
 
