@@ -46,7 +46,7 @@ struct HeadParams {
   float c2, inv_t;
   const int64_t* targets;  // [M]
   // statistics
-  float *part_m, *part_s, *part_w;  // [column tiles, M]
+  float4* part;                     // [column tiles, M]: m, S, W
   float* target_logit;              // [M]
   // gradient
   const float4* saved;  // [M]: m, 1 / S, W / S
@@ -240,9 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (live) {
           const int64_t o = static_cast<int64_t>(t.nb) * p.M + row;
-          p.part_m[o] = st.m;
-          p.part_s[o] = st.s;
-          p.part_w[o] = st.w;
+          p.part[o] = make_float4(st.m, st.s, st.w, 0.f);
         }
       } else {
 #pragma unroll 1
@@ -293,43 +291,52 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the column tiles of each row: 8 rows a block, 64 slices of the tiles. The largest reference first, so that
-// no term waits for the one before; slices are added in slice order.
-constexpr int kJoinRows = 8, kJoinSlices = 64;
-__global__ void __launch_bounds__(kJoinRows * kJoinSlices)
+// Joins the column tiles of each row: 4 rows a block, 128 slices of the tiles. The largest reference first, so that
+// no term waits for the one before; the order of the sums is fixed.
+constexpr int kJoinRows = 4, kJoinThreads = 512;
+__global__ void __launch_bounds__(kJoinThreads)
     lm_head_join_kernel(const HeadParams p, const int* __restrict__ where, int tiles, float* __restrict__ log_probs,
                         float* __restrict__ entropy, float4* __restrict__ saved) {
-  __shared__ float part[2][kJoinSlices][kJoinRows];
-  const int lane = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows;
+  __shared__ float part[3][kJoinThreads / 32][kJoinRows];
+  constexpr int kSlices = kJoinThreads / kJoinRows;
+  const int lane = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows, warp = threadIdx.x >> 5;
   const int i = blockIdx.x * kJoinRows + lane;
   const bool live = i < (p.rows != nullptr ? min(*p.rows, p.M) : p.M);
+  const float4* mine = p.part + i;
   float m = -INFINITY;
   if (live)
-    for (int t = slice; t < tiles; t += kJoinSlices) {
-      const int64_t o = static_cast<int64_t>(t) * p.M + i;
-      if (p.part_s[o] != 0.f) m = fmaxf(m, p.part_m[o]);
+#pragma unroll 4
+    for (int t = slice; t < tiles; t += kSlices) {
+      const float4 u = mine[static_cast<int64_t>(t) * p.M];
+      m = fmaxf(m, u.y != 0.f ? u.x : -INFINITY);
     }
-  part[0][slice][lane] = m;
+#pragma unroll
+  for (int o = kJoinRows; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) < kJoinRows) part[0][warp][lane] = m;
   __syncthreads();
-  for (int s = 0; s < kJoinSlices; ++s) m = fmaxf(m, part[0][s][lane]);
-  __syncthreads();
-  float sum = 0.f, w = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) m = fmaxf(m, part[0][w][lane]);
+  float sum = 0.f, weighted = 0.f;
   if (live)
-    for (int t = slice; t < tiles; t += kJoinSlices) {
-      const int64_t o = static_cast<int64_t>(t) * p.M + i;
-      const float s = p.part_s[o];
-      if (s == 0.f) continue;
-      const float d = (p.part_m[o] - m) * p.c2, f = exp2_fast(d);
-      sum += s * f;
-      w += (p.part_w[o] + s * fmaxf(d, kMinExponent)) * f;
+#pragma unroll 4
+    for (int t = slice; t < tiles; t += kSlices) {
+      const float4 u = mine[static_cast<int64_t>(t) * p.M];
+      const float d = (u.x - m) * p.c2, f = exp2_fast(d);
+      sum += u.y != 0.f ? u.y * f : 0.f;
+      weighted += u.y != 0.f ? (u.z + u.y * fmaxf(d, kMinExponent)) * f : 0.f;
     }
-  part[0][slice][lane] = sum;
-  part[1][slice][lane] = w;
+#pragma unroll
+  for (int o = kJoinRows; o < 32; o <<= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    weighted += __shfl_xor_sync(0xffffffffu, weighted, o);
+  }
+  if ((threadIdx.x & 31) < kJoinRows) part[1][warp][lane] = sum, part[2][warp][lane] = weighted;
   __syncthreads();
   if (slice != 0 || !live) return;
   RowStats st;
   st.m = m;
-  for (int s = 0; s < kJoinSlices; ++s) st.s += part[0][s][lane], st.w += part[1][s][lane];
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) st.s += part[1][w][lane], st.w += part[2][w][lane];
   const int64_t target = p.targets[i];
   const int r = where != nullptr ? where[i] : i;
   float lp = 0.f, ent = 0.f;
@@ -535,15 +542,13 @@ std::vector<at::Tensor> lm_head_stats_fwd(const at::Tensor& hidden_in, const at:
     p.targets = kept_targets.data_ptr<int64_t>();
   }
   const int64_t tiles = (vocab + (keep ? BN : tile_columns(rows, vocab)) - 1) / (keep ? BN : tile_columns(rows, vocab));
-  auto part = at::empty({3 * tiles + 1, rows}, f32);
-  p.part_m = part.data_ptr<float>();
-  p.part_s = p.part_m + tiles * rows;
-  p.part_w = p.part_s + tiles * rows;
-  p.target_logit = p.part_w + tiles * rows;
+  auto part = at::empty({4 * tiles + 1, rows}, f32);
+  p.part = reinterpret_cast<float4*>(part.data_ptr<float>());
+  p.target_logit = part.data_ptr<float>() + 4 * tiles * rows;
   const CUtensorMap unused{};
   if (keep) launch_head<kStatsKeep>(hidden, weight, head_map(logits, (vocab + 7) / 8 * 8, 32), p);
   else launch_head<kStats>(hidden, weight, unused, p);
-  lm_head_join_kernel<<<static_cast<unsigned>((rows + kJoinRows - 1) / kJoinRows), kJoinRows * kJoinSlices, 0, stream()>>>(
+  lm_head_join_kernel<<<static_cast<unsigned>((rows + kJoinRows - 1) / kJoinRows), kJoinThreads, 0, stream()>>>(
       p, where.defined() ? where.data_ptr<int>() : nullptr, static_cast<int>(tiles), log_probs.data_ptr<float>(),
       entropy.data_ptr<float>(), save ? reinterpret_cast<float4*>(saved.data_ptr<float>()) : nullptr);
   TDSV_LAUNCH_CHECK();

@@ -9,7 +9,9 @@ the row's largest value, plus one rounding to its type (2^-9 for bf16, 2^-11 for
 fp16's smallest step of 6e-8).
 """
 
+import importlib.util
 import math
+from pathlib import Path
 
 import pytest
 import torch
@@ -703,3 +705,32 @@ def test_distillation_ids_beyond_the_vocabulary_set_the_status():
     assert loss.rows.isnan().tolist() == [True, False] and bool(grad[1].isfinite().all())
     with pytest.raises(ops.DeviceStatusError, match="out of bounds"):
         ops.check_status("distillation")
+
+
+# -- together ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("device", DEVICES)
+def test_distillation_example(device):
+    path = Path(__file__).resolve().parents[1] / "examples" / "distill" / "distill_top_logits.py"
+    spec = importlib.util.spec_from_file_location(path.stem, path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    rows = example.main(["--steps", "12", "--top", "8", "--device", device, "--seq-len", "16"])
+    losses = [r["loss"] for r in rows if r["event"] == "train"]
+    assert len(losses) == 12 and all(map(math.isfinite, losses)) and losses[-1] < 0.8 * losses[0]
+    assert rows[0]["event"] == rows[-1]["event"] == "evaluate"
+    assert 0 < rows[-1]["entropy"] < rows[0]["entropy"] <= math.log(256) + 1e-3  # the student took on opinions
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_lm_head_statistics_mode(device):
+    from tiny_dsv41_b200.models.common import LMHead
+
+    torch.manual_seed(0)
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    head = LMHead(64, 300).to(device, dtype)
+    hidden = torch.randn(2, 5, 64, device=device, dtype=dtype)
+    targets = torch.randint(0, 300, (2, 5), device=device)
+    got = head(hidden, targets, mode="statistics", temperature=0.7)
+    want = _statistics((hidden.double() @ head.weight.detach().double().t()).reshape(10, 300).cpu(), targets.reshape(-1).cpu(), 0.7, 0)
+    _close_rows(got.log_probs.detach().reshape(-1), want["log_probs"], 3e-5, 1e-5)
+    _close_rows(got.entropy.detach().reshape(-1), want["entropy"], 3e-4)

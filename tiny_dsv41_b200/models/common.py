@@ -9,8 +9,9 @@ from .. import ops
 
 
 class LMHead(nn.Linear):
-    """``nn.Linear`` LM head whose forward can also return the fused cross-entropy sum or
-    selected-token log-probabilities.
+    """``nn.Linear`` LM head whose forward can also return the fused cross-entropy sum, selected-token
+    log-probabilities, or (``mode="statistics"``) log-probabilities with the entropy, straight from the
+    product (:func:`ops.linear_token_statistics`).
 
     Going through ``forward`` matters under FSDP2: the (sharded) weight is only gathered inside
     the module's forward, so the loss kernels must run there rather than on ``self.weight``
@@ -21,7 +22,7 @@ class LMHead(nn.Linear):
         super().__init__(hidden_size, vocab_size, bias=False)
 
     def forward(self, hidden: torch.Tensor, targets: torch.Tensor | None = None, *, mode: str = "logits",
-                temperature: float = 1.0) -> torch.Tensor:
+                temperature: float = 1.0):
         if mode == "logits":
             return ops.linear(hidden, self.weight)
         if mode == "ce_sum":
@@ -29,6 +30,8 @@ class LMHead(nn.Linear):
         if mode == "logprob":
             logits = ops.linear(hidden, self.weight).float()
             return ops.token_log_probs(logits, targets, temperature)
+        if mode == "statistics":
+            return ops.linear_token_statistics(hidden, self.weight, targets, temperature=temperature)
         raise ValueError(f"unknown LM head mode {mode!r}")
 
 
