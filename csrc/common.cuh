@@ -39,7 +39,7 @@ enum StatusCode : int {
   kTimeoutAccumFree = 4, // MMA warp waited too long for the epilogue to drain TMEM
   kTimeoutPeer = 5,      // a peer rank never raised its flag
   kBadShape = 6,
-  kOutOfBounds = 7,      // a computed index fell outside its buffer (TDSV_BOUNDS_CHECK builds only)
+  kOutOfBounds = 7,      // a token id outside the vocabulary; in TDSV_BOUNDS_CHECK builds any index outside its buffer
 };
 
 

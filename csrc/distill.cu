@@ -40,7 +40,8 @@ struct RowPlan {
   int read;                             // whether the row is read at all
   int bad;                              // an id beyond the vocabulary
   int copied;                           // whether the bulk copy was started
-  float q_sum, q_rest, q_log_q, q_y;    // sums over the alternatives: q, the rest, q ln q, q y
+  float q_sum, q_rest;                  // the alternatives' mass and the rest
+  double q_gap;                         // sum q (ln q - ln 2 y): the divergence but for the student's normalisation
   float chosen_m, chosen_s;             // the student's sum over the alternatives
   float base;                           // reference of the pass that writes the gradient
   float outside;                        // A above
@@ -69,6 +70,10 @@ __device__ __forceinline__ void named_barrier_wait() {
 // one write, whatever its length (up to the shared memory of 16 blocks). Five blocks on an SM are in
 // different phases, which keeps copies, sums and stores going at once: the phases of one block alone are a chain
 // of latencies. Without the gradient a stretch passes through registers.
+//
+// 4096 rows of 151936 bf16 with 64 alternatives take 588 us, 4.2 TB/s of the two passes over memory (floor 380): bound
+// by a block's chain of phases and, at half of their rate, by the two exponentials of every value. The loss alone of
+// 2000 rows takes 128 us.
 //
 // One warp deals with the alternatives, up to four a lane, without block barriers.
 template <typename T, typename I, bool GRAD>
@@ -201,7 +206,8 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
 #pragma unroll
     for (int j = 0; j < kPerLane; ++j) x[j] = id[j] >= 0 ? to_float<T>(row[id[j]]) : -INFINITY;
     if (tail) shift = 0.f;
-    float q[kPerLane], q_sum = 0.f, q_log_q = 0.f, q_y = 0.f;
+    float q[kPerLane], q_sum = 0.f;
+    double q_gap = 0.0;  // (terms of ten and more that leave a divergence of a tenth: 64 bits, off the others' path)
     RowStats chosen;
 #pragma unroll
     for (int j = 0; j < kPerLane; ++j) {
@@ -218,18 +224,19 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
       if (!tail) q[j] /= q_sum;
       const float y = (x[j] - chosen.m) * c2, e = exp2_fast(y);
       if (id[j] >= 0) chosen.s += e;
-      if (q[j] != 0.f) q_log_q += q[j] * (t[j] - shift - log_sum), q_y += q[j] * y;
+      if (q[j] != 0.f)
+        q_gap += static_cast<double>(q[j]) * (static_cast<double>(t[j]) - shift - log_sum -
+                                              0.6931471805599453 * (static_cast<double>(x[j]) - chosen.m) * c2);
       q_s[j * 32 + lane] = q[j];
       e_s[j * 32 + lane] = e;
     }
-    q_log_q = warp_sum(q_log_q);
-    q_y = warp_sum(q_y);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) q_gap += __shfl_xor_sync(0xffffffffu, q_gap, o);
     chosen.s = warp_sum(chosen.s);
     if (lane == 0) {
       plan.q_sum = tail ? q_sum : 1.f;
       plan.q_rest = tail ? fmaxf(0.f, 1.f - q_sum) : 0.f;
-      plan.q_log_q = q_log_q;
-      plan.q_y = q_y;
+      plan.q_gap = q_gap;
       plan.chosen_m = chosen.m;
       plan.chosen_s = chosen.s;
     }
@@ -342,7 +349,7 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
     all.merge(rest, c2);
     const float log2s = log2f(all.s), q_sum = plan.q_sum, q_rest = rest.s == 0.f ? 0.f : plan.q_rest;
     // - ln p_k = ln 2 (log2 S + (m - m_a) c2 - y_k)
-    float loss = plan.q_log_q - kLn2 * (plan.q_y + q_sum * ((chosen.m - all.m) * c2 - log2s));
+    float loss = static_cast<float>(plan.q_gap - 0.6931471805599453 * q_sum * ((chosen.m - all.m) * c2 - log2s));
     if (q_rest > 0.f) loss += q_rest * (logf(q_rest) - kLn2 * ((rest.m - all.m) * c2 + log2f(rest.s) - log2s));
     const bool empty = all.s == 0.f;  // every logit is masked: no distribution, no gradient
     if (empty) loss = INFINITY;

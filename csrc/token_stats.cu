@@ -262,6 +262,10 @@ __device__ __noinline__ int collect_again(const T* row, int first, int last, int
 // comparison for a thread's batch, a candidate some 20 instructions (by single values it was 67, and 4096 rows
 // with 64 alternatives took 546 us). At the end the `top` first vectors hold all of the `top` first values: they
 // are read once more, value by value.
+//
+// Bound by memory without alternatives: 3001 rows of 151936 bf16 take 144 us, 6.3 TB/s. With 64 alternatives 4096 rows
+// take 339 us (3.7 TB/s): the selections of a row are serial phases that the four blocks of an SM cover in part.
+// Four blocks of 256 threads hold 64 KB of loads in flight an SM, which the registers allow and the latency needs.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kStatThreads, 4)
     stats_fwd_kernel(const T* __restrict__ logits, RowLayout layout, int v, const int64_t* __restrict__ targets,
@@ -483,8 +487,9 @@ __global__ void __launch_bounds__(kStatThreads, 4)
   }
 }
 
-// A block writes the gradient of one stretch of a row (kStretch values of 2 bytes: enough to hide the
-// start, small enough that the last wave of blocks is short).
+// A block writes the gradient of one stretch of a row: long enough to hide its start, short enough that the last round
+// of blocks is short. Bound by memory: one read and one write; 2047 x 151669 in rows that are aligned differently on
+// both sides take 309 us with their forward, 1.6 GB at 5.2 TB/s.
 constexpr int kStretchBytes = 32768;
 
 template <typename T>

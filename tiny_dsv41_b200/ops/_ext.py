@@ -42,7 +42,7 @@ def on_gpu(*tensors: torch.Tensor | None) -> bool:
 STATUS_CODES = {
     1: "TMA stage wait timed out", 2: "TMA stage wait timed out", 3: "accumulator wait timed out",
     4: "accumulator wait timed out", 5: "a peer rank never raised its flag (peer wait timed out)",
-    6: "bad shape", 7: "index out of bounds (bounds-check build)",
+    6: "bad shape", 7: "index out of bounds (a token id beyond the vocabulary, or any index in a bounds-check build)",
 }
 
 
