@@ -55,14 +55,6 @@ struct RowStats {
     s *= f;
     m = to;
   }
-  __device__ __forceinline__ void add(float x, float c2) {
-    if (x > m) rebase(x, c2);
-    if (x == -INFINITY) return;
-    const float y = (x - m) * c2;
-    const float e = exp2_fast(y);
-    s += e;
-    w += e * fmaxf(y, kMinExponent);
-  }
   __device__ __forceinline__ void merge(const RowStats& o, float c2) {
     if (o.s == 0.f) return;  // (a NaN sum is not equal to zero and is merged)
     RowStats a = o;

@@ -637,6 +637,51 @@ def test_distillation_upstream_gradient(device, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,vocab", [(torch.bfloat16, 262144), (torch.float16, 262147), (torch.float32, 500003)])
+def test_large_vocabularies(dtype, vocab):
+    """Rows that a cluster of 16 blocks, or long stretches, hold."""
+    logits = _logits(3, vocab, dtype, 90, "cuda").requires_grad_()
+    ids, teacher = _teacher(logits.detach(), 64, 91)
+    weights = torch.tensor([0.3, 1.0, 0.7])
+    loss = ops.distillation_loss(logits, ids.cuda(), teacher.cuda(), weights.cuda(), tail=True)
+    grad, = torch.autograd.grad(loss.total, logits)
+    want_rows, want_grad = _distillation(logits.detach(), ids, teacher, weights, 1.0, True)
+    _close_rows(loss.rows, want_rows, 1e-4)
+    _close_gradient(grad, want_grad)
+    targets = torch.tensor([0, vocab - 1, 77], device="cuda")
+    got = ops.token_statistics(logits, targets, top=128)
+    _check_statistics(logits.detach(), targets, 1.0, 128, S.TokenStatistics(*(x.detach() for x in got)))
+    grad, = torch.autograd.grad(got.log_probs.sum() + got.entropy.sum(), logits)
+    _close_gradient(grad, _statistics_gradient(logits.detach(), targets, 1.0, torch.ones(3), torch.ones(3)))
+
+
+@pytest.mark.gpu
+def test_operators_in_a_cuda_graph():
+    logits = _logits(5, 30011, torch.bfloat16, 92, "cuda")
+    ids, teacher = (x.cuda() for x in _teacher(logits, 8, 93))
+    targets = torch.randint(0, 30011, (5,), device="cuda")
+    hidden, weight, _ = _head(300, 64, 515, "cuda", torch.bfloat16, 94)
+    aims = torch.randint(0, 515, (300,), device="cuda")
+
+    def run():
+        with torch.no_grad():
+            s = ops.token_statistics(logits, targets, top=7)
+            d = ops.distillation_loss(logits, ids, teacher, tail=True)
+            h = ops.linear_token_statistics(hidden, weight, aims)
+        return [*s, *d, h.log_probs, h.entropy]
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    logits.copy_(_logits(5, 30011, torch.bfloat16, 95, "cuda"))
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(out, run()):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_distillation_second_backward_is_refused():
     logits = _logits(2, 64, torch.float32, 57, "cuda").requires_grad_()
     loss = ops.distillation_loss(logits, torch.tensor([[1], [2]], device="cuda"), torch.zeros(2, 1, device="cuda"))
