@@ -41,7 +41,7 @@ struct RowPlan {
   int bad;                              // an id beyond the vocabulary
   int copied;                           // whether the bulk copy was started
   float q_sum, q_rest;                  // the alternatives' mass and the rest
-  double q_gap;                         // sum q (ln q - ln 2 y): the divergence but for the student's normalisation
+  double q_gap, log_chosen;             // sum q (ln q - ln 2 y) and ln of chosen_s: see the loss below
   float chosen_m, chosen_s;             // the student's sum over the alternatives
   float base;                           // reference of the pass that writes the gradient
   float outside;                        // A above
@@ -71,9 +71,9 @@ __device__ __forceinline__ void named_barrier_wait() {
 // different phases, which keeps copies, sums and stores going at once: the phases of one block alone are a chain
 // of latencies. Without the gradient a stretch passes through registers.
 //
-// 4096 rows of 151936 bf16 with 64 alternatives take 588 us, 4.2 TB/s of the two passes over memory (floor 380): bound
+// 4096 rows of 151936 bf16 with 64 alternatives take 582 us, 4.3 TB/s of the two passes over memory (floor 380): bound
 // by a block's chain of phases and, at half of their rate, by the two exponentials of every value. The loss alone of
-// 2000 rows takes 128 us.
+// 2000 rows takes 129 us.
 //
 // One warp deals with the alternatives, up to four a lane, without block barriers.
 template <typename T, typename I, bool GRAD>
@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
       plan.q_sum = tail ? q_sum : 1.f;
       plan.q_rest = tail ? fmaxf(0.f, 1.f - q_sum) : 0.f;
       plan.q_gap = q_gap;
+      plan.log_chosen = log(static_cast<double>(chosen.s));
       plan.chosen_m = chosen.m;
       plan.chosen_s = chosen.s;
     }
@@ -347,20 +348,28 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
     }
     RowStats all = chosen;
     all.merge(rest, c2);
-    const float log2s = log2f(all.s), q_sum = plan.q_sum, q_rest = rest.s == 0.f ? 0.f : plan.q_rest;
-    // - ln p_k = ln 2 (log2 S + (m - m_a) c2 - y_k)
-    float loss = static_cast<float>(plan.q_gap - 0.6931471805599453 * q_sum * ((chosen.m - all.m) * c2 - log2s));
-    if (q_rest > 0.f) loss += q_rest * (logf(q_rest) - kLn2 * ((rest.m - all.m) * c2 + log2f(rest.s) - log2s));
+    // The student's mass at and outside the alternatives. With ln p_k = ln 2 y_k - ln S_a + ln p_a the loss is
+    //   sum q (ln q - ln 2 y + ln S_a) - q_sum ln p_a + q_rest (ln q_rest - ln p_rest)
+    // whose first part is known before the row is, in 64 bits, and whose logarithms are of masses: small numbers, so
+    // a small divergence keeps its digits. (Below 1e-30 a mass's logarithm comes from its parts.)
+    const float q_sum = plan.q_sum, q_rest = rest.s == 0.f ? 0.f : plan.q_rest;
+    const float to_p = chosen.s == 0.f ? 0.f : exp2_fast((chosen.m - all.m) * c2) / all.s, p_chosen = chosen.s * to_p;
+    const float p_rest = rest.s == 0.f ? 0.f : exp2_fast((rest.m - all.m) * c2) * rest.s / all.s;
+    auto log_mass = [&](float p, const RowStats& of) {
+      return p > 1e-30f ? logf(p) : kLn2 * ((of.m - all.m) * c2 + log2f(of.s) - log2f(all.s));
+    };
+    float loss = 0.f;
+    if (q_sum > 0.f) {  // (a masked token with mass: q_gap is +inf)
+      const double log_chosen = repeated ? log(static_cast<double>(chosen.s)) : plan.log_chosen;
+      loss = chosen.s == 0.f ? INFINITY
+                             : static_cast<float>(plan.q_gap + q_sum * (log_chosen - log_mass(p_chosen, chosen)));
+    }
+    if (q_rest > 0.f) loss += q_rest * (logf(q_rest) - log_mass(p_rest, rest));
     const bool empty = all.s == 0.f;  // every logit is masked: no distribution, no gradient
     if (empty) loss = INFINITY;
     if (plan.bad) loss = NAN;
     const float scale = w * inv_t, whole = q_sum + q_rest;
-    const float to_p = chosen.s == 0.f ? 0.f : exp2_fast((chosen.m - all.m) * c2) / all.s;
-    float outside = 0.f;
-    if (rest.s != 0.f) {
-      const float p_rest = exp2_fast((rest.m - all.m) * c2) * rest.s / all.s;
-      outside = scale * (q_sum * p_rest - q_rest * (chosen.s * to_p)) / rest.s;
-    }
+    const float outside = rest.s == 0.f ? 0.f : scale * (q_sum * p_rest - q_rest * p_chosen) / rest.s;
     if (GRAD) {
       for (int a = lane; a < k; a += 32) {
         float mass = q_s[a];
