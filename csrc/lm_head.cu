@@ -22,7 +22,7 @@
 // timeout records a status code and the CTA drains and exits.
 //
 // Bound by the tensor cores: 4096 x 2048 x 151936 takes 1.80 ms, 1417 TFLOP/s (the plain library product 1.85 ms). One
-// row block is bound by the weight's way from memory instead: 16 rows take 146 us, 4.3 TB/s.
+// row block is bound by the weight's way from memory instead: 16 rows take 105 us, 5.9 TB/s.
 #include "logit_rows.cuh"
 
 #include <mutex>
@@ -35,11 +35,20 @@ constexpr int BM = 128;
 constexpr int BN = 256;
 constexpr int BK = 64;
 constexpr int kThreads = 192;
-constexpr int kStages = 4;
-constexpr int kStageA = BM * BK * 2;
 constexpr int kStageB = BN * BK * 2;
 constexpr int kStageC = 32 * 128;
-constexpr int kSmemBytes = kStages * (kStageA + kStageB) + 4 * kStageC + 1024 /*align*/ + 256 /*barriers*/;
+
+// FEW: at most 32 rows. The weight is then read once, from memory, and what is on its way sets the pace (16 rows: 144 us
+// with 4 stages of 208 columns, 200 with 128 columns), so a stage holds 32 rows of hidden and there are six: 105 us. The
+// MMA still takes 128 rows: the others are whatever follows in shared memory, and their accumulators are not read.
+template <bool FEW>
+struct Ring {
+  static constexpr int kRows = FEW ? 32 : BM;
+  static constexpr int kStages = FEW ? 6 : 4;
+  static constexpr int kStageA = kRows * BK * 2;
+  static constexpr int kStaging = FEW ? 0 : 4 * kStageC;
+  static constexpr int kSmemBytes = kStages * (kStageA + kStageB) + kStaging + 1024 /*align*/ + 256 /*barriers*/;
+};
 
 enum Epilogue : int { kStats = 0, kStatsKeep = 1, kGrad = 2 };
 
@@ -72,16 +81,18 @@ __device__ __forceinline__ bool head_tile(const HeadParams& p, int rows, int til
   return true;
 }
 
-template <int EPI>
+template <int EPI, bool FEW>
 __global__ void __launch_bounds__(kThreads, 1)
     lm_head_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                    const __grid_constant__ CUtensorMap tma_c, const HeadParams p) {
+  using R = Ring<FEW>;
+  constexpr int kStages = R::kStages, kStageA = R::kStageA;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smem_a = smem;
   uint8_t* smem_b = smem + kStages * kStageA;
   uint8_t* smem_c = smem_b + kStages * kStageB;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem_c + 4 * kStageC);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_c + R::kStaging);
   uint64_t* empty = full + kStages;
   uint64_t* tfull = empty + kStages;  // [2]
   uint64_t* tempty = tfull + 2;       // [2]
@@ -166,6 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int buf = tcount & 1;
       const int row = t.m0 + quarter * 32 + lane;
       const bool live = row < rows;
+      const bool some = t.m0 + quarter * 32 < rows;  // (rows of this warp)
       const int64_t target = live ? p.targets[row] : -1;
       // the target's column inside this tile, or a column no chunk has
       const int64_t rel = target - t.n0;
@@ -187,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!mbar_wait(&tfull[buf], (tcount >> 1) & 1, p.status, kTimeoutAccum)) { *aborted = 1; break; }
       tc_fence_after();
       const uint32_t t_addr = tmem_base + buf * BN + (static_cast<uint32_t>(quarter * 32) << 16);
-      if (EPI != kGrad) {
+      if (EPI != kGrad && some) {
         RowStats st;
 #pragma unroll 1
         for (int c0 = 0; c0 < BN; c0 += 32) {
@@ -246,7 +258,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int64_t o = static_cast<int64_t>(t.nb) * p.M + row;
           p.part[o] = make_float4(st.m, st.s, st.w, 0.f);
         }
-      } else {
+      }
+      if (EPI == kGrad) {
 #pragma unroll 1
         for (int c0 = 0; c0 < BN; c0 += 64) {
           uint32_t raw[64];
@@ -489,24 +502,25 @@ int tile_columns(int64_t rows, int64_t vocab) {
   return best;
 }
 
-template <int EPI>
+template <int EPI, bool FEW>
 void launch_head(const at::Tensor& hidden, const at::Tensor& weight, const CUtensorMap& mc, HeadParams& p) {
-  auto kern = lm_head_kernel<EPI>;
+  using R = Ring<FEW>;
+  auto kern = lm_head_kernel<EPI, FEW>;
   static std::once_flag once;
   std::call_once(once, [&] {
-    TDSV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+    TDSV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kSmemBytes));
   });
   p.M = static_cast<int>(hidden.size(0));
   p.N = static_cast<int>(weight.size(0));
   p.K = static_cast<int>(hidden.size(1));
   p.bn = EPI == kStats ? tile_columns(p.M, p.N) : BN;
   p.status = status_word_ptr();
-  const CUtensorMap ma = head_map(hidden, hidden.size(1), BM), mb = head_map(weight, weight.size(1), p.bn);
+  const CUtensorMap ma = head_map(hidden, hidden.size(1), R::kRows), mb = head_map(weight, weight.size(1), p.bn);
   const int64_t tiles = static_cast<int64_t>((p.M + BM - 1) / BM) * ((p.N + p.bn - 1) / p.bn);
   TDSV_CHECK(tiles < (int64_t(1) << 30), "linear_token_statistics: too many tiles");
   const int grid = static_cast<int>(std::min<int64_t>(num_sms(), tiles));
   void* args[] = {const_cast<CUtensorMap*>(&ma), const_cast<CUtensorMap*>(&mb), const_cast<CUtensorMap*>(&mc), &p};
-  TDSV_CUDA_CHECK(cudaLaunchKernel(reinterpret_cast<const void*>(kern), dim3(grid), dim3(kThreads), args, kSmemBytes,
+  TDSV_CUDA_CHECK(cudaLaunchKernel(reinterpret_cast<const void*>(kern), dim3(grid), dim3(kThreads), args, R::kSmemBytes,
                                    stream()));
 }
 
@@ -550,8 +564,9 @@ std::vector<at::Tensor> lm_head_stats_fwd(const at::Tensor& hidden_in, const at:
   p.part = reinterpret_cast<float4*>(part.data_ptr<float>());
   p.target_logit = part.data_ptr<float>() + 4 * tiles * rows;
   const CUtensorMap unused{};
-  if (keep) launch_head<kStatsKeep>(hidden, weight, head_map(logits, (vocab + 7) / 8 * 8, 32), p);
-  else launch_head<kStats>(hidden, weight, unused, p);
+  if (keep) launch_head<kStatsKeep, false>(hidden, weight, head_map(logits, (vocab + 7) / 8 * 8, 32), p);
+  else if (rows <= Ring<true>::kRows) launch_head<kStats, true>(hidden, weight, unused, p);
+  else launch_head<kStats, false>(hidden, weight, unused, p);
   lm_head_join_kernel<<<static_cast<unsigned>((rows + kJoinRows - 1) / kJoinRows), kJoinThreads, 0, stream()>>>(
       p, where.defined() ? where.data_ptr<int>() : nullptr, static_cast<int>(tiles), log_probs.data_ptr<float>(),
       entropy.data_ptr<float>(), save ? reinterpret_cast<float4*>(saved.data_ptr<float>()) : nullptr);
@@ -599,7 +614,7 @@ at::Tensor lm_head_stats_bwd(const at::Tensor& hidden, const at::Tensor& weight,
     TDSV_LAUNCH_CHECK();
     return dlogits;
   }
-  launch_head<kGrad>(hidden, weight, head_map(dlogits, pitch, 32), p);
+  launch_head<kGrad, false>(hidden, weight, head_map(dlogits, pitch, 32), p);
   return dlogits;
 }
 
