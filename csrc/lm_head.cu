@@ -482,6 +482,9 @@ void check_head(const at::Tensor& hidden, const at::Tensor& weight, const at::Te
   TDSV_CHECK(hidden.scalar_type() == at::kBFloat16 && weight.scalar_type() == at::kBFloat16,
              "linear_token_statistics: bf16 hidden and weight");
   TDSV_CHECK(hidden.size(1) % 8 == 0 && hidden.size(1) > 0, "linear_token_statistics: K must be a multiple of 8");
+  // (every reader of both, the gather of the kept rows among them, moves 16 bytes at a time)
+  TDSV_CHECK(reinterpret_cast<uintptr_t>(hidden.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(weight.data_ptr()) % 16 == 0,
+             "linear_token_statistics: hidden and weight must start on 16-byte boundaries");
   TDSV_CHECK(targets.scalar_type() == at::kLong && targets.numel() == hidden.size(0),
              "linear_token_statistics: int64 targets, one per row");
   TDSV_CHECK(weight.size(0) >= 1 && weight.size(0) < (1 << 30) && hidden.size(0) < (1 << 30),

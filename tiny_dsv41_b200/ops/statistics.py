@@ -174,6 +174,11 @@ def token_statistics(logits: torch.Tensor, targets: torch.Tensor | None = None, 
 
 
 # -- statistics of the LM head's product ------------------------------------------------------------
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """``x``, or a copy where it starts inside a 16-byte unit (a view at an odd offset), which TMA cannot read."""
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
 class _LinearTokenStatistics(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, temperature):
@@ -237,8 +242,8 @@ def linear_token_statistics(hidden: torch.Tensor, weight: torch.Tensor, targets:
     if not (on_gpu(hidden) and hidden.dtype == weight.dtype == torch.bfloat16 and hidden.shape[-1] % 8 == 0):
         logits = F.linear(hidden, weight.to(hidden.dtype))
         return token_statistics(logits, targets, temperature=temperature)
-    flat = hidden.reshape(-1, hidden.shape[-1]).contiguous()
-    weight, targets = weight.contiguous(), targets.reshape(-1).contiguous()
+    flat = _aligned(hidden.reshape(-1, hidden.shape[-1]).contiguous())
+    weight, targets = _aligned(weight.contiguous()), targets.reshape(-1).contiguous()
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         lp, entropy = _LinearTokenStatistics.apply(flat, weight, targets, temperature)
     else:
