@@ -381,7 +381,16 @@ __global__ void __launch_bounds__(kStatThreads, 4)
       }
       // after 2, 4, 8, ... batches a warp, another each time, raises the threshold; the others go on meanwhile
       if (batch > 0 && ((batch + 1) & batch) == 0 && from + 2 * kBatch < v1 && tid >> 5 == (__ffs(batch + 1) & 7)) {
-        const int n = min(*const_cast<volatile int*>(&sc.n), kCandidates);
+        // (other warps add candidates and may raise the threshold meanwhile: one lane reads both for the warp, whose
+        // branches and reductions have to be the same for every lane)
+        __syncwarp();
+        int n = 0;
+        if ((tid & 31) == 0) {
+          n = min(*const_cast<volatile int*>(&sc.n), kCandidates);
+          threshold = *const_cast<volatile float*>(&sc.threshold);
+        }
+        n = __shfl_sync(0xffffffffu, n, 0);
+        threshold = __shfl_sync(0xffffffffu, threshold, 0);
         if (n > top) {
           const uint32_t* keys = reinterpret_cast<const uint32_t*>(top_smem) + 1;
           int kept;

@@ -67,3 +67,26 @@ def test_head_operands_at_odd_addresses(rows):
         trained = ops.linear_token_statistics(h, w, targets)
         trained.log_probs.sum().backward()
         assert h.grad.shape == h.shape and w.grad.shape == w.shape and bool(h.grad.isfinite().all())
+
+
+# -- alternatives -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,rows,vocab", [(torch.bfloat16, 640, 70001), (torch.float32, 600, 33003),
+                                              (torch.float16, 700, 40000), (torch.bfloat16, 3, 151936)])
+@pytest.mark.parametrize("top", [1, 20, 128])
+def test_alternatives_while_candidates_arrive(device, dtype, rows, vocab, top):
+    """Rows that keep adding candidates while a threshold is raised over them: rising in part, in steps, everywhere."""
+    if device == "cpu":
+        rows = min(rows, 8)
+    x = torch.randn(rows, vocab, generator=_generator(vocab))
+    ramp = torch.arange(vocab) / vocab
+    x[0::4] += 12.0 * ramp                                    # each batch holds larger values than the one before
+    x[1::4] = (x[1::4] + 8.0 * ramp).round()                  # ... with many equal ones
+    x[2::8] = 40.0 * ramp                                     # rising throughout: the candidates do not fit
+    x[2::8, ::97] = -INF
+    x = x.to(dtype).to(device)
+    got = ops.token_statistics(x, top=top)
+    order = torch.sort(x.float(), dim=-1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(got.top_ids, order)
+    want = torch.log_softmax(x.double(), -1).gather(-1, order)
+    assert bool(((got.top_log_probs - want).abs() <= 1e-5 + 1e-6 * want.abs()).all())
