@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kStatThreads, 4)
                      float4* __restrict__ saved, int* status) {
   namespace cg = cooperative_groups;
   constexpr int kSize = LogitVec<T>::kSize;
-  extern __shared__ uint64_t top_smem[];  // [kCandidates], then [blocks of the cluster][kKept]
+  extern __shared__ __align__(16) uint64_t top_smem[];  // [kCandidates], then [blocks of the cluster][kKept]
   __shared__ JoinScratch<kStatThreads> scratch;
   __shared__ RowStats parts[kMaxCluster];
   __shared__ TopScratch sc;
