@@ -337,14 +337,24 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
     RowStats chosen;
     chosen.m = plan.chosen_m, chosen.s = plan.chosen_s;
     const bool repeated = __any_sync(0xffffffffu, lane < blocks && repeats[lane] != 0);
-    if (repeated) {  // the first place of an id counts
+    double merged = 0.0;
+    if (repeated) {  // one token: the first place of an id counts, with the mass of all of its places
       chosen.s = 0.f;
       for (int a = lane; a < k; a += 32) {
         bool counts = at[a] >= 0;
-        for (int i = 0; i < a && counts; ++i) counts = at[i] != at[a];
+        float mass = 0.f;
+        for (int i = 0; i < k; ++i) {
+          if (at[i] != at[a]) continue;
+          counts &= i >= a;
+          mass += q_s[i];
+        }
         if (counts) chosen.s += e_s[a];
+        // q_gap has a term q_k ln q_k for each place; the token's is q ln q, its places' q_k ln q in sum
+        if (q_s[a] > 0.f) merged += q_s[a] * log(static_cast<double>(mass) / q_s[a]);
       }
       chosen.s = warp_sum(chosen.s);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) merged += __shfl_xor_sync(0xffffffffu, merged, o);
     }
     RowStats all = chosen;
     all.merge(rest, c2);
@@ -362,7 +372,7 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
     if (q_sum > 0.f) {  // (a masked token with mass: q_gap is +inf)
       const double log_chosen = repeated ? log(static_cast<double>(chosen.s)) : plan.log_chosen;
       loss = chosen.s == 0.f ? INFINITY
-                             : static_cast<float>(plan.q_gap + q_sum * (log_chosen - log_mass(p_chosen, chosen)));
+                             : static_cast<float>(plan.q_gap + merged + q_sum * (log_chosen - log_mass(p_chosen, chosen)));
     }
     if (q_rest > 0.f) loss += q_rest * (logf(q_rest) - log_mass(p_rest, rest));
     const bool empty = all.s == 0.f;  // every logit is masked: no distribution, no gradient

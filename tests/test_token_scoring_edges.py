@@ -90,3 +90,109 @@ def test_alternatives_while_candidates_arrive(device, dtype, rows, vocab, top):
     assert torch.equal(got.top_ids, order)
     want = torch.log_softmax(x.double(), -1).gather(-1, order)
     assert bool(((got.top_log_probs - want).abs() <= 1e-5 + 1e-6 * want.abs()).all())
+
+
+# -- distillation -----------------------------------------------------------------------------------
+def _distillation(logits, ids, teacher, weights, temperature, tail):
+    """(rows' divergences, gradient) over the vocabulary: a token's mass is the sum of its places'."""
+    x, ids, t = logits.detach().double().cpu(), ids.cpu().long(), teacher.double().cpu()
+    there, at = ids >= 0, ids.cpu().clamp(min=0)
+    q = torch.zeros_like(x).scatter_add_(-1, at, t.exp().masked_fill(~there, 0.0))
+    inside = torch.zeros_like(x).scatter_add_(-1, at, there.double()) > 0
+    read = inside.any(-1) if tail else q.sum(-1) > 0
+    lp = torch.log_softmax(x / temperature, -1)
+    p, left = lp.exp(), lp.masked_fill(inside, -INF).logsumexp(-1)
+    rest = torch.zeros(len(x), dtype=torch.float64)
+    if tail:
+        rest = torch.where(left > -INF, (1 - q.sum(-1)).clamp(min=0), rest)
+    else:
+        q = q / torch.where(read, q.sum(-1), 1.0)[:, None]
+    rows = torch.where(q > 0, q * (q.log() - lp), 0.0).sum(-1)
+    rows = (rows + torch.where(rest > 0, rest * (rest.log() - left), 0.0)).masked_fill(~read, 0.0)
+    outside = torch.where((rest > 0)[:, None] & ~inside, (lp - left[:, None]).exp() * rest[:, None], 0.0)
+    grad = (q.sum(-1) + rest)[:, None] * p - q - outside
+    return rows, grad.masked_fill(~read[:, None], 0.0) * (weights.double().cpu() / temperature)[:, None]
+
+
+def _close_gradient(got, want, relative=2e-5):
+    """Within `relative` of the row's largest value, and half a unit in the last place of the type."""
+    dtype, got = got.dtype, got.double().cpu()
+    half_unit = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float64: 0.0}[dtype]
+    bound = relative * want.abs().amax(-1, keepdim=True) + half_unit * want.abs()
+    if dtype == torch.float16:
+        bound = bound + 2.0 ** -25
+    assert bool(((got - want).abs() <= bound + 1e-30).all()), ((got - want).abs() / (bound + 1e-30)).max()
+
+
+def _close_loss(got, want):
+    got = got.detach().double().cpu()
+    assert bool(((got - want).abs() <= 1e-4 + 1e-5 * want.abs()).all()), (got - want).abs().max()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("vocab,k", [(9, 7), (2051, 6), (2051, 128), (151936, 64)])
+def test_repeated_alternatives_are_one_token(device, dtype, tail, vocab, k):
+    g = _generator(vocab + k)
+    rows = 6
+    logits = (torch.randn(rows, vocab, generator=g) * 3).to(dtype).to(device)
+    logits[2] = 0.0
+    teacher = torch.log_softmax(torch.randn(rows, k, generator=g), -1) - 0.2
+    ids = torch.randint(0, max(2, k // 2), (rows, k), generator=g) * (vocab // k)
+    ids[1] = vocab - 1                        # one token throughout
+    ids[2, : min(k, 6)] = torch.tensor([7, 7, 8, -1, 8, 7])[:k]
+    ids[3, 1:] = -1                           # nothing repeated but the absent
+    teacher[4, ::2] = -INF                    # places without mass
+    weights = torch.rand(rows, generator=g)
+    leaf = logits.clone().requires_grad_()
+    loss = ops.distillation_loss(leaf, ids.to(device), teacher.to(device), weights.to(device), temperature=1.3, tail=tail)
+    want, want_grad = _distillation(logits, ids, teacher, weights, 1.3, tail)
+    _close_loss(loss.rows, want)
+    assert bool((loss.rows >= -1e-6).all())   # a divergence
+    grad, = torch.autograd.grad(loss.total, leaf)
+    _close_gradient(grad, want_grad)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_repeated_alternatives_of_an_equal_student(device):
+    """A teacher equal to the student with a token recorded as two halves is at distance zero."""
+    logits = torch.zeros(2, 8, device=device)
+    ids = torch.tensor([[3, 3, 5], [3, 5, -1]], device=device)
+    share = torch.tensor([[1 / 16, 1 / 16, 1 / 8], [1 / 8, 1 / 8, 0.0]], device=device)
+    rows = ops.distillation_loss(logits, ids, share.log(), tail=True).rows
+    assert bool((rows.abs() < 1e-6).all())
+    one = ops.distillation_loss(torch.tensor([[-INF, 2.0]], device=device), torch.tensor([[1, 1]], device=device),
+                                torch.full((1, 2), 0.5, device=device).log())
+    assert abs(float(one.rows)) < 1e-6
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("tail", [False, True])
+def test_distillation_of_special_rows(device, tail):
+    """Rows at which a maximum, a mask or a mass can go wrong, repeated ids among them."""
+    vocab, g = 2051, _generator(60)
+    x = torch.randn(12, vocab, generator=g) * 3
+    x[1, 1:] = -INF                             # one token left
+    x[2] = 0.0
+    x[3] = torch.arange(vocab) * 0.01
+    x[4] += 1.0e4
+    x[5, ::2] = -INF
+    x[6, 5:] = -1.0e4
+    x[7, -1] = 80.0
+    x[8, :-6] -= 200.0                          # the student's mass is all on the alternatives
+    ids = torch.stack([torch.randperm(vocab, generator=g)[:6] for _ in range(12)])
+    teacher = torch.log_softmax(torch.randn(12, 6, generator=g), -1) - 0.2
+    ids[1, 0], ids[7, 0], ids[8] = 0, vocab - 1, torch.arange(vocab - 6, vocab)
+    ids[1, 1:], ids[5] = -1, torch.arange(1, 13, 2)
+    ids[2] = torch.tensor([7, 7, 9, -1, 9, 7])
+    teacher[3, 2:] = -INF
+    teacher[9] -= 60.0                          # nearly all of the teacher's mass in the tail
+    teacher[10] = -0.7                          # more than one in all
+    weights = torch.linspace(0.1, 1.0, 12)
+    leaf = x.to(device).requires_grad_()
+    loss = ops.distillation_loss(leaf, ids.to(device), teacher.to(device), weights.to(device), tail=tail)
+    want, want_grad = _distillation(x, ids, teacher, weights, 1.0, tail)
+    _close_loss(loss.rows, want)
+    grad, = torch.autograd.grad(loss.total, leaf)
+    _close_gradient(grad, want_grad)

@@ -108,6 +108,9 @@ def _distillation_reference(logits, ids, teacher, weights, temperature, tail) ->
         log_q = torch.log_softmax(t, dim=-1)
         q = log_q.exp()
     chosen = lp.gather(-1, at)
+    # the mass of a token recorded more than once is the sum of its places'
+    mass = torch.zeros_like(x).scatter_add_(-1, at, q).gather(-1, at)
+    log_q = torch.where(mass == q, log_q, mass.log())
     rows = torch.where(q > 0, q * (log_q.masked_fill(q == 0, 0.0) - chosen), torch.zeros_like(q)).sum(-1)
     if tail:
         inside = torch.zeros_like(x).scatter_add_(-1, at, there.to(x.dtype)) > 0
