@@ -483,8 +483,8 @@ std::vector<at::Tensor> distill_fwd(const at::Tensor& logits_in, const at::Tenso
   }
   const auto f32 = logits.options().dtype(at::kFloat);
   auto row_loss = at::empty(logits.sizes().slice(0, logits.dim() - 1), f32);
-  auto weighted = at::empty({rows + 1}, f32);  // each row's share of the total, and the total
-  auto total = weighted.select(0, rows);
+  auto weighted = at::empty({rows}, f32);  // each row's share of the total
+  auto total = at::empty({}, f32);         // (no view: autograd refuses to update a Function's view in place)
   auto dlogits = grad ? at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous))
                       : at::Tensor();
   if (rows == 0) return {total.zero_(), row_loss, dlogits};
@@ -533,9 +533,8 @@ std::vector<at::Tensor> distill_fwd(const at::Tensor& logits_in, const at::Tenso
     else with_ids(static_cast<int32_t*>(nullptr));
   });
   TDSV_LAUNCH_CHECK();
-  const float* shares = weighted.data_ptr<float>();
   sum_kernel<<<1, static_cast<unsigned>(std::min<int64_t>(1024, (rows + 31) / 32 * 32)), 0, stream()>>>(
-      shares, rows, weighted.data_ptr<float>() + rows);
+      weighted.data_ptr<float>(), rows, total.data_ptr<float>());
   TDSV_LAUNCH_CHECK();
   return {total, row_loss, dlogits};
 }

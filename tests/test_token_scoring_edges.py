@@ -196,3 +196,28 @@ def test_distillation_of_special_rows(device, tail):
     _close_loss(loss.rows, want)
     grad, = torch.autograd.grad(loss.total, leaf)
     _close_gradient(grad, want_grad)
+
+
+def _pair(rows, vocab, k, seed, dtype=torch.float32):
+    g = _generator(seed)
+    logits = (torch.randn(rows, vocab, generator=g) * 3).to(dtype)
+    values, ids = torch.log_softmax(logits.float() + torch.randn(rows, vocab, generator=g), -1).topk(k, dim=-1)
+    return logits, ids, values
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_distillation_total_is_updated_in_place(device):
+    """A total is a tensor of its own: `total += other` and `total *= factor` are what they are elsewhere."""
+    logits, ids, teacher = _pair(5, 300, 8, 70)
+    _, want = _distillation(logits, ids, teacher, torch.full((5,), 0.5), 1.0, True)
+    leaf = logits.to(device).requires_grad_()
+    total = ops.distillation_loss(leaf, ids.to(device), teacher.to(device), tail=True).total
+    assert total.shape == () and not total._is_view()
+    total += 1.0
+    total *= 0.5
+    total.backward()
+    _close_gradient(leaf.grad, want)
+    other = ops.token_statistics(leaf, ids[:, 0].to(device), top=2)
+    for x in (other.log_probs, other.entropy, other.top_log_probs):
+        x *= 2.0
+    other.entropy.sum().backward()
