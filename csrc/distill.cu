@@ -17,7 +17,8 @@
 // is formed as sum q p_rest - q_rest p_a, whose terms do not cancel where either has little mass:
 //   dx_i = 2^((x_i - m_r) c2) A,   A = w / T (sum q p_rest - q_rest p_a) / S_r.
 //
-// A row without alternatives (every id negative; without the tail also: no finite t_k) is not read: loss
+// A row of weight zero has its loss reported, but no share of the total and a gradient of zeros, even where its loss
+// is infinite or its logits are NaN. A row without alternatives (every id negative; without the tail also: no finite t_k) is not read: loss
 // 0, zero gradient. Where no token is left outside the alternatives, the tail has no outcome and is
 // dropped. Repeated ids count as one token whose q is the sum.
 #include "logit_rows.cuh"
@@ -43,6 +44,7 @@ struct RowPlan {
   float q_sum, q_rest;                  // the alternatives' mass and the rest
   double q_gap, log_chosen;             // sum q (ln q - ln 2 y) and ln of chosen_s: see the loss below
   float chosen_m, chosen_s;             // the student's sum over the alternatives
+  int masked;                           // a weight of zero: no share of the total and no gradient, whatever the row holds
   float base;                           // reference of the pass that writes the gradient
   float outside;                        // A above
 };
@@ -392,7 +394,8 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
       }
     }
     if (lane == 0) {
-      if (part == 0) rows_out[r] = loss, weighted[r] = w * loss;
+      if (part == 0) rows_out[r] = loss, weighted[r] = w == 0.f ? 0.f : w * loss;  // (a loss may be infinite or NaN)
+      plan.masked = w == 0.f;
       plan.base = rest.s == 0.f ? 0.f : rest.m;  // (every other logit is -inf there)
       plan.outside = plan.bad ? NAN : outside;
     }
@@ -400,6 +403,7 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
   if constexpr (GRAD) {
     __syncthreads();
     T* out = dlogits + r * v;
+    if (plan.masked) return write_zeros<T, kDistillThreads>(out + first, last - first);
     write_gradient<T, kDistillThreads, true, 1>(kept_values, out + first, last - first, plan.base, c2, plan.outside, 0.f);
     __syncthreads();
     if (tid < k && at[tid] >= first && at[tid] < last) out[at[tid]] = from_float<T>(e_s[tid]);

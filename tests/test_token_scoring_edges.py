@@ -221,3 +221,26 @@ def test_distillation_total_is_updated_in_place(device):
     for x in (other.log_probs, other.entropy, other.top_log_probs):
         x *= 2.0
     other.entropy.sum().backward()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("vocab", [300, 40003])
+def test_a_weight_of_zero_masks_its_row(device, dtype, tail, vocab):
+    logits, ids, teacher = _pair(8, vocab, 8, 71, dtype)
+    weights = torch.tensor([0.5, 0.0, 0.0, 0.0, 0.25, 0.0, -0.0, 1.0])
+    want, want_grad = _distillation(logits, ids, teacher, weights, 1.0, tail)
+    logits[1] = -INF                       # no distribution
+    logits[2] = float("nan")
+    logits[3, ids[3, 0]] = -INF            # the teacher's first alternative is impossible: infinite
+    logits[5, 17] = INF
+    leaf = logits.to(device).requires_grad_()
+    loss = ops.distillation_loss(leaf, ids.to(device), teacher.to(device), weights.to(device), tail=tail)
+    loss.total.backward()
+    off = weights == 0
+    _close_loss(loss.total, (want * weights.double()).sum())
+    _close_gradient(leaf.grad, want_grad)
+    assert bool((leaf.grad[off.to(device)] == 0).all())
+    _close_loss(loss.rows[[0, 4, 6, 7]], want[[0, 4, 6, 7]])   # a masked row's divergence is reported
+    assert loss.rows[1] == INF and loss.rows[3] == INF and bool(loss.rows[2].isnan()) and bool(loss.rows[5].isnan())

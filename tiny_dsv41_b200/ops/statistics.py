@@ -97,6 +97,8 @@ def _distillation_reference(logits, ids, teacher, weights, temperature, tail) ->
     x = logits.double()
     if bool((ids >= x.shape[-1]).any()):
         raise ValueError("teacher id outside the vocabulary")
+    off = torch.zeros(x.shape[:-1], dtype=torch.bool) if weights is None else weights == 0
+    x = torch.where(off.unsqueeze(-1), x.detach(), x)  # no gradient, whatever such a row holds
     there, at = ids >= 0, ids.clamp(min=0).long()
     t = teacher.to(x.dtype).masked_fill(~there, float("-inf"))
     used = there.any(-1) if tail else (t > float("-inf")).any(-1) | t.isnan().any(-1)
@@ -123,7 +125,7 @@ def _distillation_reference(logits, ids, teacher, weights, temperature, tail) ->
                                   torch.zeros_like(rest))
     rows = rows.masked_fill(~used, 0.0).masked_fill(used & empty, float("inf"))
     w = torch.ones_like(rows) if weights is None else weights.to(rows.dtype)
-    total, rows = (w * rows).sum(), rows.detach()
+    total, rows = (w * rows).masked_fill(off, 0.0).sum(), rows.detach()
     return DistillationLoss(total, rows) if logits.dtype == torch.float64 else DistillationLoss(total.float(), rows.float())
 
 
@@ -284,10 +286,12 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     they are and compares the rest of the mass with the student's mass outside the K tokens. A negative
     id is no alternative, and a row without any has loss 0 and zero gradient and is not read. Repeated
     ids count as one token. ``weights`` (fp32, one per row; 1 by default) carry masks and the
-    normalisation, e.g. 1 / tokens: the gradient is written in the same pass over the logits as the loss,
-    so a factor applied to ``total`` afterwards costs another pass. Because that gradient is handed over
-    on ``backward``, the operator is called again for a second one. Teacher, ids and weights take no
-    gradient. On a GPU an id beyond the vocabulary gives NaN and sets the device status."""
+    normalisation, e.g. 1 / tokens: a weight of 0 leaves its row out of the total and gives it a gradient of
+    zeros, even where its divergence is infinite or its logits are NaN (``rows`` reports it all the same).
+    The gradient is written in the same pass over the logits as the loss, so a factor applied to ``total``
+    afterwards costs another pass. Because that gradient is handed over on ``backward``, the operator is
+    called again for a second one. Teacher, ids and weights take no gradient. On a GPU an id beyond the
+    vocabulary gives NaN and sets the device status."""
     _check_logits(logits)
     temperature = _check_temperature(temperature)
     shape = logits.shape[:-1]
