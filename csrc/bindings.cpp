@@ -99,7 +99,8 @@ at::Tensor lm_head_stats_bwd(const at::Tensor& hidden, const at::Tensor& weight,
 // distill.cu
 std::vector<at::Tensor> distill_fwd(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher,
                                     const c10::optional<at::Tensor>& weights, double temperature, bool tail, bool grad);
-void distill_scale(at::Tensor& dlogits, const at::Tensor& factor);
+void distill_again(at::Tensor& dlogits, const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& saved,
+                   const at::Tensor& factor, double temperature);
 // optim.cu
 void adamw_step(at::Tensor& master, const at::Tensor& grad, at::Tensor& m, at::Tensor& v,
                 const c10::optional<at::Tensor>& out, double lr, double beta1, double beta2, double eps,
@@ -229,7 +230,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("lm_head_stats_fwd", &tdsv::lm_head_stats_fwd, "token statistics fused with the LM head's product");
   m.def("lm_head_stats_bwd", &tdsv::lm_head_stats_bwd);
   m.def("distill_fwd", &tdsv::distill_fwd, "KL from a teacher's top alternatives, with its gradient");
-  m.def("distill_scale", &tdsv::distill_scale);
+  m.def("distill_again", &tdsv::distill_again, "the gradient of distill_fwd for an upstream gradient other than one");
   m.def("adamw_step", &tdsv::adamw_step, py::arg("master"), py::arg("grad"), py::arg("m"), py::arg("v"),
         py::arg("out"), py::arg("lr"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"),
         py::arg("step"), py::arg("grad_scale"), py::arg("grad_scale_t"), py::arg("step_t") = py::none(),

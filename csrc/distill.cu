@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
     distill_kernel(const T* __restrict__ logits, RowLayout layout, int v, const I* __restrict__ ids,
                    const float* __restrict__ teacher, int k, const float* __restrict__ weights, float c2, float inv_t,
                    bool tail, float* __restrict__ rows_out, float* __restrict__ weighted, T* __restrict__ dlogits,
-                   int* status) {
+                   float2* __restrict__ saved, float* __restrict__ saved_chosen, int* status) {
   namespace cg = cooperative_groups;
   constexpr int kSize = LogitVec<T>::kSize;
   extern __shared__ uint4 smem[];  // GRAD: the stretch (one vector ahead of it, one after); then its bitmap
@@ -250,6 +250,7 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
   if (!plan.read) {  // the same for the whole cluster
     if (tid == 0 && part == 0) rows_out[r] = 0.f, weighted[r] = 0.f;
     if (GRAD) {
+      if (tid == 0 && part == 0) saved[r] = make_float2(INFINITY, 0.f);
       if (plan.copied) mbar_wait(&arrived, 0, status, kTimeoutFull);
       write_zeros<T, kDistillThreads>(dlogits + r * v + first, last - first);
     }
@@ -389,8 +390,9 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
           mass = 0.f;
           for (int i = 0; i < k; ++i) mass += at[i] == at[a] ? q_s[i] : 0.f;
         }
-        const float d = empty ? 0.f : scale * (whole * (e_s[a] * to_p) - mass);
-        e_s[a] = plan.bad ? NAN : d;
+        const float d = plan.bad ? NAN : empty ? 0.f : scale * (whole * (e_s[a] * to_p) - mass);
+        e_s[a] = d;
+        if (part == 0) saved_chosen[r * k + a] = d;
       }
     }
     if (lane == 0) {
@@ -398,6 +400,7 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
       plan.masked = w == 0.f;
       plan.base = rest.s == 0.f ? 0.f : rest.m;  // (every other logit is -inf there)
       plan.outside = plan.bad ? NAN : outside;
+      if (GRAD && part == 0) saved[r] = make_float2(w == 0.f ? INFINITY : plan.base, plan.outside);
     }
   }
   if constexpr (GRAD) {
@@ -419,28 +422,34 @@ __global__ void __launch_bounds__(1024) sum_kernel(const float* __restrict__ x, 
   if (threadIdx.x == 0) *total = s;
 }
 
-// x *= *factor, unless it is one: the gradient was written for an upstream gradient of one. x is an
-// allocation's start, so its vectors are aligned.
-template <typename T>
-__global__ void scale_kernel(T* __restrict__ x, int64_t n, const float* __restrict__ factor) {
+// The gradient once more, for an upstream gradient other than one: from the logits, the reference and the constant A of
+// each row and the unrounded gradients of its alternatives, so that it is rounded once and an fp16 loss scale meets the
+// values before they are lost (w = 1 / 4096 puts every p below 1e-4 under fp16's smallest step). One read and one write of
+// the logits, as scaling the rounded gradient would be. A reference of infinity marks a row whose zeros (or NaN) stay.
+constexpr int kAgainBytes = 32768;
+template <typename T, typename I>
+__global__ void __launch_bounds__(kDistillThreads)
+    distill_again_kernel(const T* __restrict__ logits, RowLayout layout, int v, int64_t items, int parts,
+                         const I* __restrict__ ids, int k, const float2* __restrict__ saved,
+                         const float* __restrict__ saved_chosen, const float* __restrict__ factor, float c2,
+                         T* __restrict__ dlogits) {
+  constexpr int kStretch = kAgainBytes / static_cast<int>(sizeof(T));
   const float f = *factor;
   if (f == 1.f) return;
-  const int64_t vecs = n / LogitVec<T>::kSize, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  const int64_t me = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  uint4* xv = reinterpret_cast<uint4*>(x);
-  for (int64_t i = me; i < vecs; i += step) {
-    const uint4 v = xv[i];
-    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int p = 0; p < LogitVec<T>::kPairs; ++p) {
-      const float2 d = unpack_pair<T>(v, p);
-      if constexpr (sizeof(T) == 2) w[p] = pack_pair<T>(d.x * f, d.y * f);
-      else w[2 * p] = __float_as_uint(d.x * f), w[2 * p + 1] = __float_as_uint(d.y * f);
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t r = item / parts;
+    const int first = static_cast<int>(item - r * parts) * kStretch, n = min(kStretch, v - first);
+    const float2 s = saved[r];
+    if (s.x == INFINITY) continue;
+    T* out = dlogits + r * v;
+    write_gradient<T, kDistillThreads, true, 4>(logits + layout.offset(static_cast<uint32_t>(r)) + first, out + first, n,
+                                                s.x, c2, f * s.y, 0.f);
+    __syncthreads();
+    for (int j = threadIdx.x; j < k; j += kDistillThreads) {
+      const int64_t id = static_cast<int64_t>(ids[r * k + j]);
+      if (id >= first && id < first + n) out[id] = from_float<T>(f * saved_chosen[r * k + j]);
     }
-    xv[i] = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  const int64_t i = vecs * LogitVec<T>::kSize + me;
-  if (i < n) x[i] = from_float<T>(to_float<T>(x[i]) * f);
 }
 
 constexpr int kMostShared = 200 * 1024;
@@ -459,7 +468,8 @@ int blocks_per_row(int64_t rows, int64_t vocab, int64_t item, bool grad) {
 
 }  // namespace
 
-// (total [], the rows' divergences, the gradient like logits, or undefined where it is not asked for).
+// (total [], the rows' divergences, the gradient like logits, what distill_again needs); the last two are undefined
+// where no gradient is asked for.
 std::vector<at::Tensor> distill_fwd(const at::Tensor& logits_in, const at::Tensor& ids, const at::Tensor& teacher,
                                     const c10::optional<at::Tensor>& weights, double temperature, bool tail, bool grad) {
   check_logits(logits_in, "distillation_loss");
@@ -491,8 +501,9 @@ std::vector<at::Tensor> distill_fwd(const at::Tensor& logits_in, const at::Tenso
   auto total = at::empty({}, f32);         // (no view: autograd refuses to update a Function's view in place)
   auto dlogits = grad ? at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous))
                       : at::Tensor();
-  if (rows == 0) return {total.zero_(), row_loss, dlogits};
   const int k = static_cast<int>(ids.size(-1));
+  auto saved = grad ? at::empty({rows * (k + 2)}, f32) : at::Tensor();  // per row: reference and A; then its alternatives
+  if (rows == 0) return {total.zero_(), row_loss, dlogits, saved};
   const int item = static_cast<int>(logits.element_size());
   const int blocks = blocks_per_row(rows, vocab, item, grad);
   // the largest stretch of a block: its vectors, one ahead and one after, and a bit for each value
@@ -526,7 +537,8 @@ std::vector<at::Tensor> distill_fwd(const at::Tensor& logits_in, const at::Tenso
         static_cast<const I*>(ids.data_ptr<I>()), static_cast<const float*>(teacher.data_ptr<float>()), k,
         static_cast<const float*>(weighted_rows ? weights->data_ptr<float>() : nullptr), c2, inv_t, tail,
         row_loss.data_ptr<float>(), weighted.data_ptr<float>(), grad ? static_cast<T*>(dlogits.data_ptr()) : nullptr,
-        status_word_ptr()));
+        grad ? reinterpret_cast<float2*>(saved.data_ptr<float>()) : nullptr,
+        grad ? saved.data_ptr<float>() + 2 * rows : nullptr, status_word_ptr()));
   };
   with_logit_type(logits.scalar_type(), [&](auto* tag) {
     auto with_ids = [&](auto* itag) {
@@ -540,21 +552,47 @@ std::vector<at::Tensor> distill_fwd(const at::Tensor& logits_in, const at::Tenso
   sum_kernel<<<1, static_cast<unsigned>(std::min<int64_t>(1024, (rows + 31) / 32 * 32)), 0, stream()>>>(
       weighted.data_ptr<float>(), rows, total.data_ptr<float>());
   TDSV_LAUNCH_CHECK();
-  return {total, row_loss, dlogits};
+  return {total, row_loss, dlogits, saved};
 }
 
-// dlogits *= factor (a device scalar), in place; nothing is touched where it is one.
-void distill_scale(at::Tensor& dlogits, const at::Tensor& factor) {
+// dlogits for an upstream gradient of `factor` (a device scalar), in place; nothing is touched where it is one.
+void distill_again(at::Tensor& dlogits, const at::Tensor& logits_in, const at::Tensor& ids, const at::Tensor& saved,
+                   const at::Tensor& factor, double temperature) {
+  check_logits(logits_in, "distillation_loss");
+  const int64_t vocab = logits_in.size(-1), rows = logits_in.numel() / vocab;
   check_cuda_tensor(dlogits, "dlogits");
+  check_cuda_tensor(ids, "teacher_ids");
+  check_cuda_tensor(saved, "saved");
   check_cuda_tensor(factor, "gradient");
+  TDSV_CHECK(dlogits.sizes() == logits_in.sizes() && dlogits.scalar_type() == logits_in.scalar_type(),
+             "distillation_loss: gradient like the logits");
   TDSV_CHECK(factor.scalar_type() == at::kFloat && factor.numel() == 1, "distillation_loss: fp32 scalar gradient");
-  const int64_t n = dlogits.numel();
-  if (n == 0) return;
-  c10::cuda::CUDAGuard guard(dlogits.device());
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n + 2047) / 2048, 8 * num_sms()));
-  with_logit_type(dlogits.scalar_type(), [&](auto* tag) {
+  if (rows == 0) return;
+  const int k = static_cast<int>(ids.size(-1));
+  TDSV_CHECK(ids.numel() == rows * k && saved.scalar_type() == at::kFloat && saved.numel() == rows * (k + 2),
+             "distillation_loss: saved rows");
+  c10::cuda::CUDAGuard guard(logits_in.device());
+  RowLayout layout;
+  at::Tensor logits = logits_in;
+  if (!row_layout(logits, layout)) {
+    logits = logits.contiguous();
+    TDSV_CHECK(row_layout(logits, layout), "distillation_loss: logits layout");
+  }
+  const float c2 = static_cast<float>(1.4426950408889634 / temperature);
+  const int64_t stretch = kAgainBytes / logits.element_size(), parts = (vocab + stretch - 1) / stretch;
+  // (eight blocks an SM, so that a factor of one costs a launch and not a pass over the rows)
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(rows * parts, 8 * num_sms()));
+  with_logit_type(logits.scalar_type(), [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    scale_kernel<T><<<grid, 256, 0, stream()>>>(static_cast<T*>(dlogits.data_ptr()), n, factor.data_ptr<float>());
+    auto run = [&](auto* itag) {
+      using I = std::remove_pointer_t<decltype(itag)>;
+      distill_again_kernel<T, I><<<grid, kDistillThreads, 0, stream()>>>(
+          static_cast<const T*>(logits.data_ptr()), layout, static_cast<int>(vocab), rows * parts, static_cast<int>(parts),
+          ids.data_ptr<I>(), k, reinterpret_cast<const float2*>(saved.data_ptr<float>()),
+          saved.data_ptr<float>() + 2 * rows, factor.data_ptr<float>(), c2, static_cast<T*>(dlogits.data_ptr()));
+    };
+    if (ids.scalar_type() == at::kLong) run(static_cast<int64_t*>(nullptr));
+    else run(static_cast<int32_t*>(nullptr));
   });
   TDSV_LAUNCH_CHECK();
 }

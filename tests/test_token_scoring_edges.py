@@ -244,3 +244,49 @@ def test_a_weight_of_zero_masks_its_row(device, dtype, tail, vocab):
     assert bool((leaf.grad[off.to(device)] == 0).all())
     _close_loss(loss.rows[[0, 4, 6, 7]], want[[0, 4, 6, 7]])   # a masked row's divergence is reported
     assert loss.rows[1] == INF and loss.rows[3] == INF and bool(loss.rows[2].isnan()) and bool(loss.rows[5].isnan())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("factor,share", [(65536.0, 1 / 4096), (0.3, 1.0), (0.0, 1.0), (-1.7, 0.5)])
+@pytest.mark.parametrize("vocab", [777, 70001])
+def test_distillation_gradient_is_rounded_after_the_upstream_factor(device, dtype, tail, factor, share, vocab):
+    """One rounding to the logits' type, whatever multiplies the total: a loss scale reaches fp16's small values."""
+    logits, ids, teacher = _pair(7, vocab, 16, 72, dtype)
+    ids[1], ids[2, 8:], ids[3, 1] = -1, -1, ids[3, 0]
+    weights = torch.full((7,), share)
+    weights[4] = 0.0
+    _, want = _distillation(logits, ids, teacher, weights * factor, 1.3, tail)
+    for view in (False, True):
+        leaf = torch.cat((logits, logits[:, :3]), 1).to(device)[:, :vocab] if view else logits.to(device)
+        leaf = leaf.detach().requires_grad_()
+        for i in (ids, ids.int()):
+            loss = ops.distillation_loss(leaf, i.to(device), teacher.to(device), weights.to(device), temperature=1.3, tail=tail)
+            grad, = torch.autograd.grad(loss.total * factor, leaf)
+            _close_gradient(grad, want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_distillation_under_saved_tensor_hooks(device):
+    """What the backward needs is saved where hooks (offloading, checkpointing) see it."""
+    from torch.utils.checkpoint import checkpoint
+
+    logits, ids, teacher = _pair(4, 500, 8, 73)
+    args = (ids.to(device), teacher.to(device))
+    _, want = _distillation(logits, ids, teacher, torch.ones(4), 1.0, True)
+    seen = []
+
+    def pack(x):
+        seen.append(tuple(x.shape))
+        return x.cpu()
+
+    leaf = logits.to(device).requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda x: x.to(device)):
+        total = ops.distillation_loss(leaf, *args, tail=True).total
+    assert (4, 500) in seen
+    total.backward()
+    _close_gradient(leaf.grad, want)
+    leaf.grad = None
+    checkpoint(lambda x: ops.distillation_loss(x, *args, tail=True).total, leaf, use_reentrant=False).backward()
+    _close_gradient(leaf.grad, want)

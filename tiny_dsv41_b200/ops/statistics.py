@@ -260,18 +260,21 @@ def linear_token_statistics(hidden: torch.Tensor, weight: torch.Tensor, targets:
 class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, teacher, weights, temperature, tail):
-        total, rows, ctx.dlogits = ext().distill_fwd(logits, ids, teacher, weights, temperature, tail, True)
+        total, rows, dlogits, saved = ext().distill_fwd(logits, ids, teacher, weights, temperature, tail, True)
+        ctx.save_for_backward(logits, ids, dlogits, saved)
+        ctx.temperature, ctx.handed_out = temperature, False
         ctx.mark_non_differentiable(rows)
         return total, rows
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_total, _g_rows):
-        dlogits, ctx.dlogits = ctx.dlogits, None
-        if dlogits is None:
+        if ctx.handed_out:
             raise RuntimeError("distillation_loss: the gradient was handed out by an earlier backward; call the "
                                "operator again")
-        ext().distill_scale(dlogits, g_total.contiguous())
+        logits, ids, dlogits, saved = ctx.saved_tensors
+        ctx.handed_out = True
+        ext().distill_again(dlogits, logits, ids, saved, g_total.contiguous(), ctx.temperature)
         return dlogits, None, None, None, None, None
 
 
@@ -288,9 +291,10 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     ids count as one token. ``weights`` (fp32, one per row; 1 by default) carry masks and the
     normalisation, e.g. 1 / tokens: a weight of 0 leaves its row out of the total and gives it a gradient of
     zeros, even where its divergence is infinite or its logits are NaN (``rows`` reports it all the same).
-    The gradient is written in the same pass over the logits as the loss, so a factor applied to ``total``
-    afterwards costs another pass. Because that gradient is handed over on ``backward``, the operator is
-    called again for a second one. Teacher, ids and weights take no gradient. On a GPU an id beyond the
+    The gradient is written in the same pass over the logits as the loss, for an upstream gradient of one;
+    for any other (a factor applied to ``total``, a loss scale) ``backward`` writes it once more from the
+    logits, which costs another pass, and rounds it once. Because it is handed over on ``backward``, the
+    operator is called again for a second one. Teacher, ids and weights take no gradient. On a GPU an id beyond the
     vocabulary gives NaN and sets the device status."""
     _check_logits(logits)
     temperature = _check_temperature(temperature)
@@ -316,7 +320,7 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     if logits.requires_grad and torch.is_grad_enabled():
         total, rows = _Distillation.apply(logits, ids, teacher, weights, temperature, tail)
     else:
-        total, rows, _ = ext().distill_fwd(logits, ids, teacher, weights, temperature, tail, False)
+        total, rows, _, _ = ext().distill_fwd(logits, ids, teacher, weights, temperature, tail, False)
     return DistillationLoss(total, rows)
 
 
