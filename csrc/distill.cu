@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
     const float to_p = chosen.s == 0.f ? 0.f : exp2_fast((chosen.m - all.m) * c2) / all.s, p_chosen = chosen.s * to_p;
     const float p_rest = rest.s == 0.f ? 0.f : exp2_fast((rest.m - all.m) * c2) * rest.s / all.s;
     auto log_mass = [&](float p, const RowStats& of) {
-      return p > 1e-30f ? logf(p) : kLn2 * ((of.m - all.m) * c2 + log2f(of.s) - log2f(all.s));
+      return p > 1e-30f ? logf(p) : (of.m - all.m) * inv_t + kLn2 * (log2f(of.s) - log2f(all.s));
     };
     float loss = 0.f;
     if (q_sum > 0.f) {  // (a masked token with mass: q_gap is +inf)

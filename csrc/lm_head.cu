@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     const float log2s = log2f(st.s);
     ent = st.s == 0.f ? 0.f : kLn2 * (log2s - st.w / st.s);
     if (target >= 0 && target < p.N) {
-      lp = st.s == 0.f ? -INFINITY : kLn2 * ((p.target_logit[i] - st.m) * p.c2 - log2s);
+      lp = st.s == 0.f ? -INFINITY : (p.target_logit[i] - st.m) * p.inv_t - kLn2 * log2s;
     } else {
       lp = NAN;
       report_status(p.status, kOutOfBounds);
@@ -544,6 +544,7 @@ std::vector<at::Tensor> lm_head_stats_fwd(const at::Tensor& hidden_in, const at:
   if (rows == 0) return {log_probs, entropy, saved, logits};
   HeadParams p{};
   p.c2 = static_cast<float>(1.4426950408889634 / temperature);
+  p.inv_t = static_cast<float>(1.0 / temperature);
   p.targets = targets.data_ptr<int64_t>();
   p.ignore_index = ignore_index;
   if (!save && rows > 2 * BM) {  // (fewer would hardly save a row block)

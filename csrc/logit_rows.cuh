@@ -6,7 +6,8 @@
 //     S  = sum 2^((x - m) c2)
 //     W  = sum 2^((x - m) c2) (x - m) c2
 // so that  ln sum e^y = m / T + ln S  and the entropy is  ln S - ln 2 * W / S. x - m is formed first
-// and exactly scaled after, so logits of any common offset lose nothing; W is a sum relative to m, so
+// and exactly scaled after, so logits of any common offset lose nothing (a log-probability is (x - m) / T - ln S: in
+// base 2 a token masked by its type's lowest value would leave fp32's range); W is a sum relative to m, so
 // the entropy has no cancellation of large terms. All three are fp32.
 #pragma once
 

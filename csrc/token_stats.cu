@@ -269,7 +269,7 @@ __device__ __noinline__ int collect_again(const T* row, int first, int last, int
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kStatThreads, 4)
     stats_fwd_kernel(const T* __restrict__ logits, RowLayout layout, int v, const int64_t* __restrict__ targets,
-                     int64_t ignore_index, float c2, int top, float* __restrict__ log_probs,
+                     int64_t ignore_index, float c2, float inv_t, int top, float* __restrict__ log_probs,
                      float* __restrict__ entropy, int64_t* __restrict__ top_ids, float* __restrict__ top_lp,
                      float4* __restrict__ saved, int* status) {
   namespace cg = cooperative_groups;
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(kStatThreads, 4)
     }
     __syncthreads();
     const int m = sc.kept_n;
-    const float log2s = log2f(all.s);
+    const float log_s = kLn2 * log2f(all.s);
     for (int j = min(m, top) + tid; j < top; j += kStatThreads) {
       top_ids[r * top + j] = -1;
       top_lp[r * top + j] = -INFINITY;
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kStatThreads, 4)
     rank_kept(sc, m, [&](int rank, uint64_t c) {
       if (rank >= top) return;
       top_ids[r * top + rank] = 0xffffffffu - static_cast<uint32_t>(c);
-      top_lp[r * top + rank] = kLn2 * ((key_value(candidate_key(c)) - all.m) * c2 - log2s);
+      top_lp[r * top + rank] = (key_value(candidate_key(c)) - all.m) * inv_t - log_s;
     });
   }
   if (tid == 0) {
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kStatThreads, 4)
     if (targets != nullptr) {
       float lp = NAN;
       if (target >= 0 && target < v) {
-        lp = all.s == 0.f ? -INFINITY : kLn2 * ((to_float<T>(row[target]) - all.m) * c2 - log2s);
+        lp = all.s == 0.f ? -INFINITY : (to_float<T>(row[target]) - all.m) * inv_t - kLn2 * log2s;
       } else {
         report_status(status, kOutOfBounds);
       }
@@ -606,7 +606,7 @@ std::vector<at::Tensor> token_stats_fwd(const at::Tensor& logits_in, const c10::
   }
   if (save) saved = at::empty({rows, 4}, f32);
   if (rows == 0) return {log_probs, entropy, top_ids, top_lp, saved};
-  const float c2 = static_cast<float>(1.4426950408889634 / temperature);
+  const float c2 = static_cast<float>(1.4426950408889634 / temperature), inv_t = static_cast<float>(1.0 / temperature);
   const int blocks = blocks_per_row(rows, vocab, logits.element_size());
   with_logit_type(logits.scalar_type(), [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
@@ -625,7 +625,7 @@ std::vector<at::Tensor> token_stats_fwd(const at::Tensor& logits_in, const c10::
       TDSV_CUDA_CHECK(cudaLaunchKernelEx(
           &config, kern, static_cast<const T*>(logits.data_ptr()), layout, static_cast<int>(vocab),
           static_cast<const int64_t*>(has_target ? targets->data_ptr<int64_t>() : nullptr), ignore_index, c2,
-          static_cast<int>(top), has_target ? log_probs.data_ptr<float>() : nullptr, entropy.data_ptr<float>(),
+          inv_t, static_cast<int>(top), has_target ? log_probs.data_ptr<float>() : nullptr, entropy.data_ptr<float>(),
           top ? top_ids.data_ptr<int64_t>() : nullptr, top ? top_lp.data_ptr<float>() : nullptr,
           save ? reinterpret_cast<float4*>(saved.data_ptr<float>()) : nullptr, status_word_ptr()));
     };

@@ -290,3 +290,48 @@ def test_distillation_under_saved_tensor_hooks(device):
     leaf.grad = None
     checkpoint(lambda x: ops.distillation_loss(x, *args, tail=True).total, leaf, use_reentrant=False).backward()
     _close_gradient(leaf.grad, want)
+
+
+# -- masks of the type's lowest value ---------------------------------------------------------------
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab", [40, 3001])
+@pytest.mark.parametrize("temperature", [0.5, 1.0, 2.0])
+def test_masks_of_the_lowest_value(device, dtype, vocab, temperature):
+    """A masked token's log-probability is (lowest - m) / T - ln S wherever fp32 holds that, and -inf beyond."""
+    x = torch.randn(5, vocab, generator=_generator(74)) * 3
+    x[:, 6:] = torch.finfo(dtype).min
+    x[2] = torch.finfo(dtype).min
+    x[3, 1:] = torch.finfo(dtype).min
+    x[4, 20:] = -INF
+    x = x.to(dtype).to(device)
+    targets = torch.tensor([vocab - 1, 2, 7, 0, 9], device=device)
+    got = ops.token_statistics(x, targets, temperature=temperature, top=10)
+    lp = torch.log_softmax(x.double() / temperature, -1).float()   # (beyond fp32: -inf)
+    order = torch.sort(x.float(), dim=-1, descending=True, stable=True).indices[:, :10]
+    assert torch.equal(got.top_ids, order)
+    chosen, entropy = _scores(x, targets, temperature)
+    for a, b in ((got.log_probs, chosen.float()), (got.top_log_probs, lp.gather(-1, order).cpu())):
+        a = a.cpu()
+        assert torch.equal(a == -INF, b == -INF), (a, b)
+        fine = b > -INF
+        assert bool(((a - b).abs()[fine] <= 1e-5 + 1e-6 * b.abs()[fine]).all()), (a, b)
+    assert bool(((got.entropy.cpu() - entropy).abs() <= 1e-4).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tail", [False, True])
+def test_distillation_of_tokens_masked_by_the_lowest_value(device, dtype, tail):
+    """A teacher whose alternatives the student masks: a divergence of 1e38 and a gradient of -q, not infinities."""
+    x = torch.randn(3, 600, generator=_generator(75)) * 3
+    x[0, :8] = x[1, 3:8] = torch.finfo(dtype).min
+    x = x.to(dtype)
+    ids, teacher = torch.arange(8).expand(3, 8).contiguous(), torch.full((3, 8), -2.5)
+    want, want_grad = _distillation(x, ids, teacher, torch.ones(3), 1.0, tail)
+    leaf = x.to(device).requires_grad_()
+    loss = ops.distillation_loss(leaf, ids.to(device), teacher.to(device), tail=tail)
+    assert bool(loss.rows.isfinite().all())
+    _close_loss(loss.rows, want)
+    grad, = torch.autograd.grad(loss.total, leaf)
+    _close_gradient(grad, want_grad)
