@@ -9,6 +9,7 @@ smallest step of 6e-8).
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from tiny_dsv41_b200 import ops
 
@@ -335,3 +336,23 @@ def test_distillation_of_tokens_masked_by_the_lowest_value(device, dtype, tail):
     _close_loss(loss.rows, want)
     grad, = torch.autograd.grad(loss.total, leaf)
     _close_gradient(grad, want_grad)
+
+
+# -- autograd ---------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_tangents_are_refused(grad):
+    """The kernels have no forward-mode derivative: a tangent is refused, with gradients on or off, not dropped."""
+    x = torch.randn(3, 64, device="cuda")
+    hidden, weight = torch.randn(3, 64, device="cuda").bfloat16(), torch.randn(100, 64, device="cuda").bfloat16()
+    targets, ids = torch.tensor([1, 2, 3], device="cuda"), torch.tensor([[1], [2], [3]], device="cuda")
+    teacher = torch.zeros(3, 1, device="cuda")
+    calls = ((x, lambda d: ops.token_statistics(d, targets, top=3)),
+             (x, lambda d: ops.distillation_loss(d, ids, teacher)),
+             (hidden, lambda d: ops.linear_token_statistics(d, weight, targets)),
+             (weight, lambda d: ops.linear_token_statistics(hidden, d, targets)))
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        for primal, call in calls:
+            with pytest.raises((RuntimeError, NotImplementedError), match="forward mode|jvp"):
+                call(forward_ad.make_dual(primal, torch.ones_like(primal)))
+        ops.token_statistics(x, targets)

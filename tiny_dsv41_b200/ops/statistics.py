@@ -18,6 +18,7 @@ from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from ._ext import ext, on_gpu
 from .loss import IGNORE_INDEX
@@ -58,6 +59,13 @@ def _check_targets(targets: torch.Tensor, shape, device) -> None:
         raise TypeError("targets must be int64")
     if targets.shape != shape or targets.device != device:
         raise ValueError("targets must hold one token id per row, on the logits' device")
+
+
+def _differentiates(*tensors: torch.Tensor) -> bool:
+    """Whether a call has to go through its autograd function: a gradient is wanted, or a tensor carries a forward-mode
+    tangent, which the function refuses and a direct call would drop in silence."""
+    return (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+            or any(forward_ad.unpack_dual(t).tangent is not None for t in tensors))
 
 
 def _check_logits(logits: torch.Tensor) -> None:
@@ -172,7 +180,7 @@ def token_statistics(logits: torch.Tensor, targets: torch.Tensor | None = None, 
         return _scores_reference(logits, targets, temperature, top)
     if targets is not None:
         targets = targets.contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
+    if _differentiates(logits):
         return TokenStatistics(*_TokenStatistics.apply(logits, targets, temperature, top))
     lp, entropy, ids, values, _ = ext().token_stats_fwd(logits, targets, temperature, top, IGNORE_INDEX, False)
     return TokenStatistics(lp, entropy, ids, values)
@@ -249,7 +257,7 @@ def linear_token_statistics(hidden: torch.Tensor, weight: torch.Tensor, targets:
         return token_statistics(logits, targets, temperature=temperature)
     flat = _aligned(hidden.reshape(-1, hidden.shape[-1]).contiguous())
     weight, targets = _aligned(weight.contiguous()), targets.reshape(-1).contiguous()
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+    if _differentiates(hidden, weight):
         lp, entropy = _LinearTokenStatistics.apply(flat, weight, targets, temperature)
     else:
         lp, entropy, _, _ = ext().lm_head_stats_fwd(flat, weight, targets, temperature, IGNORE_INDEX, False, False)
@@ -317,7 +325,7 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
                                        None if weights is None else weights.detach(), temperature, tail)
     ids, teacher = teacher_ids.contiguous(), teacher_log_probs.detach().float().contiguous()
     weights = None if weights is None else weights.detach().float().contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
+    if _differentiates(logits):
         total, rows = _Distillation.apply(logits, ids, teacher, weights, temperature, tail)
     else:
         total, rows, _, _ = ext().distill_fwd(logits, ids, teacher, weights, temperature, tail, False)
