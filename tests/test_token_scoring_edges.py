@@ -356,3 +356,126 @@ def test_forward_mode_tangents_are_refused(grad):
             with pytest.raises((RuntimeError, NotImplementedError), match="forward mode|jvp"):
                 call(forward_ad.make_dual(primal, torch.ones_like(primal)))
         ops.token_statistics(x, targets)
+
+
+@pytest.mark.gpu
+def test_gradients_in_a_cuda_graph():
+    """Forward and backward of the three operators captured once and replayed on other inputs."""
+    g = _generator(76)
+    logits, ids, teacher = _pair(6, 20011, 8, 77, torch.bfloat16)
+    logits, ids, teacher = logits.cuda(), ids.cuda(), teacher.cuda()
+    targets = torch.randint(0, 515, (6,), generator=g).cuda()
+    hidden, weight = torch.randn(6, 64, generator=g).bfloat16().cuda(), torch.randn(515, 64, generator=g).bfloat16().cuda()
+    for x in (logits, hidden, weight):
+        x.requires_grad_()
+    factor = torch.tensor(0.3, device="cuda")
+
+    def run():
+        s = ops.token_statistics(logits, targets, top=7)
+        d = ops.distillation_loss(logits, ids, teacher, tail=True)
+        h = ops.linear_token_statistics(hidden, weight, targets)
+        grads = torch.autograd.grad(s.log_probs.sum() + s.top_log_probs.sum() + d.total * factor, logits)
+        grads += torch.autograd.grad(h.log_probs.sum() + h.entropy.sum(), (hidden, weight))
+        return [x.detach() for x in (*s, *d, h.log_probs, h.entropy, *grads)]
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    with torch.no_grad():
+        logits.copy_(torch.randn(6, 20011, generator=g) * 3)
+        hidden.copy_(torch.randn(6, 64, generator=g))
+        factor.fill_(1.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(out, run()):
+        assert torch.equal(a, b)
+
+
+# -- the LM head ------------------------------------------------------------------------------------
+def _head(rows, hidden, vocab, seed):
+    g = _generator(seed)
+    h = torch.randn(rows, hidden, generator=g).bfloat16()
+    w = (torch.randn(vocab, hidden, generator=g) * 3 / hidden ** 0.5).bfloat16()
+    t = torch.randint(0, vocab, (rows,), generator=g)
+    if rows > 2:
+        t[1] = -100
+    return h.cuda(), w.cuda(), t.cuda()
+
+
+def _close_scores(got, logits, targets, temperature):
+    # a logit is a sum of up to 2048 products in fp32: 1e-5 at most (of values up to 15)
+    lp, entropy = _scores(logits, targets, temperature)
+    assert bool(((got.log_probs.detach().cpu() - lp).abs() <= 3e-5 + 1e-5 * lp.abs()).all())
+    assert bool(((got.entropy.detach().cpu() - entropy).abs() <= 3e-4).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 16, 31, 32, 33, 128, 129])
+@pytest.mark.parametrize("hidden", [72, 2048])
+@pytest.mark.parametrize("vocab", [1003, 40007, 151669])
+def test_head_of_few_rows(rows, hidden, vocab):
+    """Several tiles to a block, a ring that wraps, narrow and partial tiles, a partial block of the hidden dimension."""
+    h, w, t = _head(rows, hidden, vocab, rows + vocab)
+    t[0] = vocab - 1
+    got = ops.linear_token_statistics(h, w, t, temperature=0.8)
+    _close_scores(got, h.double() @ w.double().t(), t, 0.8)
+    again = ops.linear_token_statistics(h, w, t, temperature=0.8)
+    assert torch.equal(got.log_probs, again.log_probs) and torch.equal(got.entropy, again.entropy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kept", [True, False])
+@pytest.mark.parametrize("rows,hidden,vocab", [(5, 72, 257), (130, 256, 515), (300, 128, 4099), (129, 2048, 1000),
+                                               (40, 512, 20011)])
+def test_head_gradients_value_by_value(monkeypatch, kept, rows, hidden, vocab):
+    """The logits' gradient is rounded to bf16 once (2^-8 of each value, beside 3e-5 of its row's largest from the
+    statistics and the fp32 logits) before the products, whose results are rounded once more: each value of a
+    gradient is within what its own terms allow."""
+    if not kept:
+        monkeypatch.setattr(ops.statistics, "KEPT_BYTES", 0)
+    h, w, t = _head(rows, hidden, vocab, 78)
+    g = _generator(79)
+    up, down = torch.randn(rows, generator=g), torch.randn(rows, generator=g)
+    h.requires_grad_(), w.requires_grad_()
+    got = ops.linear_token_statistics(h, w, t, temperature=0.7)
+    logits = h.detach().double() @ w.detach().double().t()
+    _close_scores(got, logits, t, 0.7)
+    torch.autograd.backward((got.log_probs, got.entropy), (up.cuda(), down.cuda()))
+    lp = torch.log_softmax(logits / 0.7, -1)
+    p = lp.exp()
+    entropy = -(p * lp).sum(-1, keepdim=True)
+    one = torch.zeros_like(p).scatter_(1, t.clamp(min=0)[:, None], 1.0)
+    d = (up.cuda().double()[:, None] * (one - p) - down.cuda().double()[:, None] * p * (lp + entropy)) / 0.7
+    d = d * (t != -100)[:, None]
+    off = 2.0 ** -8 * d.abs() + 3e-5 * d.abs().amax(-1, keepdim=True)
+    hd, wd = h.detach().double(), w.detach().double()
+    for grad, want, bound in ((h.grad, d @ wd, off @ wd.abs()), (w.grad, d.t() @ hd, off.t() @ hd.abs())):
+        bound = bound + 2.0 ** -8 * want.abs() + 1e-30
+        assert bool(((grad.double() - want).abs() <= bound).all()), ((grad.double() - want).abs() / bound).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [4, 40, 300])
+@pytest.mark.parametrize("grad", [False, True])
+def test_head_bad_targets_and_nan_rows(rows, grad):
+    h, w, t = _head(rows, 64, 1003, 80)
+    h[2], h[3, 5] = float("nan"), INF
+    t[0] = 7
+    h.requires_grad_(grad)
+    got = ops.linear_token_statistics(h, w, t)
+    assert bool(got.log_probs[2:4].isnan().all()) and bool(got.entropy[2:4].isnan().all())
+    fine = [0] + list(range(4, rows))
+    picked = type(got)(got.log_probs[fine], got.entropy[fine])
+    _close_scores(picked, h.detach()[fine].double() @ w.double().t(), t[fine], 1.0)
+    assert got.log_probs[1] == 0 and got.entropy[1] == 0
+    ops.check_status("head")
+    t[0] = 1003
+    bad = ops.linear_token_statistics(h, w, t)
+    assert bool(bad.log_probs[0].isnan()) and bool(bad.entropy[0].isfinite())
+    with pytest.raises(ops.DeviceStatusError, match="out of bounds"):
+        ops.check_status("head")
