@@ -264,7 +264,7 @@ __device__ __noinline__ int collect_again(const T* row, int first, int last, int
 // are read once more, value by value.
 //
 // Bound by memory without alternatives: 3001 rows of 151936 bf16 take 144 us, 6.3 TB/s. With 64 alternatives 4096 rows
-// take 342 us (3.7 TB/s): the selections of a row are serial phases that the four blocks of an SM cover in part.
+// take 340 us (3.7 TB/s): the selections of a row are serial phases that the four blocks of an SM cover in part.
 // Four blocks of 256 threads hold 64 KB of loads in flight an SM, which the registers allow and the latency needs.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kStatThreads, 4)

@@ -3,7 +3,7 @@
 * :func:`token_statistics` - one pass over each row of logits gives the log-probability of a given
   token, the entropy of the distribution and its most likely alternatives, all differentiable.
 * :func:`linear_token_statistics` - log-probability and entropy straight from hidden states and the LM
-  head's weight: the logits exist only in the tensor cores' accumulators.
+  head's weight: without a backward the logits exist only in the tensor cores' accumulators.
 * :func:`distillation_loss` - KL divergence from a teacher's recorded top alternatives (what
   ``token_statistics(..., top=k)`` returns) to a student's logits, the gradient written with the loss.
 
@@ -236,15 +236,17 @@ class _LinearTokenStatistics(torch.autograd.Function):
 
 def linear_token_statistics(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *,
                             temperature: float = 1.0) -> TokenStatistics:
-    """:func:`token_statistics` of ``hidden @ weight.T`` without writing the logits: log-probability of
-    ``targets`` and entropy of each row of ``hidden`` [..., H] under the LM head ``weight`` [V, H].
+    """:func:`token_statistics` of ``hidden @ weight.T``: log-probability of ``targets`` and entropy of each
+    row of ``hidden`` [..., H] under the LM head ``weight`` [V, H].
 
     The reduction runs in the epilogue of the tensor-core product on its fp32 accumulators, so no
     logit is rounded to bf16. Without a backward no logit is written, and rows with target -100, whose
-    results are 0, take no part in the product. For a backward the fp32 logits are kept while they take at
-    most ``KEPT_BYTES`` (4 GiB), else their product is repeated; the logits' bf16 gradient, in row blocks of
-    at most 4 GiB, is multiplied into ``hidden`` and ``weight``. bf16 operands with H a multiple of 8; on a GPU other types go through the product
-    and :func:`token_statistics`, where the logits exist in ``hidden``'s type."""
+    results are 0, take no part in the product. Where a backward may follow, each call keeps its fp32 logits
+    until then while they take at most ``KEPT_BYTES`` (4 GiB; twice what bf16 logits take), else the product
+    is repeated; the logits' gradient, rounded to bf16 and in row blocks of at most ``GRADIENT_BYTES``
+    (4 GiB), is multiplied into ``hidden`` and ``weight``. bf16 operands with H a multiple of 8 (a view that
+    starts off a 16-byte boundary is copied); on a GPU other types go through the product and
+    :func:`token_statistics`, where the logits exist in ``hidden``'s type."""
     temperature = _check_temperature(temperature)
     if hidden.ndim < 1 or weight.ndim != 2 or hidden.shape[-1] != weight.shape[1] or weight.shape[0] < 1:
         raise ValueError("hidden must be [..., H] and weight [V, H]")
@@ -301,7 +303,7 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     zeros, even where its divergence is infinite or its logits are NaN (``rows`` reports it all the same).
     The gradient is written in the same pass over the logits as the loss, for an upstream gradient of one;
     for any other (a factor applied to ``total``, a loss scale) ``backward`` writes it once more from the
-    logits, which costs another pass, and rounds it once. Because it is handed over on ``backward``, the
+    logits, which costs another pass; either way it is rounded once. Because it is handed over on ``backward``, the
     operator is called again for a second one. Teacher, ids and weights take no gradient. On a GPU an id beyond the
     vocabulary gives NaN and sets the device status."""
     _check_logits(logits)
