@@ -110,7 +110,9 @@ def _distillation(logits, ids, teacher, weights, temperature, tail):
         q = q / torch.where(read, q.sum(-1), 1.0)[:, None]
     rows = torch.where(q > 0, q * (q.log() - lp), 0.0).sum(-1)
     rows = (rows + torch.where(rest > 0, rest * (rest.log() - left), 0.0)).masked_fill(~read, 0.0)
-    outside = torch.where((rest > 0)[:, None] & ~inside, (lp - left[:, None]).exp() * rest[:, None], 0.0)
+    # (the rest's own distribution, not exp(lp - left): at -5e38 a difference of logarithms is below 64 bits)
+    share = torch.softmax((x / temperature).masked_fill(inside, -INF), -1)
+    outside = torch.where((rest > 0)[:, None] & ~inside, share * rest[:, None], 0.0)
     grad = (q.sum(-1) + rest)[:, None] * p - q - outside
     return rows, grad.masked_fill(~read[:, None], 0.0) * (weights.double().cpu() / temperature)[:, None]
 
@@ -479,3 +481,20 @@ def test_head_bad_targets_and_nan_rows(rows, grad):
     assert bool(bad.log_probs[0].isnan()) and bool(bad.entropy[0].isfinite())
     with pytest.raises(ops.DeviceStatusError, match="out of bounds"):
         ops.check_status("head")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+def test_gradient_of_a_rest_masked_by_the_lowest_value(device, dtype, temperature):
+    """Every token outside the alternatives has the same share of the teacher's rest, however unlikely all of them are."""
+    x = torch.randn(2, 600, generator=_generator(82)) * 3
+    x[0, 2:] = torch.finfo(dtype).min
+    x[1, 5:] = -1.0e30
+    x = x.to(dtype)
+    ids, share = torch.tensor([[0, 1], [0, 3]]), torch.tensor([[0.45, 0.45], [0.3, 0.2]])
+    _, want_grad = _distillation(x, ids, share.log(), torch.ones(2), temperature, True)
+    leaf = x.to(device).requires_grad_()
+    total = ops.distillation_loss(leaf, ids.to(device), share.log().to(device), temperature=temperature, tail=True).total
+    grad, = torch.autograd.grad(total, leaf)
+    _close_gradient(grad, want_grad)

@@ -126,8 +126,12 @@ def _distillation_reference(logits, ids, teacher, weights, temperature, tail) ->
         inside = torch.zeros_like(x).scatter_add_(-1, at, there.to(x.dtype)) > 0
         left = ~(inside | (lp == float("-inf"))).all(-1)
         rest = (1 - q.sum(-1)).clamp(min=0)
-        outside = torch.where(left.unsqueeze(-1), lp, torch.zeros_like(lp)).masked_fill(
-            inside & left.unsqueeze(-1), float("-inf")).logsumexp(-1)
+        apart = torch.where(left.unsqueeze(-1), lp, torch.zeros_like(lp)).masked_fill(
+            inside & left.unsqueeze(-1), float("-inf"))
+        # (logsumexp's gradient exp(lp - result) is 1 for each of many tokens masked by a lowest value: at -1e38 their
+        # number is below 64 bits)
+        largest = apart.amax(-1, keepdim=True).detach()
+        outside = largest.squeeze(-1) + (apart - largest).exp().sum(-1).log()
         keep = left & (rest > 0)
         rows = rows + torch.where(keep, rest * (torch.where(keep, rest, torch.ones_like(rest)).log() - outside),
                                   torch.zeros_like(rest))
