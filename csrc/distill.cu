@@ -371,8 +371,11 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
     const float q_sum = plan.q_sum, q_rest = rest.s == 0.f ? 0.f : plan.q_rest;
     const float to_p = chosen.s == 0.f ? 0.f : exp2_fast((chosen.m - all.m) * c2) / all.s, p_chosen = chosen.s * to_p;
     const float p_rest = rest.s == 0.f ? 0.f : exp2_fast((rest.m - all.m) * c2) * rest.s / all.s;
+    // (in 64 bits where it comes from the parts: (x - m) / T of a token masked by the lowest value leaves fp32's range at
+    // T < 1, while the teacher's mass times it may not)
     auto log_mass = [&](float p, const RowStats& of) {
-      return p > 1e-30f ? logf(p) : (of.m - all.m) * inv_t + kLn2 * (log2f(of.s) - log2f(all.s));
+      return p > 1e-30f ? static_cast<double>(logf(p))
+                        : static_cast<double>(of.m - all.m) * inv_t + kLn2 * (log2f(of.s) - log2f(all.s));
     };
     float loss = 0.f;
     if (q_sum > 0.f) {  // (a masked token with mass: q_gap is +inf)
@@ -380,7 +383,7 @@ __global__ void __launch_bounds__(kDistillThreads, 5)
       loss = chosen.s == 0.f ? INFINITY
                              : static_cast<float>(plan.q_gap + merged + q_sum * (log_chosen - log_mass(p_chosen, chosen)));
     }
-    if (q_rest > 0.f) loss += q_rest * (logf(q_rest) - log_mass(p_rest, rest));
+    if (q_rest > 0.f) loss += static_cast<float>(q_rest * (logf(q_rest) - log_mass(p_rest, rest)));
     const bool empty = all.s == 0.f;  // every logit is masked: no distribution, no gradient
     if (empty) loss = INFINITY;
     if (plan.bad) loss = NAN;

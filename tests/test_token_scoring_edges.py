@@ -498,3 +498,23 @@ def test_gradient_of_a_rest_masked_by_the_lowest_value(device, dtype, temperatur
     total = ops.distillation_loss(leaf, ids.to(device), share.log().to(device), temperature=temperature, tail=True).total
     grad, = torch.autograd.grad(total, leaf)
     _close_gradient(grad, want_grad)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [0.6, 2.0])
+def test_divergences_of_tokens_masked_by_the_lowest_value_below_fp32s_edge(device, dtype, temperature):
+    """q (lowest - m) / T fits fp32 although (lowest - m) / T does not: 1e37 and 2e38, not infinities."""
+    x = torch.randn(4, 600, generator=_generator(81)) * 3
+    x[0, :2] = x[1, :2] = torch.finfo(dtype).min
+    x[2, 2:] = torch.finfo(dtype).min            # the rest of the vocabulary is masked
+    x = x.to(dtype)
+    ids = torch.tensor([[0, 1]] * 4)
+    share = torch.tensor([[0.01, 0.01], [0.2, 0.15], [0.45, 0.45], [0.3, 0.2]])
+    want, want_grad = _distillation(x, ids, share.log(), torch.ones(4), temperature, True)
+    assert bool((want < 3e38).all()) and bool((want[:3] > 1e36).all())
+    leaf = x.to(device).requires_grad_()
+    loss = ops.distillation_loss(leaf, ids.to(device), share.log().to(device), temperature=temperature, tail=True)
+    _close_loss(loss.rows, want)
+    grad, = torch.autograd.grad(loss.total, leaf)
+    _close_gradient(grad, want_grad)
