@@ -26,7 +26,7 @@ _EPS = 1e-6
 # What the largest listed cases cost: drawn ones stay below.
 _MOST_TOKENS = 8192
 _MOST_CACHE = 8 * 40960 * 4  # cached tokens x key heads
-_MOST_SCORES = 2 * 2048 * 8192 * 32  # (query, key) pairs x heads
+_MOST_SCORES = 3 * 2048 * 8192 * 32  # (query, key) pairs x heads
 _MOST_LOGITS = 512 * 151936
 
 
@@ -266,31 +266,31 @@ def _plain_append(state):
 def _plain_attend(state):
     case, q = state["case"], state["q"]
     heads, kv_heads, page = case["heads"], case["kv_heads"], case["page"]
-    group = heads // kv_heads
-    out = torch.empty_like(q)
-    first = 0
-    for b, (n, length) in enumerate(zip(state["new"], state["length"])):
-        pages = state["tables"][b, :-(-length // page)].long()
-        # [kv_heads, length, dim]
-        k = state["keys"][pages].transpose(0, 1).reshape(kv_heads, -1, _DIM)[:, :length].float()
-        v = state["values"][pages].transpose(0, 1).reshape(kv_heads, -1, _DIM)[:, :length].float()
-        column = torch.arange(length, device=q.device)
-        if case["tree"]:
-            j = column - (length - n)
-            words = state["tree"][first:first + n].long()
-            drafted = (words[:, (j // 32).clamp(min=0)] >> (j % 32)) & 1
-            seen = (j < 0) | (drafted == 1)
-        else:
-            seen = column <= torch.arange(length - n, length, device=q.device)[:, None]
-        mine = q[first:first + n].float().view(n, kv_heads, group, _DIM)
-        for h in range(kv_heads):
-            s = torch.matmul(mine[:, h].reshape(n * group, _DIM), k[h].t()).view(n, group, length)
-            s = torch.where(seen[:, None], s / math.sqrt(_DIM), float("-inf"))
-            e = (s - s.amax(dim=-1, keepdim=True)).exp()
-            o = torch.matmul(e.view(n * group, length), v[h]).view(n, group, _DIM) / e.sum(dim=-1, keepdim=True)
-            out[first:first + n, h * group:(h + 1) * group] = o.to(out.dtype)
-        first += n
-    return out
+    seqs, most, longest = case["seqs"], max(state["new"]), max(state["length"])
+    starts, lengths = state["starts"].long(), state["lengths"].long()
+    new = starts[1:] - starts[:-1]
+    # the sequences side by side, each as long as the longest
+    pages = state["tables"][:, :-(-longest // page)].clamp(min=0).long()
+    k, v = (state[name][pages].transpose(1, 2).reshape(seqs, kv_heads, -1, _DIM)[:, :, :longest].float()
+            for name in ("keys", "values"))
+    rows = (starts[:-1, None] + torch.arange(most, device=q.device)).clamp(max=len(q) - 1)
+    x = q[rows].float().view(seqs, most, kv_heads, heads // kv_heads, _DIM).transpose(1, 2)
+    # which of the new tokens a column is: those before them are negative
+    j = torch.arange(longest, device=q.device) - (lengths - new)[:, None]
+    if case["tree"]:
+        word = (j // 32).clamp(0, state["tree"].shape[1] - 1)[:, None].expand(-1, most, -1)
+        bit = state["tree"][rows].gather(2, word) >> (j % 32).int()[:, None] & 1
+        seen = (j[:, None] < 0) | (bit == 1) & (j < new[:, None])[:, None]
+    else:
+        seen = j[:, None] <= torch.arange(most, device=q.device)[:, None]
+    s = torch.matmul(x.reshape(seqs, kv_heads, -1, _DIM), k.transpose(2, 3)) / math.sqrt(_DIM)
+    s = torch.where(seen[:, None, :, None], s.view(seqs, kv_heads, most, -1, longest), float("-inf"))
+    e = (s - s.amax(dim=-1, keepdim=True)).exp()
+    o = torch.matmul(e.view(seqs, kv_heads, -1, longest), v) / e.sum(dim=-1).view(seqs, kv_heads, -1, 1)
+    row = torch.arange(len(q), device=q.device)
+    seq = torch.searchsorted(starts[1:], row, right=True)
+    o = o.view(seqs, kv_heads, most, -1, _DIM).transpose(1, 2)[seq, row - starts[seq]]
+    return o.reshape(q.shape).to(q.dtype)
 
 
 def _plain_logits(state):
