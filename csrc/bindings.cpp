@@ -89,6 +89,20 @@ at::Tensor token_stats_bwd(const at::Tensor& logits, const c10::optional<at::Ten
                            const c10::optional<at::Tensor>& top_ids, const at::Tensor& saved, double temperature,
                            const c10::optional<at::Tensor>& g_log_probs, const c10::optional<at::Tensor>& g_entropy,
                            const c10::optional<at::Tensor>& g_top);
+// paged_cache.cu
+at::Tensor paged_append(const at::Tensor& qkv, const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& positions,
+                        const at::Tensor& freqs, int64_t hq, double eps, at::Tensor& keys, at::Tensor& values,
+                        const at::Tensor& tables, const at::Tensor& starts, const at::Tensor& lengths);
+// paged_attention.cu
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& values, const at::Tensor& tables,
+                           const at::Tensor& starts, const at::Tensor& lengths, double scale,
+                           const c10::optional<at::Tensor>& tree);
+// logit_process.cu
+at::Tensor process_logits(const at::Tensor& logits, const c10::optional<at::Tensor>& history,
+                          const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& prompt_lengths,
+                          const c10::optional<at::Tensor>& repetition, const c10::optional<at::Tensor>& presence,
+                          const c10::optional<at::Tensor>& frequency, const c10::optional<at::Tensor>& bias_ids,
+                          const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& allowed);
 // lm_head.cu
 std::vector<at::Tensor> lm_head_stats_fwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
                                           double temperature, int64_t ignore_index, bool save, bool keep);
@@ -227,6 +241,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("token_logprob_bwd", &tdsv::token_logprob_bwd);
   m.def("token_stats_fwd", &tdsv::token_stats_fwd, "log-probability, entropy and top alternatives of rows of logits");
   m.def("token_stats_bwd", &tdsv::token_stats_bwd);
+  m.def("paged_append", &tdsv::paged_append, "norms and rotation of queries and keys, keys and values into a paged cache");
+  m.def("paged_attention", &tdsv::paged_attention, "attention of new tokens over a paged cache, causal or under a tree");
+  m.def("process_logits", &tdsv::process_logits, "penalties, biases and a grammar's mask on rows of logits");
   m.def("lm_head_stats_fwd", &tdsv::lm_head_stats_fwd, "token statistics fused with the LM head's product");
   m.def("lm_head_stats_bwd", &tdsv::lm_head_stats_bwd);
   m.def("distill_fwd", &tdsv::distill_fwd, "KL from a teacher's top alternatives, with its gradient");

@@ -1,0 +1,293 @@
+// What a sampler does to the logits before it draws a token: penalties for tokens that were said, biases, and the
+// mask of a grammar. For token v of a row, with c the number of times that the row's history holds v as output
+// and `said` whether it holds v at all:
+//
+//     x <- x / r if x > 0 else x r     where said                      (repetition r)
+//     x <- x - f c - p                 where c > 0                     (frequency f, presence p)
+//     x <- x + sum of v's biases
+//     x <- -inf                        where the grammar's bit is clear
+//
+// in fp32, rounded once to the logits' type.
+//
+// A row is cut into slices of the vocabulary, a block each. A block counts the history's tokens of its slice in
+// shared memory (whole numbers: the order of the atomics changes nothing), copies the slice under the mask in 16-byte
+// vectors, and then rewrites the few tokens that a count or a bias touches: what is copied never passes through fp32,
+// and the counts cost no work per token of the vocabulary beyond a scan of shared memory.
+#include "logit_rows.cuh"
+
+namespace tdsv {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kAhead = 4;  // vectors a thread has in flight
+
+// A token's word: how often it is output, and flags.
+constexpr uint32_t kPrompt = 1u << 31, kBiased = 1u << 30, kRepeated = 1u << 29, kCount = kRepeated - 1;
+
+template <typename T>
+__device__ __forceinline__ uint32_t minus_inf_pair() {  // two of a 16-bit type, or one of fp32
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) return 0xff80ff80u;
+  else if constexpr (std::is_same_v<T, __half>) return 0xfc00fc00u;
+  else return 0xff800000u;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t mask_word(uint32_t w, uint32_t bits) {
+  if constexpr (sizeof(T) == 4) {
+    return bits & 1u ? w : minus_inf_pair<T>();
+  } else {
+    const uint32_t keep = (bits & 1u ? 0x0000ffffu : 0u) | (bits & 2u ? 0xffff0000u : 0u);
+    return (w & keep) | (minus_inf_pair<T>() & ~keep);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 mask_vec(uint4 v, uint32_t bits) {
+  constexpr int kStep = 4 / sizeof(T);
+  v.x = mask_word<T>(v.x, bits);
+  v.y = mask_word<T>(v.y, bits >> kStep);
+  v.z = mask_word<T>(v.z, bits >> 2 * kStep);
+  v.w = mask_word<T>(v.w, bits >> 3 * kStep);
+  return v;
+}
+
+// The mask's bits from token `at` of the slice on, `count` (at most 8) of them; all set without a mask.
+__device__ __forceinline__ uint32_t mask_bits(const uint32_t* words, int at, int count) {
+  if (words == nullptr) return 0xffffffffu;
+  const int shift = at & 31;
+  uint32_t bits = words[at >> 5] >> shift;
+  if (shift + count > 32) bits |= words[(at >> 5) + 1] << (32 - shift);
+  return bits;
+}
+
+// out[0, n) = row[0, n) where the mask allows it. Vectors are aligned at `out`; where the logits lie at another
+// offset in their 16 bytes, two of theirs are joined. A vector whose bits are all clear is not read.
+template <typename T>
+__device__ __forceinline__ void copy_masked(const T* row, T* out, int n, const uint32_t* words) {
+  constexpr int kSize = LogitVec<T>::kSize;
+  constexpr uint32_t kAll = (1u << kSize) - 1;
+  const RowCut cut = cut_row(out, n);
+  const int tid = threadIdx.x;
+  const auto one = [&](int i) { out[i] = mask_bits(words, i, 1) & 1u ? row[i] : from_float<T>(-INFINITY); };
+  if (tid < cut.head) one(tid);
+  if (tid >= 32 && tid < 32 + cut.tail) one(n - cut.tail + tid - 32);
+  const T* from = row + cut.head;
+  uint4* to = reinterpret_cast<uint4*>(out + cut.head);
+  const int off = static_cast<int>((reinterpret_cast<uintptr_t>(from) & 15) / sizeof(T));
+  // the vectors whose parts all lie inside the row: with an offset, at most the first and the last do not
+  const uint4* x = reinterpret_cast<const uint4*>(from - off);
+  const int first = off > cut.head ? 1 : 0;
+  const int last = off == 0 ? cut.vecs : min(cut.vecs, (n - cut.head + off) / kSize - 1);
+  for (int i = first + tid; i < last; i += kThreads * kAhead) {
+    uint4 lo[kAhead], hi[kAhead];
+    uint32_t bits[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int at = i + u * kThreads;
+      bits[u] = at < last ? mask_bits(words, cut.head + at * kSize, kSize) & kAll : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (bits[u] == 0) continue;
+      lo[u] = load_stream(x + i + u * kThreads);
+      if (off != 0) hi[u] = load_stream(x + i + u * kThreads + 1);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (i + u * kThreads >= last) continue;
+      uint4 v = lo[u];
+      if (off != 0) v = shift_vec(lo[u], hi[u], off * static_cast<int>(sizeof(T)));
+      to[i + u * kThreads] = mask_vec<T>(v, bits[u]);
+    }
+  }
+  if (off != 0 && tid < 2 * kSize && cut.vecs > 0) {  // (two vectors at most, one value a thread)
+    const int i = tid < kSize ? 0 : cut.vecs - 1;
+    const bool todo = tid < kSize ? first == 1 : last < cut.vecs && (cut.vecs > 1 || first == 0);
+    if (todo) one(cut.head + i * kSize + tid % kSize);
+  }
+}
+
+struct Penalties {
+  const void* history;         // ids so far [rows, history], int64 or int32; null: none
+  const int* lengths;          // of each row's history; null: all of it
+  const int* prompt_lengths;   // of its part that is not output; null: 0
+  const float *repetition, *presence, *frequency;  // one per row; null: none
+  const int64_t* bias_ids;     // [rows, biases]; null: none
+  const float* bias;
+  const uint32_t* allowed;     // [rows, words]; null: all
+  int64_t history_stride, bias_stride, allowed_stride;
+  int history_size, biases;
+  bool wide;  // ids of 64 bits
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) process_kernel(const T* __restrict__ logits, RowLayout layout, int vocab,
+                                                           int slice, int parts, Penalties p, T* __restrict__ out,
+                                                           int* __restrict__ status) {
+  extern __shared__ uint4 smem[];
+  uint32_t* counts = reinterpret_cast<uint32_t*>(smem);                    // [slice], where any token is touched
+  float* biases = reinterpret_cast<float*>(counts + slice);                // [slice], where there are biases
+  const uint32_t r = blockIdx.x / parts;
+  const int begin = static_cast<int>(blockIdx.x - r * parts) * slice, n = min(slice, vocab - begin);
+  const int tid = threadIdx.x;
+  const T* row = logits + layout.offset(r) + begin;
+  T* to = out + static_cast<int64_t>(r) * vocab + begin;
+  const uint32_t* words = p.allowed == nullptr ? nullptr : p.allowed + r * p.allowed_stride + begin / 32;
+  const bool touched = p.history != nullptr || p.bias_ids != nullptr;
+  if (touched) {
+    for (int i = tid; i < slice / 4; i += kThreads) smem[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    if (p.history != nullptr) {
+      int length = p.history_size;
+      if (p.lengths != nullptr) {
+        const int given = p.lengths[r];
+        if (given > length || given < 0) report_status(status, kOutOfBounds);
+        length = max(0, min(given, length));
+      }
+      const int prompt = p.prompt_lengths == nullptr ? 0 : p.prompt_lengths[r];
+      const int64_t* wide = static_cast<const int64_t*>(p.history) + r * p.history_stride;
+      const int* narrow = static_cast<const int*>(p.history) + r * p.history_stride;
+      for (int i = tid; i < length; i += kThreads * kAhead) {
+        int64_t id[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int at = i + u * kThreads;
+          id[u] = at >= length ? -1 : p.wide ? wide[at] : narrow[at];
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          if (id[u] >= vocab) report_status(status, kOutOfBounds);
+          if (id[u] < begin || id[u] >= begin + n) continue;
+          if (i + u * kThreads < prompt) atomicOr(&counts[id[u] - begin], kPrompt);
+          else atomicAdd(&counts[id[u] - begin], 1u);
+        }
+      }
+    }
+    for (int i = tid; i < p.biases; i += kThreads) {
+      const int64_t id = p.bias_ids[r * p.bias_stride + i];
+      if (id >= vocab) report_status(status, kOutOfBounds);
+      if (id < begin || id >= begin + n) continue;
+      if (atomicOr(&counts[id - begin], kBiased) & kBiased) atomicOr(&counts[id - begin], kRepeated);
+      biases[id - begin] = p.bias[r * p.bias_stride + i];
+    }
+  }
+  copy_masked(row, to, n, words);
+  if (!touched) return;
+  __syncthreads();  // the counts, and the copies that the touched tokens replace
+  const float repetition = p.repetition == nullptr ? 1.f : p.repetition[r];
+  const float presence = p.presence == nullptr ? 0.f : p.presence[r];
+  const float frequency = p.frequency == nullptr ? 0.f : p.frequency[r];
+  for (int i = tid; i < slice / 4; i += kThreads) {
+    const uint4 four = smem[i];
+    if ((four.x | four.y | four.z | four.w) == 0) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t c = j == 0 ? four.x : j == 1 ? four.y : j == 2 ? four.z : four.w;
+      const int v = 4 * i + j;
+      if (c == 0 || !(mask_bits(words, v, 1) & 1u)) continue;
+      float x = to_float<T>(row[v]);
+      const uint32_t times = c & kCount;
+      if (times != 0 || (c & kPrompt)) x = x > 0.f ? x / repetition : x * repetition;
+      if (times != 0) x = x - frequency * static_cast<float>(times) - presence;
+      if (c & kRepeated) {  // in the list's order
+        float sum = 0.f;
+        for (int k = 0; k < p.biases; ++k)
+          if (p.bias_ids[r * p.bias_stride + k] == begin + v) sum += p.bias[r * p.bias_stride + k];
+        x += sum;
+      } else if (c & kBiased) {
+        x += biases[v];
+      }
+      to[v] = from_float<T>(x);
+    }
+  }
+}
+
+// Tokens of a slice (a multiple of 32): as many as the counts' shared memory holds, fewer while there are too few
+// blocks for the SMs.
+int slice_size(int64_t rows, int64_t vocab, bool touched) {
+  int64_t slice = touched ? 16384 : 32768;
+  while (slice > 4096 && rows * ((vocab + slice - 1) / slice) < 2 * num_sms()) slice /= 2;
+  return static_cast<int>(slice);
+}
+
+}  // namespace
+
+// Contiguous, in the logits' shape and type.
+at::Tensor process_logits(const at::Tensor& logits_in, const c10::optional<at::Tensor>& history,
+                          const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& prompt_lengths,
+                          const c10::optional<at::Tensor>& repetition, const c10::optional<at::Tensor>& presence,
+                          const c10::optional<at::Tensor>& frequency, const c10::optional<at::Tensor>& bias_ids,
+                          const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& allowed) {
+  constexpr const char* what = "process_logits";
+  check_logits(logits_in, what);
+  const int64_t vocab = logits_in.size(-1), rows = logits_in.numel() / vocab;
+  c10::cuda::CUDAGuard guard(logits_in.device());
+  RowLayout layout;
+  at::Tensor logits = logits_in;
+  if (!row_layout(logits, layout)) {
+    logits = logits.contiguous();
+    TDSV_CHECK(row_layout(logits, layout), what, ": logits layout");
+  }
+  auto out = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
+  if (rows == 0) return out;
+  auto given = [&](const c10::optional<at::Tensor>& t, at::ScalarType type, const char* name) {
+    if (!t.has_value() || !t->defined()) return false;
+    TDSV_CHECK(t->is_cuda() && t->has_storage() && t->device() == logits.device() && t->scalar_type() == type, what, ": ",
+               name, " has the wrong type or device");
+    return true;
+  };
+  auto per_row = [&](const c10::optional<at::Tensor>& t, at::ScalarType type, const char* name) -> const void* {
+    if (!given(t, type, name)) return nullptr;
+    check_cuda_tensor(*t, name);
+    TDSV_CHECK(t->numel() == rows, what, ": ", name, " must hold one value per row");
+    return t->data_ptr();
+  };
+  // [rows, size], rows any stride apart (0: the same for all)
+  auto table = [&](const at::Tensor& t, const char* name) {
+    TDSV_CHECK(t.dim() == 2 && t.size(0) == rows && (t.size(1) <= 1 || t.stride(1) == 1), what, ": ", name,
+               " must be [rows, size] with dense rows");
+    TDSV_CHECK(t.size(1) < (int64_t(1) << 29), what, ": ", name, " is too wide");
+    return rows == 1 ? int64_t(0) : t.stride(0);
+  };
+  Penalties p{};
+  if (history.has_value() && history->defined() && history->size(-1) > 0) {
+    p.wide = history->scalar_type() == at::kLong;
+    given(history, p.wide ? at::kLong : at::kInt, "history");
+    p.history_stride = table(*history, "history");
+    p.history_size = static_cast<int>(history->size(1));
+    p.history = history->data_ptr();
+    p.lengths = static_cast<const int*>(per_row(lengths, at::kInt, "lengths"));
+    p.prompt_lengths = static_cast<const int*>(per_row(prompt_lengths, at::kInt, "prompt_lengths"));
+  }
+  p.repetition = static_cast<const float*>(per_row(repetition, at::kFloat, "repetition"));
+  p.presence = static_cast<const float*>(per_row(presence, at::kFloat, "presence"));
+  p.frequency = static_cast<const float*>(per_row(frequency, at::kFloat, "frequency"));
+  if (given(bias_ids, at::kLong, "bias_ids") && bias_ids->size(-1) > 0) {
+    TDSV_CHECK(given(bias, at::kFloat, "bias") && bias->sizes() == bias_ids->sizes(), what, ": bias and bias_ids must be alike");
+    p.bias_stride = table(*bias_ids, "bias_ids");
+    TDSV_CHECK(table(*bias, "bias") == p.bias_stride, what, ": bias and bias_ids must lie alike");
+    p.biases = static_cast<int>(bias_ids->size(1));
+    p.bias_ids = bias_ids->data_ptr<int64_t>();
+    p.bias = bias->data_ptr<float>();
+  }
+  if (given(allowed, at::kInt, "allowed")) {
+    p.allowed_stride = table(*allowed, "allowed");
+    TDSV_CHECK(allowed->size(1) >= (vocab + 31) / 32, what, ": allowed must hold a bit per token");
+    p.allowed = reinterpret_cast<const uint32_t*>(allowed->data_ptr<int>());
+  }
+  const bool touched = p.history != nullptr || p.bias_ids != nullptr;
+  const int slice = slice_size(rows, vocab, touched);
+  const int64_t parts = (vocab + slice - 1) / slice;
+  TDSV_CHECK(rows * parts < (int64_t(1) << 31), what, ": too many rows");
+  const size_t smem = touched ? static_cast<size_t>(slice) * (p.bias_ids != nullptr ? 8 : 4) : 0;
+  with_logit_type(logits.scalar_type(), [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    TDSV_CUDA_CHECK(cudaFuncSetAttribute(process_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 16384 * 8));
+    process_kernel<T><<<static_cast<unsigned>(rows * parts), kThreads, smem, stream()>>>(
+        static_cast<const T*>(logits.data_ptr()), layout, static_cast<int>(vocab), slice, static_cast<int>(parts), p,
+        static_cast<T*>(out.data_ptr()), status_word_ptr());
+  });
+  TDSV_LAUNCH_CHECK();
+  return out;
+}
+
+}  // namespace tdsv

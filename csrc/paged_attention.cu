@@ -1,0 +1,516 @@
+// Attention of new tokens over a paged cache.
+//
+// Row (i, h) of a sequence is query head h of its new token i, at position length - n + i. With the keys and values of
+// h's key head,
+//
+//     out = sum_j p_j v_j / sum_j p_j,   p_j = 2^(c (q . k_j) - m),   c = scale log2(e)
+//
+// over the positions j that the row sees: up to its own, or, under the mask of a drafted tree, those before the new
+// tokens and the new tokens whose bit is set. m is the running maximum; sums are fp32, p is rounded to the cache's
+// type for its product with v (the sum of p is not, so that a row's weights err by their own roundings alone). A row
+// that sees nothing gives zeros, as do rows of the call that no sequence has.
+//
+// The rows of a sequence under one key head are its n tokens times the heads of the group, in tiles of 16. The keys of
+// a tile are cut into units of 128, and all units of all tiles stand in one line, of which each block takes an equal
+// stretch: a batch of very different lengths fills the SMs as evenly as one of equal ones, and one long sequence as well
+// as many short ones. A tile whose units lie in several blocks is joined by a second kernel from its parts. The line
+// follows from starts and lengths on the GPU; each block sums them for itself.
+//
+// Four warps take 32 of a unit's keys each, with their own running maximum and sum, and with their own ring of
+// tiles that TMA fills: no warp waits for another until the tile is joined. A key or value crosses HBM once for each
+// 16 rows.
+#include "paged.cuh"
+#include "tc_util.cuh"
+
+#include <type_traits>
+
+namespace tdsv {
+
+namespace {
+
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kTileRows = 16;
+constexpr int kWarpKeys = 32, kUnitKeys = kWarps * kWarpKeys;
+constexpr int kStages = 3;
+constexpr int kHalfBytes = kWarpKeys * 128;   // 64 dims of a warp's keys
+constexpr int kSideBytes = 2 * kHalfBytes;    // keys, or values
+constexpr int kStageBytes = 2 * kSideBytes;
+
+enum : int { kWaitTile = 341 };
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+struct AttendArgs {
+  PagedBatch batch;
+  const uint32_t* tree;  // [rows, tree_words]
+  int tree_words;        // -1: causal
+  int group, hq;
+  float scale_log2;      // c
+  float* parts;          // [2 blocks][kTileRows][kHeadDim] of tiles that lie in several blocks
+  float2* part_stats;    // [2 blocks][kTileRows]: m, sum
+  int2* blocks_of;       // [rows][hq]: first and last block of a row's tile
+  int* status;
+};
+
+// Units of a sequence: key heads x row tiles x units of keys.
+struct Line {
+  int tiles, units;  // row tiles, units of keys a tile
+  __device__ __forceinline__ Line(const PagedSequence& s, int group) {
+    tiles = (s.n * group + kTileRows - 1) / kTileRows;
+    units = s.n == 0 ? 0 : (s.length + kUnitKeys - 1) / kUnitKeys;
+  }
+  __device__ __forceinline__ int64_t all(int kv_heads) const { return static_cast<int64_t>(tiles) * units * kv_heads; }
+};
+
+// A place in the line.
+struct Cursor {
+  int b = -1, head = 0, tile = 0, unit = 0;
+  PagedSequence s;
+  int tiles = 0, units = 0;
+
+  __device__ __forceinline__ void enter(const AttendArgs& a, int seq) {
+    b = seq;
+    s = paged_sequence(a.batch, b, nullptr);
+    const Line l(s, a.group);
+    tiles = l.tiles, units = l.units;
+    head = tile = unit = 0;
+  }
+  __device__ __forceinline__ void place(int64_t offset) {
+    unit = static_cast<int>(offset % units);
+    offset /= units;
+    tile = static_cast<int>(offset % tiles);
+    head = static_cast<int>(offset / tiles);
+  }
+  // (the caller knows that there is a next unit)
+  __device__ __forceinline__ void next(const AttendArgs& a) {
+    if (++unit < units) return;
+    unit = 0;
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++head < a.batch.kv_heads) return;
+    do enter(a, b + 1);
+    while (units == 0 && b + 1 < a.batch.seqs);
+  }
+};
+
+struct Shared {
+  float out[kWarps][kTileRows][kHeadDim];
+  float2 stats[kWarps][kTileRows];
+  uint64_t full[kWarps][kStages];
+  int64_t sums[kWarps];
+  int64_t first_offset;
+  int first_seq;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    attend_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
+                  const T* __restrict__ q, T* __restrict__ out, const __grid_constant__ AttendArgs a) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  Shared& sm = *reinterpret_cast<Shared*>(ring + kWarps * kStages * kStageBytes);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const PagedBatch& batch = a.batch;
+
+  // this block's stretch of the line: thread t sums the sequences [t * per, ...)
+  const int per = (batch.seqs + kThreads - 1) / kThreads;
+  int64_t mine = 0;
+  for (int i = tid * per; i < min(batch.seqs, (tid + 1) * per); ++i)
+    mine += Line(paged_sequence(batch, i, a.status), a.group).all(batch.kv_heads);
+  int64_t before = mine;  // inclusive, then exclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += v;
+  }
+  if (lane == 31) sm.sums[warp] = before;
+  if (tid == 0) {
+    for (int i = 0; i < kWarps * kStages; ++i) mbar_init(&sm.full[i / kStages][i % kStages], 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sm.sums[w];
+    total += sm.sums[w];
+  }
+  before -= mine;
+  const int64_t share = (total + gridDim.x - 1) / gridDim.x;
+  const int64_t begin = share * blockIdx.x, end = min(total, begin + share);
+  if (begin >= end) return;
+  if (begin >= before && begin < before + mine) {
+    int64_t at = before;
+    for (int i = tid * per;; ++i) {
+      const int64_t units = Line(paged_sequence(batch, i, nullptr), a.group).all(batch.kv_heads);
+      if (begin < at + units) {
+        sm.first_seq = i;
+        sm.first_offset = begin - at;
+        break;
+      }
+      at += units;
+    }
+  }
+  __syncthreads();
+
+  Cursor compute;
+  compute.enter(a, sm.first_seq);
+  compute.place(sm.first_offset);
+  Cursor load = compute;
+  const int count = static_cast<int>(end - begin);  // units of this block
+  const int rows_per_box = min(1 << batch.page_shift, kWarpKeys);
+  const uint32_t my_ring = smem_u32(ring) + warp * kStages * kStageBytes;
+
+  // Loads unit number `i` of this block into its stage: the warp's 32 keys and values, as far as there are any.
+  auto issue = [&](int i) {
+    const int key0 = load.unit * kUnitKeys + warp * kWarpKeys;
+    if (key0 < load.s.length && lane == 0) {
+      uint64_t* bar = &sm.full[warp][i % kStages];
+      const uint32_t to = my_ring + (i % kStages) * kStageBytes;
+      const int boxes = min(kWarpKeys / rows_per_box, (load.s.length - key0 + rows_per_box - 1) / rows_per_box);
+      mbar_arrive_expect_tx(bar, boxes * rows_per_box * 512);
+      for (int x = 0; x < boxes; ++x) {
+        const int at = key0 + x * rows_per_box;
+        int page = batch.tables[load.b * batch.table_stride + (at >> batch.page_shift)];
+        if (page < 0 || page >= batch.pages) {
+          report_status(a.status, kOutOfBounds);
+          page = 0;
+        }
+        const int row = at & ((1 << batch.page_shift) - 1);
+        const uint32_t box = to + x * rows_per_box * 128;
+        tma_load_4d(box, &key_map, bar, 0, row, load.head, page);
+        tma_load_4d(box + kHalfBytes, &key_map, bar, 64, row, load.head, page);
+        tma_load_4d(box + kSideBytes, &value_map, bar, 0, row, load.head, page);
+        tma_load_4d(box + kSideBytes + kHalfBytes, &value_map, bar, 64, row, load.head, page);
+      }
+    }
+    if (i + 1 < count) load.next(a);
+  };
+  for (int i = 0; i < min(kStages, count); ++i) issue(i);
+
+  const int g = lane >> 2, c2 = (lane & 3) * 2;
+  uint32_t phases = 0;  // of this warp's stages
+  uint32_t qf[kHeadDim / 16][4];
+  float o[kHeadDim / 8][4], m[2], l[2];
+  bool ok = true;
+  int token[2];
+  for (int i = 0; i < count; ++i) {
+    const PagedSequence s = compute.s;
+    const int prefix = s.length - s.n;
+    if (i == 0 || compute.unit == 0) {  // a new tile
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = compute.tile * kTileRows + g + 8 * r;
+        token[r] = row < s.n * a.group ? row / a.group : -1;
+        m[r] = -INFINITY, l[r] = 0.f;
+        const int head = compute.head * a.group + row % a.group;
+        const T* from = q + (static_cast<int64_t>(s.start + token[r]) * a.hq + head) * kHeadDim + c2;
+#pragma unroll
+        for (int k = 0; k < kHeadDim / 16; ++k) {
+          qf[k][r] = token[r] < 0 ? 0u : *reinterpret_cast<const uint32_t*>(from + k * 16);
+          qf[k][2 + r] = token[r] < 0 ? 0u : *reinterpret_cast<const uint32_t*>(from + k * 16 + 8);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kHeadDim / 8; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[k][j] = 0.f;
+    }
+    const int key0 = compute.unit * kUnitKeys + warp * kWarpKeys;
+    const int stage = i % kStages;
+    if (key0 < s.length) {
+      ok = ok && warp_wait(&sm.full[warp][stage], (phases >> stage) & 1, a.status, kWaitTile);
+      phases ^= 1u << stage;
+      const uint32_t ks = my_ring + stage * kStageBytes, vs = ks + kSideBytes;
+      const int here = s.length - key0;  // keys of the tile that exist
+      if (here < kWarpKeys) {            // what lies behind them may be anything: a weight of 0 does not undo a NaN
+        uint8_t* v = ring + (warp * kStages + stage) * kStageBytes + kSideBytes;
+        for (int x = here * 8 + lane; x < kWarpKeys * 8; x += 32) {
+          *reinterpret_cast<uint4*>(v + x * 16) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(v + kHalfBytes + x * 16) = make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+      }
+      // scores: 16 rows x 32 keys
+      float sc[kWarpKeys / 8][4];
+#pragma unroll
+      for (int n = 0; n < kWarpKeys / 8; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[n][j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kHeadDim / 16; ++k)
+#pragma unroll
+        for (int n = 0; n < kWarpKeys / 16; ++n) {
+          uint32_t b[4];
+          const int row = n * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
+          ldmatrix4(b, ks + (k >> 2) * kHalfBytes + swz(row, (k & 3) * 2 + ((lane >> 3) & 1)));
+          mma16816<T>(sc[2 * n], qf[k], b[0], b[1]);
+          mma16816<T>(sc[2 * n + 1], qf[k], b[2], b[3]);
+        }
+      // what each row sees
+      if (key0 + kWarpKeys > prefix) {
+#pragma unroll
+        for (int n = 0; n < kWarpKeys / 8; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = j >> 1, key = key0 + n * 8 + c2 + (j & 1), x = key - prefix;
+            bool seen = token[r] >= 0 && key < s.length;
+            if (seen && x >= 0) {
+              if (a.tree_words < 0) seen = x <= token[r];
+              else
+                seen = x < a.tree_words * 32 &&
+                       (a.tree[static_cast<int64_t>(s.start + token[r]) * a.tree_words + (x >> 5)] >> (x & 31) & 1u);
+            }
+            if (!seen) sc[n][j] = -INFINITY;
+          }
+      }
+      float alpha[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < kWarpKeys / 8; ++n) mx = fmaxf(mx, fmaxf(sc[n][2 * r], sc[n][2 * r + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        mx = fmaxf(m[r], mx * a.scale_log2);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        alpha[r] = ex2_approx(m[r] - base);
+        m[r] = mx;
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < kWarpKeys / 8; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float p = ex2_approx(fmaf(sc[n][2 * r + j], a.scale_log2, -base));
+            sc[n][2 * r + j] = p;
+            sum += p;
+          }
+        l[r] = l[r] * alpha[r] + sum;  // this lane's columns; the others' are added at the end
+      }
+#pragma unroll
+      for (int n = 0; n < kHeadDim / 8; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][j] *= alpha[j >> 1];
+#pragma unroll
+      for (int k = 0; k < kWarpKeys / 16; ++k) {
+        const uint32_t p[4] = {pack2<T>(sc[2 * k][0], sc[2 * k][1]), pack2<T>(sc[2 * k][2], sc[2 * k][3]),
+                               pack2<T>(sc[2 * k + 1][0], sc[2 * k + 1][1]), pack2<T>(sc[2 * k + 1][2], sc[2 * k + 1][3])};
+#pragma unroll
+        for (int n = 0; n < kHeadDim / 16; ++n) {
+          uint32_t b[4];
+          const int row = k * 16 + (lane & 15), chunk = n * 2 + (lane >> 4);
+          ldmatrix4_t(b, vs + (chunk >> 3) * kHalfBytes + swz(row, chunk & 7));
+          mma16816<T>(o[2 * n], p, b[0], b[1]);
+          mma16816<T>(o[2 * n + 1], p, b[2], b[3]);
+        }
+      }
+      if (here < kWarpKeys) fence_proxy_async_smem();  // the zeros, before TMA writes there again
+      __syncwarp();
+    }
+    if (i + kStages < count) issue(i + kStages);
+
+    if (compute.unit == compute.units - 1 || i == count - 1) {  // the tile's last unit here: the four warps' parts join
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        if ((lane & 3) == 0) sm.stats[warp][g + 8 * r] = make_float2(m[r], l[r]);
+#pragma unroll
+        for (int n = 0; n < kHeadDim / 8; ++n)
+          *reinterpret_cast<float2*>(&sm.out[warp][g + 8 * r][n * 8 + c2]) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+      }
+      __syncthreads();
+      const int64_t unit0 = begin + i - compute.unit;  // the tile's place in the line
+      const int first = static_cast<int>(unit0 / share), last = static_cast<int>((unit0 + compute.units - 1) / share);
+      const bool whole = first == last;
+      const int slot = 2 * blockIdx.x + (static_cast<int>(blockIdx.x) == first ? 1 : 0);
+      for (int x = tid; x < kTileRows * kHeadDim / 4; x += kThreads) {
+        const int r = x / (kHeadDim / 4), d = x % (kHeadDim / 4) * 4;
+        const int row = compute.tile * kTileRows + r;
+        if (row >= s.n * a.group) break;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.stats[w][r].x);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        float sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 st = sm.stats[w][r];
+          const float f = ex2_approx(st.x - base);
+          const float4 part = *reinterpret_cast<const float4*>(&sm.out[w][r][d]);
+          sum += f * st.y;
+          v.x += f * part.x, v.y += f * part.y, v.z += f * part.z, v.w += f * part.w;
+        }
+        const int t = s.start + row / a.group;
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          T* to = out + (static_cast<int64_t>(t) * a.hq + compute.head * a.group + row % a.group) * kHeadDim + d;
+          *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+        } else {
+          *reinterpret_cast<float4*>(a.parts + (static_cast<int64_t>(slot) * kTileRows + r) * kHeadDim + d) = v;
+          if (d == 0) a.part_stats[slot * kTileRows + r] = make_float2(mx, sum);
+        }
+        // (a token's rows may lie in two tiles: each tile writes its own rows' blocks)
+        if (d == 0 && first == static_cast<int>(blockIdx.x))
+          a.blocks_of[static_cast<int64_t>(t) * a.hq + compute.head * a.group + row % a.group] = make_int2(first, last);
+      }
+      __syncthreads();
+    }
+    if (i + 1 < count) compute.next(a);
+  }
+}
+
+// One warp per row of the call and head: joins the parts of rows whose tile lies in several blocks, and writes zeros to
+// rows that no sequence has.
+template <typename T>
+__global__ void __launch_bounds__(256) attend_join_kernel(T* __restrict__ out, const __grid_constant__ AttendArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (item >= static_cast<int64_t>(a.batch.rows) * a.hq) return;
+  const int t = static_cast<int>(item / a.hq), h = static_cast<int>(item - static_cast<int64_t>(t) * a.hq);
+  const int b = paged_find(a.batch, t);
+  PagedSequence s;
+  if (b < a.batch.seqs) s = paged_sequence(a.batch, b, nullptr);
+  T* to = out + item * kHeadDim + 4 * lane;
+  if (t < s.start || t >= s.start + s.n) {
+    *reinterpret_cast<uint2*>(to) = make_uint2(0, 0);
+    return;
+  }
+  const int2 blocks = a.blocks_of[item];
+  if (blocks.x == blocks.y) return;
+  const int r = ((t - s.start) * a.group + h % a.group) % kTileRows;
+  auto slot = [&](int block) { return static_cast<int64_t>(2 * block + (block == blocks.x ? 1 : 0)) * kTileRows + r; };
+  float mx = -INFINITY;
+  for (int x = blocks.x + lane; x <= blocks.y; x += 32) mx = fmaxf(mx, a.part_stats[slot(x)].x);
+  mx = warp_max(mx);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int x = blocks.x; x <= blocks.y; ++x) {
+    const float2 st = a.part_stats[slot(x)];
+    const float4 part = *reinterpret_cast<const float4*>(a.parts + slot(x) * kHeadDim + 4 * lane);
+    const float f = ex2_approx(st.x - base);
+    sum += f * st.y;
+    v.x += f * part.x, v.y += f * part.y, v.z += f * part.z, v.w += f * part.w;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+}
+
+CUtensorMap pool_map(const at::Tensor& pool, int box_rows) {
+  const PoolStrides s = pool_strides(pool);
+  CUtensorMap map;
+  const cuuint64_t dims[4] = {kHeadDim, static_cast<cuuint64_t>(pool.size(2)), static_cast<cuuint64_t>(pool.size(1)),
+                              static_cast<cuuint64_t>(pool.size(0))};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(s.row) * 2, static_cast<cuuint64_t>(s.head) * 2,
+                                 static_cast<cuuint64_t>(s.page) * 2};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1}, steps[4] = {1, 1, 1, 1};
+  const CUresult r = encode_fn()(&map, pool.scalar_type() == at::kHalf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                 4, pool.data_ptr(), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TDSV_CHECK(r == CUDA_SUCCESS, "paged_attention: the cache's layout was refused (", static_cast<int>(r), ")");
+  return map;
+}
+
+}  // namespace
+
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& values, const at::Tensor& tables,
+                           const at::Tensor& starts, const at::Tensor& lengths, double scale,
+                           const c10::optional<at::Tensor>& tree) {
+  constexpr const char* what = "paged_attention";
+  check_cuda_tensor(q, "q");
+  c10::cuda::CUDAGuard guard(q.device());
+  TDSV_CHECK(q.dim() == 3 && q.size(2) == kHeadDim && q.size(1) >= 1, what, ": q must be [rows, heads, 128]");
+  TDSV_CHECK(keys.device() == q.device() && keys.scalar_type() == q.scalar_type(), what, ": q and the cache must be alike");
+  TDSV_CHECK(reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0, what, ": q must start on 16 bytes");
+  const int64_t rows = q.size(0), hq = q.size(1);
+  AttendArgs a{};
+  a.batch = paged_batch(keys, values, tables, starts, lengths, rows, what);
+  TDSV_CHECK(hq % a.batch.kv_heads == 0 && rows * hq < (int64_t(1) << 31), what, ": heads must be a multiple of the cache's");
+  a.group = static_cast<int>(hq / a.batch.kv_heads);
+  a.hq = static_cast<int>(hq);
+  a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  a.tree_words = -1;
+  if (tree.has_value() && tree->defined()) {
+    check_cuda_tensor(*tree, "tree");
+    TDSV_CHECK(tree->device() == q.device() && tree->scalar_type() == at::kInt && tree->dim() == 2 && tree->size(0) == rows &&
+                   tree->size(1) < (1 << 24),
+               what, ": tree must be int32 [rows, words]");
+    a.tree = reinterpret_cast<const uint32_t*>(tree->data_ptr<int>());
+    a.tree_words = static_cast<int>(tree->size(1));
+  }
+  auto out = at::empty_like(q);
+  if (rows == 0) return out;
+  a.status = status_word_ptr();
+  const int blocks = num_sms();
+  const auto f32 = q.options().dtype(at::kFloat);
+  auto parts = at::empty({2 * blocks, kTileRows, kHeadDim}, f32);
+  auto stats = at::empty({2 * blocks, kTileRows, 2}, f32);
+  auto blocks_of = at::empty({rows, hq, 2}, f32.dtype(at::kInt));
+  a.parts = parts.data_ptr<float>();
+  a.part_stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
+  a.blocks_of = reinterpret_cast<int2*>(blocks_of.data_ptr<int>());
+  bind_primary_context();
+  const int box_rows = std::min(1 << a.batch.page_shift, kWarpKeys);
+  const CUtensorMap key_map = pool_map(keys, box_rows), value_map = pool_map(values, box_rows);
+  auto launch = [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    constexpr int smem = kWarps * kStages * kStageBytes + sizeof(Shared) + 1024;
+    static_assert(smem <= 227 * 1024, "fits an SM");
+    TDSV_CUDA_CHECK(cudaFuncSetAttribute(attend_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attend_kernel<T><<<blocks, kThreads, smem, stream()>>>(key_map, value_map, static_cast<const T*>(q.data_ptr()),
+                                                           static_cast<T*>(out.data_ptr()), a);
+    TDSV_LAUNCH_CHECK();
+    attend_join_kernel<T><<<static_cast<unsigned>((rows * hq + 7) / 8), 256, 0, stream()>>>(
+        static_cast<T*>(out.data_ptr()), a);
+  };
+  if (q.scalar_type() == at::kHalf) launch(static_cast<__half*>(nullptr));
+  else launch(static_cast<__nv_bfloat16*>(nullptr));
+  TDSV_LAUNCH_CHECK();
+  return out;
+}
+
+}  // namespace tdsv

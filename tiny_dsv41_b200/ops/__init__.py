@@ -4,6 +4,7 @@ CPU tensors run the plain-PyTorch restatement used as the test oracle."""
 from ._ext import (DeviceStatusError, StatusMonitor, available, check_status, ext, on_gpu, peer_wait_limit,
                    set_peer_wait_limit)
 from .attention import causal_attention
+from .decoding import PagedBatch, paged_append, paged_attention, process_logits, tree_mask
 from .fp4 import dequantize_fp4, fp4_grouped_linear
 from .gemm import grouped_linear, linear, matmul_nt
 from .loss import linear_cross_entropy, token_log_probs
@@ -16,7 +17,7 @@ from .router import AuxGradient, route
 from .statistics import DistillationLoss, TokenStatistics, distillation_loss, linear_token_statistics, token_statistics
 
 __all__ = [
-    "AuxGradient", "DeviceStatusError", "DistillationLoss", "Routing", "StatusMonitor", "TokenStatistics", "available", "build_routing", "causal_attention", "check_status", "combine",
-    "dequantize_fp4", "distillation_loss", "ext", "fake_quant", "fp4_grouped_linear", "gather", "grouped_linear", "inv_freq", "linear", "linear_cross_entropy", "linear_token_statistics", "matmul_nt", "on_gpu", "peer_wait_limit",
-    "qk_norm_rope", "quantize_activation", "rms_norm", "rope_interleaved", "route", "set_peer_wait_limit", "swiglu", "token_log_probs", "token_statistics",
+    "AuxGradient", "DeviceStatusError", "DistillationLoss", "PagedBatch", "Routing", "StatusMonitor", "TokenStatistics", "available", "build_routing", "causal_attention", "check_status", "combine",
+    "dequantize_fp4", "distillation_loss", "ext", "fake_quant", "fp4_grouped_linear", "gather", "grouped_linear", "inv_freq", "linear", "linear_cross_entropy", "linear_token_statistics", "matmul_nt", "on_gpu", "paged_append", "paged_attention", "peer_wait_limit",
+    "process_logits", "qk_norm_rope", "quantize_activation", "rms_norm", "rope_interleaved", "route", "set_peer_wait_limit", "swiglu", "token_log_probs", "token_statistics", "tree_mask",
 ]
