@@ -19,10 +19,7 @@
 // Four warps take 32 of a unit's keys each, with their own running maximum and sum, and with their own ring of
 // tiles that TMA fills: no warp waits for another until the tile is joined. A key or value crosses HBM once for each
 // 16 rows.
-#include "paged.cuh"
-#include "tc_util.cuh"
-
-#include <type_traits>
+#include "paged_attend.cuh"
 
 namespace tdsv {
 
@@ -38,13 +35,6 @@ constexpr int kStageBytes = 2 * kSideBytes;
 
 enum : int { kWaitTile = 341 };
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -68,29 +58,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (std::is_same_v<T, __half>) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-
-struct AttendArgs {
-  PagedBatch batch;
-  const uint32_t* tree;  // [rows, tree_words]
-  int tree_words;        // -1: causal
-  int group, hq;
-  float scale_log2;      // c
-  float* parts;          // [2 blocks][kTileRows][kHeadDim] of tiles that lie in several blocks
-  float2* part_stats;    // [2 blocks][kTileRows]: m, sum
-  int2* blocks_of;       // [rows][hq]: first and last block of a row's tile
-  int* status;
-};
-
 // Units of a sequence: key heads x row tiles x units of keys.
 struct Line {
   int tiles, units;  // row tiles, units of keys a tile
@@ -136,9 +103,7 @@ struct Shared {
   float out[kWarps][kTileRows][kHeadDim];
   float2 stats[kWarps][kTileRows];
   uint64_t full[kWarps][kStages];
-  int64_t sums[kWarps];
-  int64_t first_offset;
-  int first_seq;
+  StretchScratch<kThreads> stretch;
 };
 
 template <typename T>
@@ -151,72 +116,34 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const PagedBatch& batch = a.batch;
 
-  // this block's stretch of the line: thread t sums the sequences [t * per, ...)
-  const int per = (batch.seqs + kThreads - 1) / kThreads;
-  int64_t mine = 0;
-  for (int i = tid * per; i < min(batch.seqs, (tid + 1) * per); ++i)
-    mine += Line(paged_sequence(batch, i, a.status), a.group).all(batch.kv_heads);
-  int64_t before = mine;  // inclusive, then exclusive
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += v;
-  }
-  if (lane == 31) sm.sums[warp] = before;
   if (tid == 0) {
     for (int i = 0; i < kWarps * kStages; ++i) mbar_init(&sm.full[i / kStages][i % kStages], 1);
     fence_barrier_init();
   }
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += sm.sums[w];
-    total += sm.sums[w];
-  }
-  before -= mine;
-  const int64_t share = (total + gridDim.x - 1) / gridDim.x;
-  const int64_t begin = share * blockIdx.x, end = min(total, begin + share);
-  if (begin >= end) return;
-  if (begin >= before && begin < before + mine) {
-    int64_t at = before;
-    for (int i = tid * per;; ++i) {
-      const int64_t units = Line(paged_sequence(batch, i, nullptr), a.group).all(batch.kv_heads);
-      if (begin < at + units) {
-        sm.first_seq = i;
-        sm.first_offset = begin - at;
-        break;
-      }
-      at += units;
-    }
-  }
-  __syncthreads();
+  const Stretch line = block_stretch(a, sm.stretch, [&](const PagedSequence& s) { return Line(s, a.group).all(batch.kv_heads); });
+  if (line.begin >= line.end) return;
 
   Cursor compute;
-  compute.enter(a, sm.first_seq);
-  compute.place(sm.first_offset);
+  compute.enter(a, line.seq);
+  compute.place(line.offset);
   Cursor load = compute;
-  const int count = static_cast<int>(end - begin);  // units of this block
+  const int count = static_cast<int>(line.end - line.begin);  // units of this block
   const int rows_per_box = min(1 << batch.page_shift, kWarpKeys);
   const uint32_t my_ring = smem_u32(ring) + warp * kStages * kStageBytes;
 
   // Loads unit number `i` of this block into its stage: the warp's 32 keys and values, as far as there are any.
   auto issue = [&](int i) {
     const int key0 = load.unit * kUnitKeys + warp * kWarpKeys;
-    if (key0 < load.s.length && lane == 0) {
+    if (key0 < load.s.length) {
       uint64_t* bar = &sm.full[warp][i % kStages];
       const uint32_t to = my_ring + (i % kStages) * kStageBytes;
       const int boxes = min(kWarpKeys / rows_per_box, (load.s.length - key0 + rows_per_box - 1) / rows_per_box);
-      mbar_arrive_expect_tx(bar, boxes * rows_per_box * 512);
-      for (int x = 0; x < boxes; ++x) {
-        const int at = key0 + x * rows_per_box;
-        int page = batch.tables[load.b * batch.table_stride + (at >> batch.page_shift)];
-        if (page < 0 || page >= batch.pages) {
-          report_status(a.status, kOutOfBounds);
-          page = 0;
-        }
-        const int row = at & ((1 << batch.page_shift) - 1);
-        const uint32_t box = to + x * rows_per_box * 128;
+      if (lane == 0) mbar_arrive_expect_tx(bar, boxes * rows_per_box * 512);
+      __syncwarp();
+      if (lane < boxes) {  // a lane each, so that their pages are looked up together
+        const int at = key0 + lane * rows_per_box;
+        const int page = page_at(a, load.b, at), row = at & ((1 << batch.page_shift) - 1);
+        const uint32_t box = to + lane * rows_per_box * 128;
         tma_load_4d(box, &key_map, bar, 0, row, load.head, page);
         tma_load_4d(box + kHalfBytes, &key_map, bar, 64, row, load.head, page);
         tma_load_4d(box + kSideBytes, &value_map, bar, 0, row, load.head, page);
@@ -359,10 +286,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           *reinterpret_cast<float2*>(&sm.out[warp][g + 8 * r][n * 8 + c2]) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
       }
       __syncthreads();
-      const int64_t unit0 = begin + i - compute.unit;  // the tile's place in the line
-      const int first = static_cast<int>(unit0 / share), last = static_cast<int>((unit0 + compute.units - 1) / share);
+      const int64_t unit0 = line.begin + i - compute.unit;  // the tile's place in the line
+      const int first = static_cast<int>(unit0 / line.share), last = static_cast<int>((unit0 + compute.units - 1) / line.share);
       const bool whole = first == last;
-      const int slot = 2 * blockIdx.x + (static_cast<int>(blockIdx.x) == first ? 1 : 0);
+      const int64_t slot = a.slot(blockIdx.x, first);
       for (int x = tid; x < kTileRows * kHeadDim / 4; x += kThreads) {
         const int r = x / (kHeadDim / 4), d = x % (kHeadDim / 4) * 4;
         const int row = compute.tile * kTileRows + r;
@@ -387,8 +314,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           T* to = out + (static_cast<int64_t>(t) * a.hq + compute.head * a.group + row % a.group) * kHeadDim + d;
           *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
         } else {
-          *reinterpret_cast<float4*>(a.parts + (static_cast<int64_t>(slot) * kTileRows + r) * kHeadDim + d) = v;
-          if (d == 0) a.part_stats[slot * kTileRows + r] = make_float2(mx, sum);
+          *reinterpret_cast<float4*>(a.parts + (slot + r) * kHeadDim + d) = v;
+          if (d == 0) a.part_stats[slot + r] = make_float2(mx, sum);
         }
         // (a token's rows may lie in two tiles: each tile writes its own rows' blocks)
         if (d == 0 && first == static_cast<int>(blockIdx.x))
@@ -418,8 +345,8 @@ __global__ void __launch_bounds__(256) attend_join_kernel(T* __restrict__ out, c
   }
   const int2 blocks = a.blocks_of[item];
   if (blocks.x == blocks.y) return;
-  const int r = ((t - s.start) * a.group + h % a.group) % kTileRows;
-  auto slot = [&](int block) { return static_cast<int64_t>(2 * block + (block == blocks.x ? 1 : 0)) * kTileRows + r; };
+  const int r = ((t - s.start) * a.group + h % a.group) % a.tile_rows;
+  auto slot = [&](int block) { return a.slot(block, blocks.x) + r; };
   float mx = -INFINITY;
   for (int x = blocks.x + lane; x <= blocks.y; x += 32) mx = fmaxf(mx, a.part_stats[slot(x)].x);
   mx = warp_max(mx);
@@ -457,6 +384,17 @@ CUtensorMap pool_map(const at::Tensor& pool, int box_rows) {
 
 }  // namespace
 
+void launch_attend_join(const AttendArgs& a, at::Tensor& out) {
+  const int64_t items = static_cast<int64_t>(a.batch.rows) * a.hq;
+  auto launch = [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    attend_join_kernel<T><<<static_cast<unsigned>((items + 7) / 8), 256, 0, stream()>>>(static_cast<T*>(out.data_ptr()), a);
+  };
+  if (out.scalar_type() == at::kHalf) launch(static_cast<__half*>(nullptr));
+  else launch(static_cast<__nv_bfloat16*>(nullptr));
+  TDSV_LAUNCH_CHECK();
+}
+
 at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& values, const at::Tensor& tables,
                            const at::Tensor& starts, const at::Tensor& lengths, double scale,
                            const c10::optional<at::Tensor>& tree) {
@@ -485,31 +423,38 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& keys, const at
   auto out = at::empty_like(q);
   if (rows == 0) return out;
   a.status = status_word_ptr();
+  // A tile of 16 rows reads its keys once for all of a decoding step's rows; where a sequence brings more of them (on
+  // average), tiles of 256 on the tensor cores' own pipeline do.
+  const bool many = a.group <= kRowsTile && rows * a.group > 32 * static_cast<int64_t>(a.batch.seqs);
   const int blocks = num_sms();
+  a.tile_rows = many ? kRowsTile / a.group * a.group : kTileRows;
+  a.slot_rows = many ? kRowsTile : kTileRows;
   const auto f32 = q.options().dtype(at::kFloat);
-  auto parts = at::empty({2 * blocks, kTileRows, kHeadDim}, f32);
-  auto stats = at::empty({2 * blocks, kTileRows, 2}, f32);
+  auto parts = at::empty({2 * blocks, a.slot_rows, kHeadDim}, f32);
+  auto stats = at::empty({2 * blocks, a.slot_rows, 2}, f32);
   auto blocks_of = at::empty({rows, hq, 2}, f32.dtype(at::kInt));
   a.parts = parts.data_ptr<float>();
   a.part_stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
   a.blocks_of = reinterpret_cast<int2*>(blocks_of.data_ptr<int>());
   bind_primary_context();
-  const int box_rows = std::min(1 << a.batch.page_shift, kWarpKeys);
+  const int box_rows = std::min(1 << a.batch.page_shift, many ? 128 : kWarpKeys);
   const CUtensorMap key_map = pool_map(keys, box_rows), value_map = pool_map(values, box_rows);
-  auto launch = [&](auto* tag) {
-    using T = std::remove_pointer_t<decltype(tag)>;
-    constexpr int smem = kWarps * kStages * kStageBytes + sizeof(Shared) + 1024;
-    static_assert(smem <= 227 * 1024, "fits an SM");
-    TDSV_CUDA_CHECK(cudaFuncSetAttribute(attend_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    attend_kernel<T><<<blocks, kThreads, smem, stream()>>>(key_map, value_map, static_cast<const T*>(q.data_ptr()),
-                                                           static_cast<T*>(out.data_ptr()), a);
+  if (many) {
+    launch_attend_rows(a, key_map, value_map, q, out, blocks);
+  } else {
+    auto launch = [&](auto* tag) {
+      using T = std::remove_pointer_t<decltype(tag)>;
+      constexpr int smem = kWarps * kStages * kStageBytes + sizeof(Shared) + 1024;
+      static_assert(smem <= 227 * 1024, "fits an SM");
+      TDSV_CUDA_CHECK(cudaFuncSetAttribute(attend_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      attend_kernel<T><<<blocks, kThreads, smem, stream()>>>(key_map, value_map, static_cast<const T*>(q.data_ptr()),
+                                                             static_cast<T*>(out.data_ptr()), a);
+    };
+    if (q.scalar_type() == at::kHalf) launch(static_cast<__half*>(nullptr));
+    else launch(static_cast<__nv_bfloat16*>(nullptr));
     TDSV_LAUNCH_CHECK();
-    attend_join_kernel<T><<<static_cast<unsigned>((rows * hq + 7) / 8), 256, 0, stream()>>>(
-        static_cast<T*>(out.data_ptr()), a);
-  };
-  if (q.scalar_type() == at::kHalf) launch(static_cast<__half*>(nullptr));
-  else launch(static_cast<__nv_bfloat16*>(nullptr));
-  TDSV_LAUNCH_CHECK();
+  }
+  launch_attend_join(a, out);
   return out;
 }
 

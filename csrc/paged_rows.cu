@@ -1,0 +1,437 @@
+// Attention over a paged cache where a sequence brings many rows: chunks of prompts and trees of drafted tokens.
+// (The mathematics, and the line of units that the blocks share, are at the top of paged_attention.cu.)
+//
+// A tile is up to 256 rows of one sequence and key head, whole tokens of them, as two halves of 128 (one of the
+// tensor cores' tiles each) that share every key and value. 384 threads:
+//   warp 0       producer: the unit's 128 keys, then its 128 values, by TMA through a ring of five slots of 32 KB; a lane
+//                a page, so that the pages are looked up together
+//   warp 1       issues the products: for each half PV of this unit as its weights arrive, then QK of the next one
+//   warps 4-11   softmax, a thread per row: the half's 128 scores from tensor memory into registers, the row's mask, the
+//                running maximum (raised only when it grows by more than 2^8, so that the sums in tensor memory are rarely
+//                rescaled), the weights back over the scores as the A operand of PV
+// While one half's softmax runs, the tensor cores work on the other half.
+//   TMEM: scores 0 [0, 128), scores 1 [128, 256), sums 0 [256, 384), sums 1 [384, 512).
+// Commits of QK come behind the half's last PV, so a thread that sees its next scores may touch its sums.
+#include "paged_attend.cuh"
+
+namespace tdsv {
+
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kHalfRows = 128, kUnitKeys = 128;
+constexpr int kAtomBytes = 128 * 128;    // 128 rows of 64 dims, swizzled
+constexpr int kSlotBytes = 2 * kAtomBytes;
+constexpr int kSlots = 5;
+
+enum : int { kWaitEmpty = 351, kWaitQ, kWaitKeys, kWaitValues, kWaitWeights, kWaitScores, kWaitSums, kWaitTail };
+
+template <typename T>
+__device__ __forceinline__ uint32_t product_desc(bool b_mn_major) {
+  const uint32_t d = make_idesc_bf16(128, 128, false, b_mn_major);
+  return std::is_same_v<T, __half> ? d & ~(1u << 7 | 1u << 10) : d;  // (fp16 is format 0)
+}
+
+// sum over 0 <= i < n of floor((a i + b) / m), for non-negative a and b: the lattice points under a line, by Euclid's
+// steps.
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+  int64_t sum = 0;
+  while (n > 0) {
+    sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+    a %= m;
+    b %= m;
+    const int64_t y = a * n + b;
+    if (y < m) break;
+    n = y / m;
+    b = y % m;
+    const int64_t x = a;
+    a = m;
+    m = x;
+  }
+  return sum;
+}
+
+// The units of a sequence's tiles under one key head: a causal tile ends with its last token.
+struct Tiles {
+  int tokens, prefix, n, tiles;  // tokens of a tile; cached before the new ones; new ones
+  bool causal;
+
+  __device__ __forceinline__ Tiles(const AttendArgs& a, const PagedSequence& s)
+      : tokens(a.tile_rows / a.group), prefix(s.length - s.n), n(s.n), tiles((s.n + tokens - 1) / tokens),
+        causal(a.tree_words < 0) {}
+  Tiles() = default;
+  __device__ __forceinline__ int units(int t) const {
+    return (prefix + (causal ? min(n, (t + 1) * tokens) : n) + kUnitKeys - 1) / kUnitKeys;
+  }
+  __device__ __forceinline__ int64_t before(int t) const {  // tiles [0, t)
+    if (!causal) return static_cast<int64_t>(t) * units(0);
+    if (t == 0) return 0;
+    const int64_t full = t == tiles ? units(tiles - 1) : 0;
+    return full + floor_sum(t == tiles ? t - 1 : t, kUnitKeys, tokens, prefix + tokens + kUnitKeys - 1);
+  }
+  __device__ __forceinline__ int64_t all() const { return n == 0 ? 0 : before(tiles); }
+};
+
+struct Cursor {
+  int b = 0, head = 0, tile = 0, unit = 0, units = 0;
+  PagedSequence s;
+  Tiles t;
+
+  __device__ __forceinline__ void enter(const AttendArgs& a, int seq) {
+    b = seq;
+    s = paged_sequence(a.batch, b, nullptr);
+    t = Tiles(a, s);
+    head = tile = unit = 0;
+    units = s.n == 0 ? 0 : t.units(0);
+  }
+  __device__ __forceinline__ void place(int64_t offset) {
+    const int64_t all = t.all();
+    head = static_cast<int>(offset / all);
+    offset -= head * all;
+    int lo = 0, hi = t.tiles;  // before(lo) <= offset < before(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (t.before(mid) <= offset) lo = mid;
+      else hi = mid;
+    }
+    tile = lo;
+    unit = static_cast<int>(offset - t.before(lo));
+    units = t.units(tile);
+  }
+  // To the next tile. (The caller knows that there is one.)
+  __device__ __forceinline__ void next_tile(const AttendArgs& a) {
+    unit = 0;
+    if (++tile == t.tiles) {
+      tile = 0;
+      if (++head == a.batch.kv_heads) {
+        do enter(a, b + 1);
+        while (s.n == 0 && b + 1 < a.batch.seqs);
+        return;
+      }
+    }
+    units = t.units(tile);
+  }
+  __device__ __forceinline__ int rows(const AttendArgs& a) const { return min(t.tokens, s.n - tile * t.tokens) * a.group; }
+};
+
+struct Shared {
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t kv_full[kSlots], kv_empty[kSlots];
+  StretchScratch<kThreads> stretch;
+  uint32_t tmem;
+};
+
+// 32 columns of a row's mask, from column `x` of the new tokens on (negative: before them).
+__device__ __forceinline__ uint32_t tree_columns(const uint32_t* words, int count, int n, int x) {
+  auto word = [&](int i) { return i >= 0 && i < count ? words[i] : 0u; };
+  uint32_t seen;
+  if (x <= -32) return 0xffffffffu;
+  if (x < 0) seen = (1u << -x) - 1u | word(0) << -x;
+  else seen = __funnelshift_r(word(x >> 5), word((x >> 5) + 1), x & 31);
+  const int left = n - x;  // columns that are there
+  return left >= 32 ? seen : left <= 0 ? 0u : seen & ((1u << left) - 1u);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    attend_rows_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
+                       const T* __restrict__ q, T* __restrict__ out, const __grid_constant__ AttendArgs a) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* queries = base;                    // two halves of two atoms
+  uint8_t* ring = base + 2 * kSlotBytes;
+  Shared& sm = *reinterpret_cast<Shared*>(ring + kSlots * kSlotBytes);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  if (tid == 0) {
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(&sm.q_full[h], kHalfRows);
+      mbar_init(&sm.s_full[h], 1);
+      mbar_init(&sm.p_full[h], kHalfRows);
+      mbar_init(&sm.o_full[h], 1);
+    }
+    for (int i = 0; i < kSlots; ++i) mbar_init(&sm.kv_full[i], 1), mbar_init(&sm.kv_empty[i], 1);
+    fence_barrier_init();
+  }
+  const Stretch line = block_stretch(a, sm.stretch, [&](const PagedSequence& s) {
+    return Tiles(a, s).all() * a.batch.kv_heads;
+  });
+  if (line.begin >= line.end) return;
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+
+  Cursor at;
+  at.enter(a, line.seq);
+  at.place(line.offset);
+  int left = static_cast<int>(line.end - line.begin);  // units of this block
+  bool ok = true;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (warp == 0) {
+      const int rows_per_box = min(1 << a.batch.page_shift, kUnitKeys);
+      int slot = 0, round = 0;
+      auto load = [&](const CUtensorMap* map, int key0) {
+        if (round > 0 && ok) ok = warp_wait(&sm.kv_empty[slot], (round - 1) & 1, a.status, kWaitEmpty);
+        if (!ok) return;
+        const int boxes = min(kUnitKeys / rows_per_box, (at.s.length - key0 + rows_per_box - 1) / rows_per_box);
+        if (lane == 0) mbar_arrive_expect_tx(&sm.kv_full[slot], boxes * rows_per_box * 256);
+        __syncwarp();
+        if (lane < boxes) {
+          const int place = key0 + lane * rows_per_box;
+          const int page = page_at(a, at.b, place), row = place & ((1 << a.batch.page_shift) - 1);
+          const uint32_t to = smem_u32(ring) + slot * kSlotBytes + lane * rows_per_box * 128;
+          tma_load_4d(to, map, &sm.kv_full[slot], 0, row, at.head, page);
+          tma_load_4d(to + kAtomBytes, map, &sm.kv_full[slot], 64, row, at.head, page);
+        }
+        if (++slot == kSlots) slot = 0, ++round;
+      };
+      while (ok && left > 0) {
+        const int count = min(left, at.units - at.unit);
+        // keys of a unit before the values of the one before it: their product comes first
+        load(&key_map, at.unit * kUnitKeys);
+        for (int i = 1; i <= count; ++i) {
+          if (i < count) load(&key_map, (at.unit + i) * kUnitKeys);
+          load(&value_map, (at.unit + i - 1) * kUnitKeys);
+        }
+        left -= count;
+        if (left > 0) at.next_tile(a);
+      }
+    } else if (warp == 1) {
+      if (elect_one()) {
+        const uint32_t desc_s = product_desc<T>(false), desc_o = product_desc<T>(true);
+        const uint32_t qs = smem_u32(queries), rs = smem_u32(ring);
+        int slot = 0, slot_round = 0;
+        int q_turn[2] = {0, 0}, p_turn[2] = {0, 0};
+        auto take = [&](int code) {  // the ring's next slot, when it is full
+          ok = ok && mbar_sleep_wait(&sm.kv_full[slot], slot_round & 1, a.status, code);
+          const int s = slot;
+          if (++slot == kSlots) slot = 0, ++slot_round;
+          return s;
+        };
+        auto scores = [&](int h, int s) {
+#pragma unroll
+          for (int k = 0; k < kHeadDim / 16; ++k)
+            umma_f16(tmem + h * 128, kmajor_desc(qs + h * kSlotBytes, k, kAtomBytes),
+                     kmajor_desc(rs + s * kSlotBytes, k, kAtomBytes), desc_s, k > 0);
+          umma_commit(&sm.s_full[h]);
+        };
+        auto sums = [&](int h, int s, bool more) {
+#pragma unroll
+          for (int k = 0; k < kUnitKeys / 16; ++k)
+            umma_f16_ts(tmem + 256 + h * 128, tmem + h * 128 + k * 8, mnmajor_desc(rs + s * kSlotBytes, k, kAtomBytes),
+                        desc_o, more || k > 0);
+        };
+        while (ok && left > 0) {
+          const int count = min(left, at.units - at.unit);
+          const int halves = at.rows(a) > kHalfRows ? 2 : 1;
+          const int first = take(kWaitKeys);
+          for (int h = 0; ok && h < halves; ++h) {
+            ok = mbar_sleep_wait(&sm.q_full[h], q_turn[h]++ & 1, a.status, kWaitQ);
+            if (!ok) break;
+            tc_fence_after();
+            scores(h, first);
+          }
+          if (!ok) break;
+          umma_commit(&sm.kv_empty[first]);
+          for (int i = 0; ok && i < count; ++i) {
+            const bool more = i + 1 < count;
+            const int ks = more ? take(kWaitKeys) : 0;
+            const int vs = take(kWaitValues);
+            for (int h = 0; ok && h < halves; ++h) {
+              ok = mbar_sleep_wait(&sm.p_full[h], p_turn[h]++ & 1, a.status, kWaitWeights);
+              if (!ok) break;
+              tc_fence_after();
+              sums(h, vs, i > 0);
+              if (more) scores(h, ks);
+              else umma_commit(&sm.o_full[h]);
+            }
+            if (!ok) break;
+            umma_commit(&sm.kv_empty[vs]);
+            if (more) umma_commit(&sm.kv_empty[ks]);
+          }
+          left -= count;
+          if (left > 0) at.next_tile(a);
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const int half = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t s_col = lanes + half * 128, o_col = lanes + 256 + half * 128;
+    int s_turn = 0, o_turn = 0, fetched = 0;  // `fetched`: ring slots of the tiles behind
+    int64_t place0 = line.begin;              // of the tile's first unit here
+    while (ok && left > 0) {
+      const int count = min(left, at.units - at.unit);
+      const int rows = at.rows(a), row = half * kHalfRows + r;
+      const bool active = rows > half * kHalfRows, there = row < rows;
+      const int token = there ? at.tile * at.t.tokens + row / a.group : 0, head = at.head * a.group + row % a.group;
+      const int64_t to = (static_cast<int64_t>(at.s.start + token) * a.hq + head) * kHeadDim;
+      if (active) {
+        uint8_t* mine = queries + half * kSlotBytes;
+#pragma unroll
+        for (int c = 0; c < kHeadDim / 8; ++c) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (there) v = *reinterpret_cast<const uint4*>(q + to + c * 8);
+          *reinterpret_cast<uint4*>(mine + (c >> 3) * kAtomBytes + swz(r, c & 7)) = v;
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();  // (the sums of the last tile have been read)
+        mbar_arrive(&sm.q_full[half]);
+        float m = -INFINITY, l = 0.f;
+        for (int i = 0; i < count; ++i) {
+          const int key0 = (at.unit + i) * kUnitKeys;
+          if (half == 0 && key0 + kUnitKeys > at.s.length) {
+            // what lies behind the sequence may be anything, and a weight of 0 does not undo a NaN
+            // (values of unit i: behind the keys of the next one, where the tile has one here)
+            const int n = fetched + (i + 1 < count ? 2 * i + 2 : 2 * i + 1), s = n % kSlots;
+            if (!(ok = warp_wait(&sm.kv_full[s], (n / kSlots) & 1, a.status, kWaitTail))) break;
+            if (key0 + r >= at.s.length) {
+              uint8_t* v = ring + s * kSlotBytes + r * 128;
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                *reinterpret_cast<uint4*>(v + c * 16) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(v + kAtomBytes + c * 16) = make_uint4(0, 0, 0, 0);
+              }
+            }
+            fence_proxy_async_smem();
+          }
+          if (!(ok = warp_wait(&sm.s_full[half], s_turn++ & 1, a.status, kWaitScores))) break;
+          tc_fence_after();
+          uint32_t sv[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_col + c * 32, sv[c]);
+          tmem_ld_wait();
+          // what the row sees; nothing is hidden before the tile's first token
+          const int x0 = key0 - at.t.prefix;
+          if (x0 + kUnitKeys > (at.t.causal ? at.tile * at.t.tokens : 0)) {
+            const uint32_t* words = a.tree + static_cast<int64_t>(at.s.start + token) * max(a.tree_words, 0);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t seen;
+              if (at.t.causal) {
+                const int see = token - (x0 + c * 32) + 1;
+                seen = see >= 32 ? 0xffffffffu : see <= 0 ? 0u : (1u << see) - 1u;
+              } else {
+                seen = tree_columns(words, a.tree_words, at.s.n, x0 + c * 32);
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (!(seen >> j & 1u)) sv[c][j] = __float_as_uint(-INFINITY);
+            }
+          }
+          float m8[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m8[j] = __uint_as_float(sv[0][j]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int j = c == 0 ? 8 : 0; j < 32; ++j) m8[j & 7] = fmaxf(m8[j & 7], __uint_as_float(sv[c][j]));
+          const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
+                                 fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) *
+                           a.scale_log2;
+          float alpha = 1.f;
+          if (mx > m + 8.f) {
+            alpha = ex2_approx(m - mx);  // (0 from -inf)
+            m = mx;
+          }
+          if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t ov[32];
+              tmem_ld_32x32b_x32(o_col + c * 32, ov);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * alpha);
+              tmem_st_32x32b_x32(o_col + c * 32, ov);
+            }
+          }
+          const float zero = m == -INFINITY ? 0.f : m;
+          float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 4; c += 2) {
+            uint32_t packed[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float p0 = ex2_approx(fmaf(__uint_as_float(sv[c + (j >> 4)][2 * (j & 15)]), a.scale_log2, -zero));
+              const float p1 = ex2_approx(fmaf(__uint_as_float(sv[c + (j >> 4)][2 * (j & 15) + 1]), a.scale_log2, -zero));
+              s4[j & 3] += p0 + p1;
+              packed[j] = pack2<T>(p0, p1);
+            }
+            tmem_st_32x32b_x32(s_col + c * 16, packed);
+          }
+          l = l * alpha + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(&sm.p_full[half]);
+        }
+        if (!ok || !(ok = warp_wait(&sm.o_full[half], o_turn++ & 1, a.status, kWaitSums))) break;
+        tc_fence_after();
+        const int64_t unit0 = place0 - at.unit;
+        const int first = static_cast<int>(unit0 / line.share), last = static_cast<int>((unit0 + at.units - 1) / line.share);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int64_t slot = a.slot(blockIdx.x, first) + row;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t ov[32];
+          tmem_ld_32x32b_x32(o_col + c * 32, ov);
+          tmem_ld_wait();
+          if (!there) continue;
+          if (first == last) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              auto o = [&](int x) { return __uint_as_float(ov[8 * j + x]) * inv; };
+              *reinterpret_cast<uint4*>(out + to + c * 32 + j * 8) =
+                  make_uint4(pack2<T>(o(0), o(1)), pack2<T>(o(2), o(3)), pack2<T>(o(4), o(5)), pack2<T>(o(6), o(7)));
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<uint4*>(a.parts + slot * kHeadDim + c * 32 + j * 4) =
+                  make_uint4(ov[4 * j], ov[4 * j + 1], ov[4 * j + 2], ov[4 * j + 3]);
+          }
+        }
+        if (there && first != last) a.part_stats[slot] = make_float2(m, l);
+        if (there && first == static_cast<int>(blockIdx.x)) a.blocks_of[to / kHeadDim] = make_int2(first, last);
+      }
+      fetched += 2 * count;
+      place0 += count;
+      left -= count;
+      if (left > 0) at.next_tile(a);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace
+
+void launch_attend_rows(const AttendArgs& a, const CUtensorMap& key_map, const CUtensorMap& value_map, const at::Tensor& q,
+                        at::Tensor& out, int blocks) {
+  auto launch = [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    constexpr int smem = (2 + kSlots) * kSlotBytes + sizeof(Shared) + 1024;
+    static_assert(smem <= 227 * 1024, "fits an SM");
+    TDSV_CUDA_CHECK(cudaFuncSetAttribute(attend_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attend_rows_kernel<T><<<blocks, kThreads, smem, stream()>>>(key_map, value_map, static_cast<const T*>(q.data_ptr()),
+                                                                static_cast<T*>(out.data_ptr()), a);
+  };
+  if (q.scalar_type() == at::kHalf) launch(static_cast<__half*>(nullptr));
+  else launch(static_cast<__nv_bfloat16*>(nullptr));
+  TDSV_LAUNCH_CHECK();
+}
+
+}  // namespace tdsv

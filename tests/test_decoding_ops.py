@@ -285,6 +285,16 @@ def test_attention_long_and_many():
     _attend(new, [n + (b * 37) % 90 for b, n in enumerate(new)], (2, 1), 16, torch.float16, "cuda", seed=5)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads, page, dtype", [((8, 1), 16, torch.bfloat16), ((5, 1), 64, torch.float16),
+                                                ((6, 2), 128, torch.bfloat16), ((48, 1), 32, torch.bfloat16)])
+def test_attention_of_prompts(heads, page, dtype):
+    """Tiles of many rows: ragged ends, cached prefixes, tiles that several blocks share, sequences without new tokens."""
+    _attend([700, 0, 3, 1, 257], [1900, 40, 5, 1, 257], heads, page, dtype, "cuda", extra=2, sharp=3.0)
+    _attend([1100], [1100], heads, page, dtype, "cuda")
+    _attend([100, 64, 31] * 9, [6000, 64, 900] * 9, heads, page, dtype, "cuda", sharp=2.0)
+
+
 def _random_tree(new, words, seed, device="cpu"):
     parents, gen = [], _gen(seed)
     for n in new:
@@ -295,7 +305,7 @@ def _random_tree(new, words, seed, device="cpu"):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("new, lengths", [([1], [1]), ([7], [7]), ([32], [40]), ([33, 0, 5], [200, 4, 130]),
-                                          ([70, 64], [200, 64]), ([128], [300])])
+                                          ([70, 64], [200, 64]), ([128], [300]), ([60] * 5, [1000, 60, 61, 127, 129])])
 @pytest.mark.parametrize("heads, page, dtype", [((4, 2), 16, torch.bfloat16), ((8, 1), 64, torch.float16)])
 def test_attention_of_trees(device, new, lengths, heads, page, dtype):
     _attend(new, lengths, heads, page, dtype, device, tree=_random_tree(new, -(-max(new) // 32), 3))
