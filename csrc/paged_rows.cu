@@ -72,46 +72,28 @@ struct Tiles {
   __device__ __forceinline__ int64_t all() const { return n == 0 ? 0 : before(tiles); }
 };
 
-struct Cursor {
-  int b = 0, head = 0, tile = 0, unit = 0, units = 0;
+// A tile of the line, and what a block does of it: `count` units from `unit` on.
+struct Place {
+  int b, head, tile;
+};
+struct Part {
   PagedSequence s;
   Tiles t;
+  int unit, units, count, rows;
 
-  __device__ __forceinline__ void enter(const AttendArgs& a, int seq) {
-    b = seq;
-    s = paged_sequence(a.batch, b, nullptr);
-    t = Tiles(a, s);
-    head = tile = unit = 0;
-    units = s.n == 0 ? 0 : t.units(0);
-  }
-  __device__ __forceinline__ void place(int64_t offset) {
-    const int64_t all = t.all();
-    head = static_cast<int>(offset / all);
-    offset -= head * all;
-    int lo = 0, hi = t.tiles;  // before(lo) <= offset < before(hi)
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (t.before(mid) <= offset) lo = mid;
-      else hi = mid;
+  __device__ __forceinline__ Part(const AttendArgs& a, const Place& at, int unit_, int left)
+      : s(paged_sequence(a.batch, at.b, nullptr)), t(a, s), unit(unit_), units(t.units(at.tile)),
+        count(min(left, units - unit)), rows(min(t.tokens, s.n - at.tile * t.tokens) * a.group) {}
+  // (the caller knows that there is a next tile)
+  __device__ __forceinline__ void next(const AttendArgs& a, Place& at) const {
+    ++at.tile;
+    if (at.tile == t.tiles) at.tile = 0, ++at.head;
+    if (at.head == a.batch.kv_heads) {
+      at.head = 0;
+      ++at.b;
+      while (at.b + 1 < a.batch.seqs && paged_sequence(a.batch, at.b, nullptr).n == 0) ++at.b;
     }
-    tile = lo;
-    unit = static_cast<int>(offset - t.before(lo));
-    units = t.units(tile);
   }
-  // To the next tile. (The caller knows that there is one.)
-  __device__ __forceinline__ void next_tile(const AttendArgs& a) {
-    unit = 0;
-    if (++tile == t.tiles) {
-      tile = 0;
-      if (++head == a.batch.kv_heads) {
-        do enter(a, b + 1);
-        while (s.n == 0 && b + 1 < a.batch.seqs);
-        return;
-      }
-    }
-    units = t.units(tile);
-  }
-  __device__ __forceinline__ int rows(const AttendArgs& a) const { return min(t.tokens, s.n - tile * t.tokens) * a.group; }
 };
 
 struct Shared {
@@ -120,6 +102,15 @@ struct Shared {
   StretchScratch<kThreads> stretch;
   uint32_t tmem;
 };
+
+// 16 columns of this warp's 32 TMEM lanes.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
 
 // 32 columns of a row's mask, from column `x` of the new tokens on (negative: before them).
 __device__ __forceinline__ uint32_t tree_columns(const uint32_t* words, int count, int n, int x) {
@@ -166,9 +157,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
 
-  Cursor at;
-  at.enter(a, line.seq);
-  at.place(line.offset);
+  Place at{line.seq, 0, 0};
+  int unit;  // where the block's first tile begins for it; later ones begin with their first
+  {
+    const Tiles t(a, paged_sequence(a.batch, at.b, nullptr));
+    const int64_t all = t.all();
+    at.head = static_cast<int>(line.offset / all);
+    const int64_t offset = line.offset - at.head * all;
+    int hi = t.tiles;  // before(tile) <= offset < before(hi)
+    while (hi - at.tile > 1) {
+      const int mid = (at.tile + hi) / 2;
+      if (t.before(mid) <= offset) at.tile = mid;
+      else hi = mid;
+    }
+    unit = static_cast<int>(offset - t.before(at.tile));
+  }
   int left = static_cast<int>(line.end - line.begin);  // units of this block
   bool ok = true;
 
@@ -177,10 +180,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
       const int rows_per_box = min(1 << a.batch.page_shift, kUnitKeys);
       int slot = 0, round = 0;
-      auto load = [&](const CUtensorMap* map, int key0) {
+      auto load = [&](const CUtensorMap* map, int key0, int length) {
         if (round > 0 && ok) ok = warp_wait(&sm.kv_empty[slot], (round - 1) & 1, a.status, kWaitEmpty);
         if (!ok) return;
-        const int boxes = min(kUnitKeys / rows_per_box, (at.s.length - key0 + rows_per_box - 1) / rows_per_box);
+        const int boxes = min(kUnitKeys / rows_per_box, (length - key0 + rows_per_box - 1) / rows_per_box);
         if (lane == 0) mbar_arrive_expect_tx(&sm.kv_full[slot], boxes * rows_per_box * 256);
         __syncwarp();
         if (lane < boxes) {
@@ -193,22 +196,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (++slot == kSlots) slot = 0, ++round;
       };
       while (ok && left > 0) {
-        const int count = min(left, at.units - at.unit);
+        const Part p(a, at, unit, left);
         // keys of a unit before the values of the one before it: their product comes first
-        load(&key_map, at.unit * kUnitKeys);
-        for (int i = 1; i <= count; ++i) {
-          if (i < count) load(&key_map, (at.unit + i) * kUnitKeys);
-          load(&value_map, (at.unit + i - 1) * kUnitKeys);
+        load(&key_map, unit * kUnitKeys, p.s.length);
+        for (int i = 1; i <= p.count; ++i) {
+          if (i < p.count) load(&key_map, (unit + i) * kUnitKeys, p.s.length);
+          load(&value_map, (unit + i - 1) * kUnitKeys, p.s.length);
         }
-        left -= count;
-        if (left > 0) at.next_tile(a);
+        left -= p.count;
+        unit = 0;
+        if (left > 0) p.next(a, at);
       }
     } else if (warp == 1) {
       if (elect_one()) {
         const uint32_t desc_s = product_desc<T>(false), desc_o = product_desc<T>(true);
         const uint32_t qs = smem_u32(queries), rs = smem_u32(ring);
         int slot = 0, slot_round = 0;
-        int q_turn[2] = {0, 0}, p_turn[2] = {0, 0};
+        uint32_t q_turn = 0, p_turn = 0;  // parities, a bit for each half
         auto take = [&](int code) {  // the ring's next slot, when it is full
           ok = ok && mbar_sleep_wait(&sm.kv_full[slot], slot_round & 1, a.status, code);
           const int s = slot;
@@ -229,23 +233,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                         desc_o, more || k > 0);
         };
         while (ok && left > 0) {
-          const int count = min(left, at.units - at.unit);
-          const int halves = at.rows(a) > kHalfRows ? 2 : 1;
+          const Part p(a, at, unit, left);
+          const int halves = p.rows > kHalfRows ? 2 : 1;
           const int first = take(kWaitKeys);
           for (int h = 0; ok && h < halves; ++h) {
-            ok = mbar_sleep_wait(&sm.q_full[h], q_turn[h]++ & 1, a.status, kWaitQ);
+            ok = mbar_sleep_wait(&sm.q_full[h], q_turn >> h & 1, a.status, kWaitQ);
+            q_turn ^= 1u << h;
             if (!ok) break;
             tc_fence_after();
             scores(h, first);
           }
           if (!ok) break;
           umma_commit(&sm.kv_empty[first]);
-          for (int i = 0; ok && i < count; ++i) {
-            const bool more = i + 1 < count;
+          for (int i = 0; ok && i < p.count; ++i) {
+            const bool more = i + 1 < p.count;
             const int ks = more ? take(kWaitKeys) : 0;
             const int vs = take(kWaitValues);
             for (int h = 0; ok && h < halves; ++h) {
-              ok = mbar_sleep_wait(&sm.p_full[h], p_turn[h]++ & 1, a.status, kWaitWeights);
+              ok = mbar_sleep_wait(&sm.p_full[h], p_turn >> h & 1, a.status, kWaitWeights);
+              p_turn ^= 1u << h;
               if (!ok) break;
               tc_fence_after();
               sums(h, vs, i > 0);
@@ -256,8 +262,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma_commit(&sm.kv_empty[vs]);
             if (more) umma_commit(&sm.kv_empty[ks]);
           }
-          left -= count;
-          if (left > 0) at.next_tile(a);
+          left -= p.count;
+          unit = 0;
+          if (left > 0) p.next(a, at);
         }
       }
       __syncwarp();
@@ -270,11 +277,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     int s_turn = 0, o_turn = 0, fetched = 0;  // `fetched`: ring slots of the tiles behind
     int64_t place0 = line.begin;              // of the tile's first unit here
     while (ok && left > 0) {
-      const int count = min(left, at.units - at.unit);
-      const int rows = at.rows(a), row = half * kHalfRows + r;
-      const bool active = rows > half * kHalfRows, there = row < rows;
-      const int token = there ? at.tile * at.t.tokens + row / a.group : 0, head = at.head * a.group + row % a.group;
-      const int64_t to = (static_cast<int64_t>(at.s.start + token) * a.hq + head) * kHeadDim;
+      const Part p(a, at, unit, left);
+      const int row = half * kHalfRows + r;
+      const bool active = p.rows > half * kHalfRows, there = row < p.rows;
+      const int token = there ? at.tile * p.t.tokens + row / a.group : 0, head = at.head * a.group + row % a.group;
+      const int64_t to = (static_cast<int64_t>(p.s.start + token) * a.hq + head) * kHeadDim;
       if (active) {
         uint8_t* mine = queries + half * kSlotBytes;
 #pragma unroll
@@ -287,14 +294,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();  // (the sums of the last tile have been read)
         mbar_arrive(&sm.q_full[half]);
         float m = -INFINITY, l = 0.f;
-        for (int i = 0; i < count; ++i) {
-          const int key0 = (at.unit + i) * kUnitKeys;
-          if (half == 0 && key0 + kUnitKeys > at.s.length) {
+        for (int i = 0; i < p.count; ++i) {
+          const int key0 = (unit + i) * kUnitKeys;
+          if (half == 0 && key0 + kUnitKeys > p.s.length) {
             // what lies behind the sequence may be anything, and a weight of 0 does not undo a NaN
             // (values of unit i: behind the keys of the next one, where the tile has one here)
-            const int n = fetched + (i + 1 < count ? 2 * i + 2 : 2 * i + 1), s = n % kSlots;
+            const int n = fetched + (i + 1 < p.count ? 2 * i + 2 : 2 * i + 1), s = n % kSlots;
             if (!(ok = warp_wait(&sm.kv_full[s], (n / kSlots) & 1, a.status, kWaitTail))) break;
-            if (key0 + r >= at.s.length) {
+            if (key0 + r >= p.s.length) {
               uint8_t* v = ring + s * kSlotBytes + r * 128;
 #pragma unroll
               for (int c = 0; c < 8; ++c) {
@@ -306,35 +313,42 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (!(ok = warp_wait(&sm.s_full[half], s_turn++ & 1, a.status, kWaitScores))) break;
           tc_fence_after();
-          uint32_t sv[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_col + c * 32, sv[c]);
-          tmem_ld_wait();
           // what the row sees; nothing is hidden before the tile's first token
-          const int x0 = key0 - at.t.prefix;
-          if (x0 + kUnitKeys > (at.t.causal ? at.tile * at.t.tokens : 0)) {
-            const uint32_t* words = a.tree + static_cast<int64_t>(at.s.start + token) * max(a.tree_words, 0);
+          const int x0 = key0 - p.t.prefix;
+          const bool masked = x0 + kUnitKeys > (p.t.causal ? at.tile * p.t.tokens : 0);
+          uint32_t seen[4];
+          if (masked) {
+            const uint32_t* words = a.tree + static_cast<int64_t>(p.s.start + token) * max(a.tree_words, 0);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              uint32_t seen;
-              if (at.t.causal) {
+              if (p.t.causal) {
                 const int see = token - (x0 + c * 32) + 1;
-                seen = see >= 32 ? 0xffffffffu : see <= 0 ? 0u : (1u << see) - 1u;
+                seen[c] = see >= 32 ? 0xffffffffu : see <= 0 ? 0u : (1u << see) - 1u;
               } else {
-                seen = tree_columns(words, a.tree_words, at.s.n, x0 + c * 32);
+                seen[c] = tree_columns(words, a.tree_words, p.s.n, x0 + c * 32);
               }
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (!(seen >> j & 1u)) sv[c][j] = __float_as_uint(-INFINITY);
             }
           }
+          // The scores are read twice, for the maximum and for the weights: held in registers they would leave the loop
+          // spilling (to L2: the ring leaves next to nothing of L1). 32 columns are read ahead of those at work.
+          uint32_t sv[2][32];
           float m8[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) m8[j] = __uint_as_float(sv[0][j]);
+          for (int j = 0; j < 8; ++j) m8[j] = -INFINITY;
+          tmem_ld_32x32b_x32(s_col, sv[0]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 4; ++c) {
+            uint32_t(&v)[32] = sv[c & 1];
+            tmem_ld_wait();
+            tmem_ld_32x32b_x32(s_col + (c + 1 & 3) * 32, sv[c + 1 & 1]);  // (behind the last the first again, for the weights)
+            if (masked) {
 #pragma unroll
-            for (int j = c == 0 ? 8 : 0; j < 32; ++j) m8[j & 7] = fmaxf(m8[j & 7], __uint_as_float(sv[c][j]));
+              for (int j = 0; j < 32; ++j) m8[j & 7] = fmaxf(m8[j & 7], seen[c] >> j & 1u ? __uint_as_float(v[j]) : -INFINITY);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) m8[j & 7] = fmaxf(m8[j & 7], __uint_as_float(v[j]));
+            }
+          }
           const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
                                  fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) *
                            a.scale_log2;
@@ -343,30 +357,40 @@ __global__ void __launch_bounds__(kThreads, 1)
             alpha = ex2_approx(m - mx);  // (0 from -inf)
             m = mx;
           }
+          tmem_ld_wait();
           if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t ov[32];
-              tmem_ld_32x32b_x32(o_col + c * 32, ov);
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {  // (rare)
+              uint32_t ov[16];
+              tmem_ld_32x32b_x16(o_col + c * 16, ov);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * alpha);
-              tmem_st_32x32b_x32(o_col + c * 32, ov);
+              for (int j = 0; j < 16; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * alpha);
+              tmem_st_32x32b_x16(o_col + c * 16, ov);
             }
           }
           const float zero = m == -INFINITY ? 0.f : m;
           float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int c = 0; c < 4; c += 2) {
-            uint32_t packed[32];
+          for (int c = 0; c < 4; ++c) {
+            uint32_t(&v)[32] = sv[c & 1];
+            if (c > 0) tmem_ld_wait();
+            if (c < 3) tmem_ld_32x32b_x32(s_col + (c + 1) * 32, sv[c + 1 & 1]);
+            uint32_t packed[16];
+            if (masked) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float p0 = ex2_approx(fmaf(__uint_as_float(sv[c + (j >> 4)][2 * (j & 15)]), a.scale_log2, -zero));
-              const float p1 = ex2_approx(fmaf(__uint_as_float(sv[c + (j >> 4)][2 * (j & 15) + 1]), a.scale_log2, -zero));
+              for (int j = 0; j < 32; ++j)
+                if (!(seen[c] >> j & 1u)) v[j] = __float_as_uint(-INFINITY);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float p0 = ex2_approx(fmaf(__uint_as_float(v[2 * j]), a.scale_log2, -zero));
+              const float p1 = ex2_approx(fmaf(__uint_as_float(v[2 * j + 1]), a.scale_log2, -zero));
               s4[j & 3] += p0 + p1;
               packed[j] = pack2<T>(p0, p1);
             }
-            tmem_st_32x32b_x32(s_col + c * 16, packed);
+            // (these columns end before the scores that are still to be read)
+            tmem_st_32x32b_x16(s_col + c * 16, packed);
           }
           l = l * alpha + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
           tmem_st_wait();
@@ -375,8 +399,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!ok || !(ok = warp_wait(&sm.o_full[half], o_turn++ & 1, a.status, kWaitSums))) break;
         tc_fence_after();
-        const int64_t unit0 = place0 - at.unit;
-        const int first = static_cast<int>(unit0 / line.share), last = static_cast<int>((unit0 + at.units - 1) / line.share);
+        const int64_t unit0 = place0 - unit;
+        const int first = static_cast<int>(unit0 / line.share), last = static_cast<int>((unit0 + p.units - 1) / line.share);
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int64_t slot = a.slot(blockIdx.x, first) + row;
 #pragma unroll
@@ -402,10 +426,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (there && first != last) a.part_stats[slot] = make_float2(m, l);
         if (there && first == static_cast<int>(blockIdx.x)) a.blocks_of[to / kHeadDim] = make_int2(first, last);
       }
-      fetched += 2 * count;
-      place0 += count;
-      left -= count;
-      if (left > 0) at.next_tile(a);
+      fetched += 2 * p.count;
+      place0 += p.count;
+      left -= p.count;
+      unit = 0;
+      if (left > 0) p.next(a, at);
     }
   }
   tc_fence_before();
