@@ -101,7 +101,8 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& keys, const at
 at::Tensor process_logits(const at::Tensor& logits, const c10::optional<at::Tensor>& history,
                           const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& prompt_lengths,
                           const c10::optional<at::Tensor>& repetition, const c10::optional<at::Tensor>& presence,
-                          const c10::optional<at::Tensor>& frequency, const c10::optional<at::Tensor>& bias_ids,
+                          const c10::optional<at::Tensor>& frequency, double repetition_, double presence_,
+                          double frequency_, const c10::optional<at::Tensor>& bias_ids,
                           const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& allowed);
 // lm_head.cu
 std::vector<at::Tensor> lm_head_stats_fwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,

@@ -10,9 +10,9 @@
 // in fp32, rounded once to the logits' type.
 //
 // A row is cut into slices of the vocabulary, a block each. A block counts the history's tokens of its slice in
-// shared memory (whole numbers: the order of the atomics changes nothing), copies the slice under the mask in 16-byte
-// vectors, and then rewrites the few tokens that a count or a bias touches: what is copied never passes through fp32,
-// and the counts cost no work per token of the vocabulary beyond a scan of shared memory.
+// shared memory (whole numbers: the order of the atomics changes nothing) and then streams the slice in 16-byte vectors,
+// read once: a vector without a count, and most are, is only masked and never passes through fp32. A vector that the
+// mask hides altogether is not read.
 #include "logit_rows.cuh"
 
 namespace tdsv {
@@ -20,10 +20,24 @@ namespace tdsv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 4;  // vectors a thread has in flight
+constexpr int kAhead = 4;          // vectors a thread has in flight
+constexpr int kPad = 16;           // counts beyond a slice's, for their alignment
+constexpr int kListed = 1024;      // biases of a slice that shared memory holds
 
-// A token's word: how often it is output, and flags.
-constexpr uint32_t kPrompt = 1u << 31, kBiased = 1u << 30, kRepeated = 1u << 29, kCount = kRepeated - 1;
+// A token's count and two flags. 16 bits hold the counts of histories below 2^14 tokens, in half the shared memory, so
+// that four blocks of the largest slice fit an SM; longer ones take 32.
+template <typename C>
+struct Count {
+  static constexpr uint32_t kPrompt = sizeof(C) == 2 ? 0x8000u : 0x80000000u, kBiased = kPrompt >> 1, kTimes = kBiased - 1;
+  static constexpr int kMost = static_cast<int>(sizeof(C) == 2 ? kTimes : kTimes >> 1);
+  static __device__ __forceinline__ void add(C* at, uint32_t what, bool flag) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(at);
+    if (sizeof(C) == 2) what <<= (p & 2) * 8;
+    uint32_t* word = reinterpret_cast<uint32_t*>(p & ~uintptr_t(3));
+    if (flag) atomicOr(word, what);
+    else atomicAdd(word, what);
+  }
+};
 
 template <typename T>
 __device__ __forceinline__ uint32_t minus_inf_pair() {  // two of a 16-bit type, or one of fp32
@@ -59,27 +73,100 @@ __device__ __forceinline__ uint32_t mask_bits(const uint32_t* words, int at, int
   return bits;
 }
 
-// out[0, n) = row[0, n) where the mask allows it. Vectors are aligned at `out`; where the logits lie at another
-// offset in their 16 bytes, two of theirs are joined. A vector whose bits are all clear is not read.
-template <typename T>
-__device__ __forceinline__ void copy_masked(const T* row, T* out, int n, const uint32_t* words) {
+struct Penalties {
+  const void* history;         // ids so far [rows, history], int64 or int32; null: none
+  const int* lengths;          // of each row's history; null: all of it
+  const int* prompt_lengths;   // of its part that is not output; null: 0
+  const float *repetition, *presence, *frequency;  // one per row; null: the number
+  float repetition_, presence_, frequency_;
+  const int64_t* bias_ids;     // [rows, biases]; null: none
+  const float* bias;
+  const uint32_t* allowed;     // [rows, words]; null: all
+  int64_t history_stride, bias_stride, allowed_stride;
+  int history_size, biases;
+  bool wide;  // ids of 64 bits
+};
+
+// What a row's touched tokens become.
+struct Change {
+  float repetition, presence, frequency;
+  const int* ids;         // biases of the slice, in their order (token within the slice)
+  const float* values;
+  int biases;
+  // of the whole row, where shared memory does not hold the slice's
+  const int64_t* row_ids;
+  int begin;
+
+  template <typename C>
+  __device__ __forceinline__ float operator()(float x, uint32_t count, int v) const {
+    const uint32_t times = count & Count<C>::kTimes;
+    if (times != 0 || (count & Count<C>::kPrompt)) x = x > 0.f ? x / repetition : x * repetition;
+    if (times != 0) x = x - frequency * static_cast<float>(times) - presence;
+    if (count & Count<C>::kBiased) {
+      float sum = 0.f;
+      if (row_ids == nullptr) {
+        for (int k = 0; k < biases; ++k) sum += ids[k] == v ? values[k] : 0.f;
+      } else {
+        for (int k = 0; k < biases; ++k) sum += row_ids[k] == begin + v ? values[k] : 0.f;
+      }
+      x += sum;
+    }
+    return x;
+  }
+};
+
+template <typename T, typename C>
+__device__ __forceinline__ uint4 change_vec(const uint4& v, const C* counts, int at, const Change& change) {
+  uint32_t out[4];
+#pragma unroll
+  for (int i = 0; i < LogitVec<T>::kPairs; ++i) {
+    float2 f = unpack_pair<T>(v, i);
+    if (counts[2 * i] != 0) f.x = change.template operator()<C>(f.x, counts[2 * i], at + 2 * i);
+    if (counts[2 * i + 1] != 0) f.y = change.template operator()<C>(f.y, counts[2 * i + 1], at + 2 * i + 1);
+    if constexpr (sizeof(T) == 2) {
+      out[i] = pack_pair<T>(f.x, f.y);  // (an untouched value is one of the type, and stays)
+    } else {
+      out[2 * i] = __float_as_uint(f.x);
+      out[2 * i + 1] = __float_as_uint(f.y);
+    }
+  }
+  return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+// C: the counts' type; void where no token is touched. Dynamic shared memory: counts [slice + kPad].
+template <typename T, typename C>
+__global__ void __launch_bounds__(kThreads, std::is_void_v<C> ? 4 : 3)
+    process_kernel(const T* __restrict__ logits, RowLayout layout, int vocab, int slice, int parts,
+                   const __grid_constant__ Penalties p, T* __restrict__ out, int* __restrict__ status) {
+  constexpr bool kTouched = !std::is_void_v<C>;
+  using Word = std::conditional_t<kTouched, C, uint16_t>;
   constexpr int kSize = LogitVec<T>::kSize;
   constexpr uint32_t kAll = (1u << kSize) - 1;
-  const RowCut cut = cut_row(out, n);
+  extern __shared__ uint4 smem[];
+  __shared__ int listed_ids[kTouched ? kListed : 1];
+  __shared__ float listed_values[kTouched ? kListed : 1];
+  __shared__ int listed;
+  const uint32_t r = blockIdx.x / parts;
+  const int begin = static_cast<int>(blockIdx.x - r * parts) * slice, n = min(slice, vocab - begin);
   const int tid = threadIdx.x;
-  const auto one = [&](int i) { out[i] = mask_bits(words, i, 1) & 1u ? row[i] : from_float<T>(-INFINITY); };
-  if (tid < cut.head) one(tid);
-  if (tid >= 32 && tid < 32 + cut.tail) one(n - cut.tail + tid - 32);
+  const T* row = logits + layout.offset(r) + begin;
+  T* to = out + static_cast<int64_t>(r) * vocab + begin;
+  const uint32_t* words = p.allowed == nullptr ? nullptr : p.allowed + r * p.allowed_stride + begin / 32;
+  // Vectors are aligned at `out`; where the logits lie at another offset in their 16 bytes, two of theirs are joined. The
+  // vectors whose parts all lie inside the row are [first, last): with an offset, at most two do not.
+  const RowCut cut = cut_row(to, n);
   const T* from = row + cut.head;
-  uint4* to = reinterpret_cast<uint4*>(out + cut.head);
+  uint4* vecs = reinterpret_cast<uint4*>(to + cut.head);
   const int off = static_cast<int>((reinterpret_cast<uintptr_t>(from) & 15) / sizeof(T));
-  // the vectors whose parts all lie inside the row: with an offset, at most the first and the last do not
   const uint4* x = reinterpret_cast<const uint4*>(from - off);
   const int first = off > cut.head ? 1 : 0;
   const int last = off == 0 ? cut.vecs : min(cut.vecs, (n - cut.head + off) / kSize - 1);
-  for (int i = first + tid; i < last; i += kThreads * kAhead) {
-    uint4 lo[kAhead], hi[kAhead];
-    uint32_t bits[kAhead];
+  // token v of the slice is counted at counts[v]: a vector's counts are aligned as it is
+  Word* counts = reinterpret_cast<Word*>(smem) + (kSize - cut.head) % kSize;
+
+  uint4 lo[kAhead], hi[kAhead];
+  uint32_t bits[kAhead];
+  const auto fetch = [&](int i) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int at = i + u * kThreads;
@@ -91,50 +178,14 @@ __device__ __forceinline__ void copy_masked(const T* row, T* out, int n, const u
       lo[u] = load_stream(x + i + u * kThreads);
       if (off != 0) hi[u] = load_stream(x + i + u * kThreads + 1);
     }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (i + u * kThreads >= last) continue;
-      uint4 v = lo[u];
-      if (off != 0) v = shift_vec(lo[u], hi[u], off * static_cast<int>(sizeof(T)));
-      to[i + u * kThreads] = mask_vec<T>(v, bits[u]);
-    }
-  }
-  if (off != 0 && tid < 2 * kSize && cut.vecs > 0) {  // (two vectors at most, one value a thread)
-    const int i = tid < kSize ? 0 : cut.vecs - 1;
-    const bool todo = tid < kSize ? first == 1 : last < cut.vecs && (cut.vecs > 1 || first == 0);
-    if (todo) one(cut.head + i * kSize + tid % kSize);
-  }
-}
+  };
+  fetch(first + tid);  // on their way while the history is counted
 
-struct Penalties {
-  const void* history;         // ids so far [rows, history], int64 or int32; null: none
-  const int* lengths;          // of each row's history; null: all of it
-  const int* prompt_lengths;   // of its part that is not output; null: 0
-  const float *repetition, *presence, *frequency;  // one per row; null: none
-  const int64_t* bias_ids;     // [rows, biases]; null: none
-  const float* bias;
-  const uint32_t* allowed;     // [rows, words]; null: all
-  int64_t history_stride, bias_stride, allowed_stride;
-  int history_size, biases;
-  bool wide;  // ids of 64 bits
-};
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) process_kernel(const T* __restrict__ logits, RowLayout layout, int vocab,
-                                                           int slice, int parts, Penalties p, T* __restrict__ out,
-                                                           int* __restrict__ status) {
-  extern __shared__ uint4 smem[];
-  uint32_t* counts = reinterpret_cast<uint32_t*>(smem);                    // [slice], where any token is touched
-  float* biases = reinterpret_cast<float*>(counts + slice);                // [slice], where there are biases
-  const uint32_t r = blockIdx.x / parts;
-  const int begin = static_cast<int>(blockIdx.x - r * parts) * slice, n = min(slice, vocab - begin);
-  const int tid = threadIdx.x;
-  const T* row = logits + layout.offset(r) + begin;
-  T* to = out + static_cast<int64_t>(r) * vocab + begin;
-  const uint32_t* words = p.allowed == nullptr ? nullptr : p.allowed + r * p.allowed_stride + begin / 32;
-  const bool touched = p.history != nullptr || p.bias_ids != nullptr;
-  if (touched) {
-    for (int i = tid; i < slice / 4; i += kThreads) smem[i] = make_uint4(0, 0, 0, 0);
+  Change change{};
+  if constexpr (kTouched) {
+    const int all = static_cast<int>((slice + kPad) * sizeof(C) / 16);
+    for (int i = tid; i < all; i += kThreads) smem[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) listed = 0;
     __syncthreads();
     if (p.history != nullptr) {
       int length = p.history_size;
@@ -157,55 +208,98 @@ __global__ void __launch_bounds__(kThreads) process_kernel(const T* __restrict__
         for (int u = 0; u < kAhead; ++u) {
           if (id[u] >= vocab) report_status(status, kOutOfBounds);
           if (id[u] < begin || id[u] >= begin + n) continue;
-          if (i + u * kThreads < prompt) atomicOr(&counts[id[u] - begin], kPrompt);
-          else atomicAdd(&counts[id[u] - begin], 1u);
+          const bool said = i + u * kThreads < prompt;
+          Count<C>::add(&counts[id[u] - begin], said ? Count<C>::kPrompt : 1u, said);
         }
       }
     }
-    for (int i = tid; i < p.biases; i += kThreads) {
-      const int64_t id = p.bias_ids[r * p.bias_stride + i];
-      if (id >= vocab) report_status(status, kOutOfBounds);
-      if (id < begin || id >= begin + n) continue;
-      if (atomicOr(&counts[id - begin], kBiased) & kBiased) atomicOr(&counts[id - begin], kRepeated);
-      biases[id - begin] = p.bias[r * p.bias_stride + i];
+    change.values = listed_values;
+    change.ids = listed_ids;
+    if (p.biases > 0) {
+      const int64_t* ids = p.bias_ids + r * p.bias_stride;
+      const float* values = p.bias + r * p.bias_stride;
+      if (tid >= kThreads - 32) {  // one warp lists those of the slice in their order
+        const int lane = tid & 31;
+        int at = 0;
+        for (int k = 0; k < p.biases; k += 32) {
+          const int64_t id = k + lane < p.biases ? ids[k + lane] : -1;
+          if (id >= vocab) report_status(status, kOutOfBounds);
+          const bool mine = id >= begin && id < begin + n;
+          const uint32_t votes = __ballot_sync(0xffffffffu, mine);
+          const int place = at + __popc(votes & ((1u << lane) - 1u));
+          if (mine) {
+            Count<C>::add(&counts[id - begin], Count<C>::kBiased, true);
+            if (place < kListed) listed_ids[place] = static_cast<int>(id - begin), listed_values[place] = values[k + lane];
+          }
+          at += __popc(votes);
+        }
+        if (lane == 0) listed = at;
+      }
+    }
+    change.repetition = p.repetition == nullptr ? p.repetition_ : p.repetition[r];
+    change.presence = p.presence == nullptr ? p.presence_ : p.presence[r];
+    change.frequency = p.frequency == nullptr ? p.frequency_ : p.frequency[r];
+    __syncthreads();
+    change.biases = listed;
+    if (listed > kListed) {
+      change.row_ids = p.bias_ids + r * p.bias_stride;
+      change.values = p.bias + r * p.bias_stride;
+      change.biases = p.biases;
+      change.begin = begin;
     }
   }
-  copy_masked(row, to, n, words);
-  if (!touched) return;
-  __syncthreads();  // the counts, and the copies that the touched tokens replace
-  const float repetition = p.repetition == nullptr ? 1.f : p.repetition[r];
-  const float presence = p.presence == nullptr ? 0.f : p.presence[r];
-  const float frequency = p.frequency == nullptr ? 0.f : p.frequency[r];
-  for (int i = tid; i < slice / 4; i += kThreads) {
-    const uint4 four = smem[i];
-    if ((four.x | four.y | four.z | four.w) == 0) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t c = j == 0 ? four.x : j == 1 ? four.y : j == 2 ? four.z : four.w;
-      const int v = 4 * i + j;
-      if (c == 0 || !(mask_bits(words, v, 1) & 1u)) continue;
-      float x = to_float<T>(row[v]);
-      const uint32_t times = c & kCount;
-      if (times != 0 || (c & kPrompt)) x = x > 0.f ? x / repetition : x * repetition;
-      if (times != 0) x = x - frequency * static_cast<float>(times) - presence;
-      if (c & kRepeated) {  // in the list's order
-        float sum = 0.f;
-        for (int k = 0; k < p.biases; ++k)
-          if (p.bias_ids[r * p.bias_stride + k] == begin + v) sum += p.bias[r * p.bias_stride + k];
-        x += sum;
-      } else if (c & kBiased) {
-        x += biases[v];
-      }
-      to[v] = from_float<T>(x);
+  const auto one = [&](int i) {
+    T v = mask_bits(words, i, 1) & 1u ? row[i] : from_float<T>(-INFINITY);
+    if constexpr (kTouched) {
+      if (counts[i] != 0 && (mask_bits(words, i, 1) & 1u))
+        v = from_float<T>(change.template operator()<C>(to_float<T>(v), counts[i], i));
     }
+    to[i] = v;
+  };
+  for (int i = first + tid; i < last; i += kThreads * kAhead) {
+    if (i != first + tid) fetch(i);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int at = i + u * kThreads;
+      if (at >= last) continue;
+      uint4 v = lo[u];
+      if (off != 0) v = shift_vec(lo[u], hi[u], off * static_cast<int>(sizeof(T)));
+      if constexpr (kTouched) {
+        if (bits[u] != 0) {
+          alignas(16) C c[kSize];
+          const uint4* packed = reinterpret_cast<const uint4*>(counts + cut.head + at * kSize);
+          uint32_t any = 0;
+          if constexpr (sizeof(c) == 8) {
+            *reinterpret_cast<uint2*>(c) = *reinterpret_cast<const uint2*>(packed);
+            any = reinterpret_cast<const uint2*>(c)->x | reinterpret_cast<const uint2*>(c)->y;
+          } else {
+#pragma unroll
+            for (int j = 0; j < static_cast<int>(sizeof(c) / 16); ++j) {
+              const uint4 w = packed[j];
+              reinterpret_cast<uint4*>(c)[j] = w;
+              any |= w.x | w.y | w.z | w.w;
+            }
+          }
+          if (any != 0) v = change_vec<T, C>(v, c, cut.head + at * kSize, change);
+        }
+      }
+      vecs[at] = mask_vec<T>(v, bits[u]);
+    }
+  }
+  if (tid < cut.head) one(tid);
+  if (tid >= 32 && tid < 32 + cut.tail) one(n - cut.tail + tid - 32);
+  if (off != 0 && tid < 2 * kSize && cut.vecs > 0) {  // (two vectors at most, one value a thread)
+    const int i = tid < kSize ? 0 : cut.vecs - 1;
+    const bool todo = tid < kSize ? first == 1 : last < cut.vecs && (cut.vecs > 1 || first == 0);
+    if (todo) one(cut.head + i * kSize + tid % kSize);
   }
 }
 
-// Tokens of a slice (a multiple of 32): as many as the counts' shared memory holds, fewer while there are too few
-// blocks for the SMs.
-int slice_size(int64_t rows, int64_t vocab, bool touched) {
-  int64_t slice = touched ? 16384 : 32768;
-  while (slice > 4096 && rows * ((vocab + slice - 1) / slice) < 2 * num_sms()) slice /= 2;
+// Tokens of a slice (a multiple of 32): the fewer slices, the less often a history is read; more of them while there are
+// too few blocks for the SMs.
+int slice_size(int64_t rows, int64_t vocab) {
+  int64_t slice = 16384;
+  while (slice > 1024 && rows * ((vocab + slice - 1) / slice) < 4 * num_sms()) slice /= 2;
   return static_cast<int>(slice);
 }
 
@@ -215,7 +309,8 @@ int slice_size(int64_t rows, int64_t vocab, bool touched) {
 at::Tensor process_logits(const at::Tensor& logits_in, const c10::optional<at::Tensor>& history,
                           const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& prompt_lengths,
                           const c10::optional<at::Tensor>& repetition, const c10::optional<at::Tensor>& presence,
-                          const c10::optional<at::Tensor>& frequency, const c10::optional<at::Tensor>& bias_ids,
+                          const c10::optional<at::Tensor>& frequency, double repetition_, double presence_,
+                          double frequency_, const c10::optional<at::Tensor>& bias_ids,
                           const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& allowed) {
   constexpr const char* what = "process_logits";
   check_logits(logits_in, what);
@@ -258,6 +353,9 @@ at::Tensor process_logits(const at::Tensor& logits_in, const c10::optional<at::T
     p.lengths = static_cast<const int*>(per_row(lengths, at::kInt, "lengths"));
     p.prompt_lengths = static_cast<const int*>(per_row(prompt_lengths, at::kInt, "prompt_lengths"));
   }
+  p.repetition_ = static_cast<float>(repetition_);
+  p.presence_ = static_cast<float>(presence_);
+  p.frequency_ = static_cast<float>(frequency_);
   p.repetition = static_cast<const float*>(per_row(repetition, at::kFloat, "repetition"));
   p.presence = static_cast<const float*>(per_row(presence, at::kFloat, "presence"));
   p.frequency = static_cast<const float*>(per_row(frequency, at::kFloat, "frequency"));
@@ -274,17 +372,21 @@ at::Tensor process_logits(const at::Tensor& logits_in, const c10::optional<at::T
     TDSV_CHECK(allowed->size(1) >= (vocab + 31) / 32, what, ": allowed must hold a bit per token");
     p.allowed = reinterpret_cast<const uint32_t*>(allowed->data_ptr<int>());
   }
-  const bool touched = p.history != nullptr || p.bias_ids != nullptr;
-  const int slice = slice_size(rows, vocab, touched);
+  const int slice = slice_size(rows, vocab);
   const int64_t parts = (vocab + slice - 1) / slice;
   TDSV_CHECK(rows * parts < (int64_t(1) << 31), what, ": too many rows");
-  const size_t smem = touched ? static_cast<size_t>(slice) * (p.bias_ids != nullptr ? 8 : 4) : 0;
   with_logit_type(logits.scalar_type(), [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    TDSV_CUDA_CHECK(cudaFuncSetAttribute(process_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 16384 * 8));
-    process_kernel<T><<<static_cast<unsigned>(rows * parts), kThreads, smem, stream()>>>(
-        static_cast<const T*>(logits.data_ptr()), layout, static_cast<int>(vocab), slice, static_cast<int>(parts), p,
-        static_cast<T*>(out.data_ptr()), status_word_ptr());
+    auto launch = [&](auto kern, int64_t count_bytes) {
+      const size_t smem = static_cast<size_t>((slice + kPad) * count_bytes);
+      if (smem > 32 * 1024) TDSV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+      kern<<<static_cast<unsigned>(rows * parts), kThreads, smem, stream()>>>(
+          static_cast<const T*>(logits.data_ptr()), layout, static_cast<int>(vocab), slice, static_cast<int>(parts), p,
+          static_cast<T*>(out.data_ptr()), status_word_ptr());
+    };
+    if (p.history == nullptr && p.bias_ids == nullptr) launch(process_kernel<T, void>, 0);
+    else if (p.history_size <= Count<uint16_t>::kMost) launch(process_kernel<T, uint16_t>, 2);
+    else launch(process_kernel<T, uint32_t>, 4);
   });
   TDSV_LAUNCH_CHECK();
   return out;

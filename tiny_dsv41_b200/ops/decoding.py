@@ -20,9 +20,9 @@ import math
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from ._ext import ext
-from .statistics import _differentiates
 
 HEAD_DIM = 128
 MIN_PAGE = 16
@@ -74,7 +74,10 @@ def _check_cache(keys: torch.Tensor, values: torch.Tensor, batch: PagedBatch) ->
 
 
 def _refuse_gradients(what: str, *tensors: torch.Tensor | None) -> None:
-    if _differentiates(*(t for t in tensors if t is not None and t.is_floating_point())):
+    # (forward-mode tangents exist inside a level alone; asking each tensor for one costs a microsecond)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) or (
+            forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                                   for t in tensors)):
         raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad() or with detached tensors")
 
 
@@ -148,7 +151,7 @@ def _attention_reference(q, keys, values, batch, scale, tree):
 def _process_reference(x, history, lengths, prompt_lengths, repetition, presence, frequency, bias_ids, bias, allowed):
     rows, vocab = x.shape
     dtype, x = x.dtype, x.to(torch.promote_types(x.dtype, torch.float32), copy=True)
-    column = lambda v: 0.0 if v is None else v.to(x.dtype).unsqueeze(1)  # noqa: E731
+    column = lambda v: v.to(x.dtype).unsqueeze(1)  # noqa: E731
     if history is not None:
         place = torch.arange(history.shape[1]).expand(rows, -1)
         known = history >= 0
@@ -162,9 +165,8 @@ def _process_reference(x, history, lengths, prompt_lengths, repetition, presence
         at = torch.where(known, history, 0).long()
         said = torch.zeros(rows, vocab, dtype=torch.int64).scatter_add_(1, at, known.long()) > 0
         times = torch.zeros(rows, vocab, dtype=torch.int64).scatter_add_(1, at, output.long())
-        if repetition is not None:
-            r = column(repetition)
-            x = torch.where(said, torch.where(x > 0, x / r, x * r), x)
+        r = column(repetition)
+        x = torch.where(said, torch.where(x > 0, x / r, x * r), x)
         x = torch.where(times > 0, x - column(frequency) * times - column(presence), x)
     if bias_ids is not None:
         if bool((bias_ids >= vocab).any()):
@@ -288,18 +290,20 @@ def tree_mask(parents: torch.Tensor, starts: torch.Tensor, words: int | None = N
     return torch.tensor(signed, dtype=torch.int32, device=parents.device).view(len(given), words)
 
 
-def _per_row(value, name: str, logits: torch.Tensor, positive: bool = False) -> torch.Tensor | None:
-    """fp32 values, one per row, of a number or a tensor."""
+def _per_row(value, name: str, logits: torch.Tensor, default: float) -> tuple[torch.Tensor | None, float]:
+    """A penalty as fp32 values, one per row, or as a number for all rows."""
     if value is None:
-        return None
+        return None, default
     if isinstance(value, torch.Tensor):
         if value.shape != logits.shape[:-1] or value.device != logits.device or not value.is_floating_point():
             raise ValueError(f"{name} must be a number, or hold one per row on the logits' device")
-        return value.detach().float().reshape(-1).contiguous()
+        if value.dtype != torch.float32 or value.ndim != 1 or not value.is_contiguous():
+            value = value.detach().float().reshape(-1).contiguous()
+        return value, default
     value = float(value)
-    if not math.isfinite(value) or (positive and value <= 0):
-        raise ValueError(f"{name} must be finite" + (" and positive" if positive else ""))
-    return torch.full((logits.shape[:-1].numel(),), value, dtype=torch.float32, device=logits.device)
+    if not math.isfinite(value) or (name == "repetition" and value <= 0):
+        raise ValueError(f"{name} must be finite" + (" and positive" if name == "repetition" else ""))
+    return None, value
 
 
 def _rows_of(value: torch.Tensor, name: str, types, logits: torch.Tensor) -> torch.Tensor:
@@ -309,6 +313,8 @@ def _rows_of(value: torch.Tensor, name: str, types, logits: torch.Tensor) -> tor
     if value.device != logits.device:
         raise ValueError(f"{name} must be on the logits' device")
     lead = logits.shape[:-1]
+    if len(lead) == 1 and value.ndim == 2 and value.shape[0] == lead[0] and value.is_contiguous():
+        return value
     try:
         value = value.expand(*lead, value.shape[-1])
     except (RuntimeError, IndexError):
@@ -355,12 +361,14 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, *,
                 raise TypeError(f"{name} must be int32")
             if value is not None and (value.shape != lead or value.device != logits.device):
                 raise ValueError(f"{name} must hold one value per row on the logits' device")
-        lengths, prompt_lengths = (None if v is None else v.reshape(-1).contiguous() for v in (lengths, prompt_lengths))
-    repetition = _per_row(repetition, "repetition", logits, positive=True)
-    presence, frequency = _per_row(presence, "presence", logits), _per_row(frequency, "frequency", logits)
+        lengths, prompt_lengths = (v if v is None or v.ndim == 1 and v.is_contiguous() else v.reshape(-1).contiguous()
+                                   for v in (lengths, prompt_lengths))
+    repetition, all_repetition = _per_row(repetition, "repetition", logits, 1.0)
+    presence, all_presence = _per_row(presence, "presence", logits, 0.0)
+    frequency, all_frequency = _per_row(frequency, "frequency", logits, 0.0)
     if bias is not None:
         bias_ids = _rows_of(bias_ids, "bias_ids", (torch.int64,), logits)
-        bias = _rows_of(bias.detach(), "bias", (torch.float32,), logits)
+        bias = _rows_of(bias, "bias", (torch.float32,), logits)
         if bias.shape != bias_ids.shape:
             raise ValueError("bias and bias_ids must be alike")
         if bias.stride() != bias_ids.stride():
@@ -370,10 +378,12 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, *,
             raise ValueError("allowed must hold a bit per token")
         allowed = _rows_of(allowed, "allowed", (torch.int32,), logits)
     if not logits.is_cuda:
-        return _process_reference(logits.reshape(-1, vocab), history, lengths, prompt_lengths, repetition, presence,
-                                  frequency, bias_ids, bias, allowed).view(logits.shape)
-    return ext().process_logits(logits.detach(), history, lengths, prompt_lengths, repetition, presence, frequency,
-                                bias_ids, bias, allowed)
+        full = lambda v, number: torch.full((lead.numel(),), number, dtype=torch.float64) if v is None else v  # noqa: E731
+        return _process_reference(logits.reshape(-1, vocab), history, lengths, prompt_lengths,
+                                  full(repetition, all_repetition), full(presence, all_presence),
+                                  full(frequency, all_frequency), bias_ids, bias, allowed).view(logits.shape)
+    return ext().process_logits(logits, history, lengths, prompt_lengths, repetition, presence, frequency, all_repetition,
+                                all_presence, all_frequency, bias_ids, bias, allowed)
 
 
 __all__ = ["PagedBatch", "paged_append", "paged_attention", "process_logits", "tree_mask"]
