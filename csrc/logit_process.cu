@@ -10,9 +10,11 @@
 // in fp32, rounded once to the logits' type.
 //
 // A row is cut into slices of the vocabulary, a block each. A block counts the history's tokens of its slice in
-// shared memory (whole numbers: the order of the atomics changes nothing) and then streams the slice in 16-byte vectors,
-// read once: a vector without a count, and most are, is only masked and never passes through fp32. A vector that the
-// mask hides altogether is not read.
+// shared memory (whole numbers: the order of the atomics changes nothing), and whoever counts a token first puts it on a
+// list. Then it copies the slice under the mask in 16-byte vectors, which never pass through fp32; a vector that the mask
+// hides altogether is not read. Last the tokens on the list, few and evenly spread over the threads, are written anew.
+// (Applied to the vectors on their way, the penalties cost 224 us in place of 112 at 512 x 151669: frequent tokens are
+// neighbours, and the few warps that hold them work off eight tokens a thread, one after another.)
 #include "logit_rows.cuh"
 
 namespace tdsv {
@@ -20,8 +22,8 @@ namespace tdsv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 4;          // vectors a thread has in flight
-constexpr int kPad = 16;           // counts beyond a slice's, for their alignment
+constexpr int kAhead = 4;          // vectors or touched tokens a thread has in flight
+constexpr int kIds = 8;            // ids of the history
 constexpr int kListed = 1024;      // biases of a slice that shared memory holds
 
 // A token's count and two flags. 16 bits hold the counts of histories below 2^14 tokens, in half the shared memory, so
@@ -30,12 +32,13 @@ template <typename C>
 struct Count {
   static constexpr uint32_t kPrompt = sizeof(C) == 2 ? 0x8000u : 0x80000000u, kBiased = kPrompt >> 1, kTimes = kBiased - 1;
   static constexpr int kMost = static_cast<int>(sizeof(C) == 2 ? kTimes : kTimes >> 1);
-  static __device__ __forceinline__ void add(C* at, uint32_t what, bool flag) {
-    const uintptr_t p = reinterpret_cast<uintptr_t>(at);
-    if (sizeof(C) == 2) what <<= (p & 2) * 8;
-    uint32_t* word = reinterpret_cast<uint32_t*>(p & ~uintptr_t(3));
-    if (flag) atomicOr(word, what);
-    else atomicAdd(word, what);
+  // Whether it is the first that is heard of the token.
+  static __device__ __forceinline__ bool add(uint32_t* words, int token, uint32_t what, bool flag) {
+    constexpr int kEach = 4 / sizeof(C);
+    const int shift = token % kEach * 16;
+    uint32_t* word = words + token / kEach;
+    const uint32_t was = flag ? atomicOr(word, what << shift) : atomicAdd(word, what << shift);
+    return (was >> shift & (kPrompt | (kPrompt - 1u))) == 0;
   }
 };
 
@@ -71,6 +74,53 @@ __device__ __forceinline__ uint32_t mask_bits(const uint32_t* words, int at, int
   uint32_t bits = words[at >> 5] >> shift;
   if (shift + count > 32) bits |= words[(at >> 5) + 1] << (32 - shift);
   return bits;
+}
+
+// out[0, n) = row[0, n) where the mask allows it. Vectors are aligned at `out`; where the logits lie at another
+// offset in their 16 bytes, two of theirs are joined.
+template <typename T>
+__device__ __forceinline__ void copy_masked(const T* row, T* out, int n, const uint32_t* words) {
+  constexpr int kSize = LogitVec<T>::kSize;
+  constexpr uint32_t kAll = (1u << kSize) - 1;
+  const RowCut cut = cut_row(out, n);
+  const int tid = threadIdx.x;
+  const auto one = [&](int i) { out[i] = mask_bits(words, i, 1) & 1u ? row[i] : from_float<T>(-INFINITY); };
+  if (tid < cut.head) one(tid);
+  if (tid >= 32 && tid < 32 + cut.tail) one(n - cut.tail + tid - 32);
+  const T* from = row + cut.head;
+  uint4* to = reinterpret_cast<uint4*>(out + cut.head);
+  const int off = static_cast<int>((reinterpret_cast<uintptr_t>(from) & 15) / sizeof(T));
+  // the vectors whose parts all lie inside the row: with an offset, at most the first and the last do not
+  const uint4* x = reinterpret_cast<const uint4*>(from - off);
+  const int first = off > cut.head ? 1 : 0;
+  const int last = off == 0 ? cut.vecs : min(cut.vecs, (n - cut.head + off) / kSize - 1);
+  for (int i = first + tid; i < last; i += kThreads * kAhead) {
+    uint4 lo[kAhead], hi[kAhead];
+    uint32_t bits[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int at = i + u * kThreads;
+      bits[u] = at < last ? mask_bits(words, cut.head + at * kSize, kSize) & kAll : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (bits[u] == 0) continue;
+      lo[u] = load_stream(x + i + u * kThreads);
+      if (off != 0) hi[u] = load_stream(x + i + u * kThreads + 1);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (i + u * kThreads >= last) continue;
+      uint4 v = lo[u];
+      if (off != 0) v = shift_vec(lo[u], hi[u], off * static_cast<int>(sizeof(T)));
+      to[i + u * kThreads] = mask_vec<T>(v, bits[u]);
+    }
+  }
+  if (off != 0 && tid < 2 * kSize && cut.vecs > 0) {  // (two vectors at most, one value a thread)
+    const int i = tid < kSize ? 0 : cut.vecs - 1;
+    const bool todo = tid < kSize ? first == 1 : last < cut.vecs && (cut.vecs > 1 || first == 0);
+    if (todo) one(cut.head + i * kSize + tid % kSize);
+  }
 }
 
 struct Penalties {
@@ -115,78 +165,35 @@ struct Change {
   }
 };
 
+// C: the counts' type; void where no token is touched. Dynamic shared memory: counts [slice], list [room].
 template <typename T, typename C>
-__device__ __forceinline__ uint4 change_vec(const uint4& v, const C* counts, int at, const Change& change) {
-  uint32_t out[4];
-#pragma unroll
-  for (int i = 0; i < LogitVec<T>::kPairs; ++i) {
-    float2 f = unpack_pair<T>(v, i);
-    if (counts[2 * i] != 0) f.x = change.template operator()<C>(f.x, counts[2 * i], at + 2 * i);
-    if (counts[2 * i + 1] != 0) f.y = change.template operator()<C>(f.y, counts[2 * i + 1], at + 2 * i + 1);
-    if constexpr (sizeof(T) == 2) {
-      out[i] = pack_pair<T>(f.x, f.y);  // (an untouched value is one of the type, and stays)
-    } else {
-      out[2 * i] = __float_as_uint(f.x);
-      out[2 * i + 1] = __float_as_uint(f.y);
-    }
-  }
-  return make_uint4(out[0], out[1], out[2], out[3]);
-}
-
-// C: the counts' type; void where no token is touched. Dynamic shared memory: counts [slice + kPad].
-template <typename T, typename C>
-__global__ void __launch_bounds__(kThreads, std::is_void_v<C> ? 4 : 3)
+__global__ void __launch_bounds__(kThreads, 4)
     process_kernel(const T* __restrict__ logits, RowLayout layout, int vocab, int slice, int parts,
                    const __grid_constant__ Penalties p, T* __restrict__ out, int* __restrict__ status) {
   constexpr bool kTouched = !std::is_void_v<C>;
   using Word = std::conditional_t<kTouched, C, uint16_t>;
-  constexpr int kSize = LogitVec<T>::kSize;
-  constexpr uint32_t kAll = (1u << kSize) - 1;
   extern __shared__ uint4 smem[];
-  __shared__ int listed_ids[kTouched ? kListed : 1];
-  __shared__ float listed_values[kTouched ? kListed : 1];
-  __shared__ int listed;
   const uint32_t r = blockIdx.x / parts;
   const int begin = static_cast<int>(blockIdx.x - r * parts) * slice, n = min(slice, vocab - begin);
   const int tid = threadIdx.x;
   const T* row = logits + layout.offset(r) + begin;
   T* to = out + static_cast<int64_t>(r) * vocab + begin;
   const uint32_t* words = p.allowed == nullptr ? nullptr : p.allowed + r * p.allowed_stride + begin / 32;
-  // Vectors are aligned at `out`; where the logits lie at another offset in their 16 bytes, two of theirs are joined. The
-  // vectors whose parts all lie inside the row are [first, last): with an offset, at most two do not.
-  const RowCut cut = cut_row(to, n);
-  const T* from = row + cut.head;
-  uint4* vecs = reinterpret_cast<uint4*>(to + cut.head);
-  const int off = static_cast<int>((reinterpret_cast<uintptr_t>(from) & 15) / sizeof(T));
-  const uint4* x = reinterpret_cast<const uint4*>(from - off);
-  const int first = off > cut.head ? 1 : 0;
-  const int last = off == 0 ? cut.vecs : min(cut.vecs, (n - cut.head + off) / kSize - 1);
-  // token v of the slice is counted at counts[v]: a vector's counts are aligned as it is
-  Word* counts = reinterpret_cast<Word*>(smem) + (kSize - cut.head) % kSize;
-
-  uint4 lo[kAhead], hi[kAhead];
-  uint32_t bits[kAhead];
-  const auto fetch = [&](int i) {
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int at = i + u * kThreads;
-      bits[u] = at < last ? mask_bits(words, cut.head + at * kSize, kSize) & kAll : 0u;
-    }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (bits[u] == 0) continue;
-      lo[u] = load_stream(x + i + u * kThreads);
-      if (off != 0) hi[u] = load_stream(x + i + u * kThreads + 1);
-    }
-  };
-  fetch(first + tid);  // on their way while the history is counted
-
-  Change change{};
-  if constexpr (kTouched) {
-    const int all = static_cast<int>((slice + kPad) * sizeof(C) / 16);
-    for (int i = tid; i < all; i += kThreads) smem[i] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) listed = 0;
+  if constexpr (!kTouched) {
+    copy_masked(row, to, n, words);
+  } else {
+    __shared__ int listed_ids[kListed];
+    __shared__ float listed_values[kListed];
+    __shared__ int listed, touched;
+    uint32_t* counts = reinterpret_cast<uint32_t*>(smem);
+    uint16_t* list = reinterpret_cast<uint16_t*>(reinterpret_cast<Word*>(smem) + slice);
+    for (int i = tid; i < static_cast<int>(slice * sizeof(Word) / 16); i += kThreads) smem[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) listed = 0, touched = 0;
     __syncthreads();
+    const auto count = [&](int64_t id, uint32_t what, bool flag) {
+      const int v = static_cast<int>(id - begin);
+      if (Count<Word>::add(counts, v, what, flag)) list[atomicAdd(&touched, 1)] = static_cast<uint16_t>(v);
+    };
     if (p.history != nullptr) {
       int length = p.history_size;
       if (p.lengths != nullptr) {
@@ -197,49 +204,49 @@ __global__ void __launch_bounds__(kThreads, std::is_void_v<C> ? 4 : 3)
       const int prompt = p.prompt_lengths == nullptr ? 0 : p.prompt_lengths[r];
       const int64_t* wide = static_cast<const int64_t*>(p.history) + r * p.history_stride;
       const int* narrow = static_cast<const int*>(p.history) + r * p.history_stride;
-      for (int i = tid; i < length; i += kThreads * kAhead) {
-        int64_t id[kAhead];
+      for (int i = tid; i < length; i += kThreads * kIds) {
+        int64_t id[kIds];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
+        for (int u = 0; u < kIds; ++u) {
           const int at = i + u * kThreads;
           id[u] = at >= length ? -1 : p.wide ? wide[at] : narrow[at];
         }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
+        for (int u = 0; u < kIds; ++u) {
           if (id[u] >= vocab) report_status(status, kOutOfBounds);
           if (id[u] < begin || id[u] >= begin + n) continue;
           const bool said = i + u * kThreads < prompt;
-          Count<C>::add(&counts[id[u] - begin], said ? Count<C>::kPrompt : 1u, said);
+          count(id[u], said ? Count<Word>::kPrompt : 1u, said);
         }
       }
     }
-    change.values = listed_values;
-    change.ids = listed_ids;
-    if (p.biases > 0) {
+    if (p.biases > 0 && tid >= kThreads - 32) {  // one warp lists those of the slice in their order
       const int64_t* ids = p.bias_ids + r * p.bias_stride;
       const float* values = p.bias + r * p.bias_stride;
-      if (tid >= kThreads - 32) {  // one warp lists those of the slice in their order
-        const int lane = tid & 31;
-        int at = 0;
-        for (int k = 0; k < p.biases; k += 32) {
-          const int64_t id = k + lane < p.biases ? ids[k + lane] : -1;
-          if (id >= vocab) report_status(status, kOutOfBounds);
-          const bool mine = id >= begin && id < begin + n;
-          const uint32_t votes = __ballot_sync(0xffffffffu, mine);
-          const int place = at + __popc(votes & ((1u << lane) - 1u));
-          if (mine) {
-            Count<C>::add(&counts[id - begin], Count<C>::kBiased, true);
-            if (place < kListed) listed_ids[place] = static_cast<int>(id - begin), listed_values[place] = values[k + lane];
-          }
-          at += __popc(votes);
+      const int lane = tid & 31;
+      int at = 0;
+      for (int k = 0; k < p.biases; k += 32) {
+        const int64_t id = k + lane < p.biases ? ids[k + lane] : -1;
+        if (id >= vocab) report_status(status, kOutOfBounds);
+        const bool mine = id >= begin && id < begin + n;
+        const uint32_t votes = __ballot_sync(0xffffffffu, mine);
+        const int place = at + __popc(votes & ((1u << lane) - 1u));
+        if (mine) {
+          count(id, Count<Word>::kBiased, true);
+          if (place < kListed) listed_ids[place] = static_cast<int>(id - begin), listed_values[place] = values[k + lane];
         }
-        if (lane == 0) listed = at;
+        at += __popc(votes);
       }
+      if (lane == 0) listed = at;
     }
+    copy_masked(row, to, n, words);
+    Change change{};
     change.repetition = p.repetition == nullptr ? p.repetition_ : p.repetition[r];
     change.presence = p.presence == nullptr ? p.presence_ : p.presence[r];
     change.frequency = p.frequency == nullptr ? p.frequency_ : p.frequency[r];
-    __syncthreads();
+    __syncthreads();  // the list and the counts, and the copies that it replaces
+    change.ids = listed_ids;
+    change.values = listed_values;
     change.biases = listed;
     if (listed > kListed) {
       change.row_ids = p.bias_ids + r * p.bias_stride;
@@ -247,51 +254,21 @@ __global__ void __launch_bounds__(kThreads, std::is_void_v<C> ? 4 : 3)
       change.biases = p.biases;
       change.begin = begin;
     }
-  }
-  const auto one = [&](int i) {
-    T v = mask_bits(words, i, 1) & 1u ? row[i] : from_float<T>(-INFINITY);
-    if constexpr (kTouched) {
-      if (counts[i] != 0 && (mask_bits(words, i, 1) & 1u))
-        v = from_float<T>(change.template operator()<C>(to_float<T>(v), counts[i], i));
-    }
-    to[i] = v;
-  };
-  for (int i = first + tid; i < last; i += kThreads * kAhead) {
-    if (i != first + tid) fetch(i);
+    const Word* count_of = reinterpret_cast<const Word*>(smem);
+    for (int i = tid; i < touched; i += kThreads * kAhead) {
+      int v[kAhead];
+      float x[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int at = i + u * kThreads;
-      if (at >= last) continue;
-      uint4 v = lo[u];
-      if (off != 0) v = shift_vec(lo[u], hi[u], off * static_cast<int>(sizeof(T)));
-      if constexpr (kTouched) {
-        if (bits[u] != 0) {
-          alignas(16) C c[kSize];
-          const uint4* packed = reinterpret_cast<const uint4*>(counts + cut.head + at * kSize);
-          uint32_t any = 0;
-          if constexpr (sizeof(c) == 8) {
-            *reinterpret_cast<uint2*>(c) = *reinterpret_cast<const uint2*>(packed);
-            any = reinterpret_cast<const uint2*>(c)->x | reinterpret_cast<const uint2*>(c)->y;
-          } else {
-#pragma unroll
-            for (int j = 0; j < static_cast<int>(sizeof(c) / 16); ++j) {
-              const uint4 w = packed[j];
-              reinterpret_cast<uint4*>(c)[j] = w;
-              any |= w.x | w.y | w.z | w.w;
-            }
-          }
-          if (any != 0) v = change_vec<T, C>(v, c, cut.head + at * kSize, change);
-        }
+      for (int u = 0; u < kAhead; ++u) {
+        const int at = i + u * kThreads;
+        v[u] = at < touched ? list[at] : -1;
+        if (v[u] >= 0 && !(mask_bits(words, v[u], 1) & 1u)) v[u] = -1;
+        if (v[u] >= 0) x[u] = to_float<T>(row[v[u]]);
       }
-      vecs[at] = mask_vec<T>(v, bits[u]);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (v[u] >= 0) to[v[u]] = from_float<T>(change.template operator()<Word>(x[u], count_of[v[u]], v[u]));
     }
-  }
-  if (tid < cut.head) one(tid);
-  if (tid >= 32 && tid < 32 + cut.tail) one(n - cut.tail + tid - 32);
-  if (off != 0 && tid < 2 * kSize && cut.vecs > 0) {  // (two vectors at most, one value a thread)
-    const int i = tid < kSize ? 0 : cut.vecs - 1;
-    const bool todo = tid < kSize ? first == 1 : last < cut.vecs && (cut.vecs > 1 || first == 0);
-    if (todo) one(cut.head + i * kSize + tid % kSize);
   }
 }
 
@@ -377,8 +354,10 @@ at::Tensor process_logits(const at::Tensor& logits_in, const c10::optional<at::T
   TDSV_CHECK(rows * parts < (int64_t(1) << 31), what, ": too many rows");
   with_logit_type(logits.scalar_type(), [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
+    // a block's list holds each of its tokens once
+    const int64_t room = std::min<int64_t>(slice, static_cast<int64_t>(p.history_size) + p.biases);
     auto launch = [&](auto kern, int64_t count_bytes) {
-      const size_t smem = static_cast<size_t>((slice + kPad) * count_bytes);
+      const size_t smem = static_cast<size_t>(slice * count_bytes + (count_bytes != 0 ? 2 * room : 0));
       if (smem > 32 * 1024) TDSV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
       kern<<<static_cast<unsigned>(rows * parts), kThreads, smem, stream()>>>(
           static_cast<const T*>(logits.data_ptr()), layout, static_cast<int>(vocab), slice, static_cast<int>(parts), p,

@@ -14,26 +14,40 @@ namespace tdsv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGroups = kThreads / 16;  // 16 lanes take one head
+constexpr int kLanes = 8;                   // of a head
+constexpr int kGroups = kThreads / kLanes;  // heads at work
 constexpr int kHalf = kHeadDim / 2;
 
+// 16 bytes of a row.
 template <typename T>
-struct alignas(8) Four {
-  T v[4];
+struct alignas(16) Eight {
+  T v[8];
 };
 
-// Lane l of 16 has dims [4 l, 4 l + 4) and their partners 64 further: a rotation needs no other lane.
+// Lane l of 8 has dims [8 l, 8 l + 8) and their partners 64 further: a rotation needs no other lane. The values of a
+// block's next heads are on their way while the angles are taken and the heads before them are worked on.
 template <typename T, int TOKENS>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(
     const T* __restrict__ qkv, int64_t qkv_stride, const T* __restrict__ wq, const T* __restrict__ wk,
     const int64_t* __restrict__ positions, const float* __restrict__ freqs, T* __restrict__ q_out, T* __restrict__ keys,
     T* __restrict__ values, PoolStrides ks, PoolStrides vs, PagedBatch batch, int hq, float eps, int* __restrict__ status) {
-  __shared__ float cosines[TOKENS][kHalf], sines[TOKENS][kHalf];
+  __shared__ alignas(16) float cosines[TOKENS][kHalf], sines[TOKENS][kHalf];
+  __shared__ alignas(16) float weights[2][kHeadDim];
   __shared__ int page_of[TOKENS], row_of[TOKENS];  // page -1: the token is not stored
-  const int tid = threadIdx.x, lane = tid & 15, group = tid >> 4;
+  const int tid = threadIdx.x, lane = tid % kLanes, group = tid / kLanes;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * TOKENS;
   const int here = static_cast<int>(min(static_cast<int64_t>(TOKENS), batch.rows - first));
-  const int hkv = batch.kv_heads, heads = hq + 2 * hkv;
+  const int hkv = batch.kv_heads, heads = hq + 2 * hkv, items = here * heads;
+  const T* mine = qkv + first * qkv_stride + 8 * lane;
+
+  int t = group / heads, h = group - t * heads;  // token and head of item `group`
+  Eight<T> lo, hi;
+  const auto fetch = [&] {
+    const T* from = mine + t * qkv_stride + static_cast<int64_t>(h) * kHeadDim;
+    lo = *reinterpret_cast<const Eight<T>*>(from);
+    hi = *reinterpret_cast<const Eight<T>*>(from + kHalf);
+  };
+  if (group < items) fetch();
 
   for (int i = tid; i < here * kHalf; i += kThreads) {
     // turns of the circle, whole ones dropped
@@ -42,8 +56,9 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(
     turn -= rint(turn);
     sincospif(2.f * static_cast<float>(turn), &sines[i / kHalf][i % kHalf], &cosines[i / kHalf][i % kHalf]);
   }
-  for (int t = tid >> 5; t < here; t += kThreads / 32) {
-    const int row = static_cast<int>(first) + t;
+  weights[tid / kHeadDim][tid % kHeadDim] = to_float<T>((tid < kHeadDim ? wq : wk)[tid % kHeadDim]);
+  for (int x = tid >> 5; x < here; x += kThreads / 32) {
+    const int row = static_cast<int>(first) + x;
     const int b = paged_find(batch, row);
     int page = -1, at = 0;
     if (b < batch.seqs) {
@@ -58,56 +73,48 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(
         }
       }
     }
-    if ((tid & 31) == 0) page_of[t] = page, row_of[t] = at;
-  }
-  float w[2][8];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const T* from = i == 0 ? wq : wk;
-    const Four<T> lo = *reinterpret_cast<const Four<T>*>(from + 4 * lane);
-    const Four<T> hi = *reinterpret_cast<const Four<T>*>(from + kHalf + 4 * lane);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[i][j] = to_float<T>(lo.v[j]), w[i][4 + j] = to_float<T>(hi.v[j]);
+    if ((tid & 31) == 0) page_of[x] = page, row_of[x] = at;
   }
   __syncthreads();
 
-  const int items = here * heads;
   for (int base = 0; base < items; base += kGroups) {  // (the same number of turns for all: they shuffle)
-    const int item = base + group;
-    const bool some = item < items;
-    const int t = some ? item / heads : 0, h = some ? item - t * heads : 0;
-    const T* from = qkv + (first + t) * qkv_stride + static_cast<int64_t>(h) * kHeadDim + 4 * lane;
-    Four<T> lo = *reinterpret_cast<const Four<T>*>(from), hi = *reinterpret_cast<const Four<T>*>(from + kHalf);
-    const bool plain = h >= hq + hkv, is_q = h < hq;
-    float x[8], sum = 0.f;
+    const bool some = base + group < items;
+    const int token = t, head = h;
+    float x[16], sum = 0.f;
+    Eight<T> a = lo, b = hi;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = to_float<T>(lo.v[j]), x[4 + j] = to_float<T>(hi.v[j]);
+    for (int j = 0; j < 8; ++j) x[j] = some ? to_float<T>(a.v[j]) : 0.f, x[8 + j] = some ? to_float<T>(b.v[j]) : 0.f;
+    h += kGroups;
+    while (h >= heads) h -= heads, ++t;
+    if (base + kGroups + group < items) fetch();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum += x[j] * x[j];
+    for (int j = 0; j < 16; ++j) sum += x[j] * x[j];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (!some) continue;
+    const bool plain = head >= hq + hkv, is_q = head < hq;
     T* to;
     if (is_q) {
-      to = q_out + ((first + t) * hq + h) * kHeadDim;
+      to = q_out + ((first + token) * hq + head) * kHeadDim;
     } else {
-      const int page = page_of[t];
+      const int page = page_of[token];
       if (page < 0) continue;
       const PoolStrides& s = plain ? vs : ks;
-      to = (plain ? values : keys) + page * s.page + (plain ? h - hq - hkv : h - hq) * s.head + row_of[t] * s.row;
+      to = (plain ? values : keys) + page * s.page + (plain ? head - hq - hkv : head - hq) * s.head + row_of[token] * s.row;
     }
     if (!plain) {
       const float r = 1.f / sqrtf(sum * (1.f / kHeadDim) + eps);
+      const float* w = weights[is_q ? 0 : 1] + 8 * lane;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float c = cosines[t][4 * lane + j], s = sines[t][4 * lane + j];
-        const float a = x[j] * r * (is_q ? w[0][j] : w[1][j]), b = x[4 + j] * r * (is_q ? w[0][4 + j] : w[1][4 + j]);
-        lo.v[j] = from_float<T>(a * c - b * s);
-        hi.v[j] = from_float<T>(b * c + a * s);
+      for (int j = 0; j < 8; ++j) {
+        const float c = cosines[token][8 * lane + j], s = sines[token][8 * lane + j];
+        const float u = x[j] * r * w[j], v = x[8 + j] * r * w[kHalf + j];
+        a.v[j] = from_float<T>(u * c - v * s);
+        b.v[j] = from_float<T>(v * c + u * s);
       }
     }
-    *reinterpret_cast<Four<T>*>(to + 4 * lane) = lo;
-    *reinterpret_cast<Four<T>*>(to + kHalf + 4 * lane) = hi;
+    *reinterpret_cast<Eight<T>*>(to + 8 * lane) = a;
+    *reinterpret_cast<Eight<T>*>(to + kHalf + 8 * lane) = b;
   }
 }
 
@@ -175,13 +182,12 @@ at::Tensor paged_append(const at::Tensor& qkv, const at::Tensor& wq, const at::T
   const PagedBatch batch = paged_batch(keys, values, tables, starts, lengths, rows, what);
   TDSV_CHECK(hq >= 1 && qkv.size(1) == (hq + 2 * batch.kv_heads) * kHeadDim && qkv.scalar_type() == keys.scalar_type(), what,
              ": qkv must hold hq + 2 hkv heads in the cache's type");
-  TDSV_CHECK(qkv.stride(1) == 1 && (rows <= 1 || qkv.stride(0) % 4 == 0) &&
-                 reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 8 == 0,
-             what, ": qkv's rows must be dense and 8-byte aligned");
+  TDSV_CHECK(qkv.stride(1) == 1 && (rows <= 1 || qkv.stride(0) % 8 == 0) &&
+                 reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
+             what, ": qkv's rows must be dense and 16-byte aligned");
   for (const at::Tensor& w : {wq, wk}) {
     check_cuda_tensor(w, "norm weight");
-    TDSV_CHECK(w.device() == qkv.device() && w.scalar_type() == qkv.scalar_type() && w.numel() == kHeadDim &&
-                   reinterpret_cast<uintptr_t>(w.data_ptr()) % 8 == 0,
+    TDSV_CHECK(w.device() == qkv.device() && w.scalar_type() == qkv.scalar_type() && w.numel() == kHeadDim,
                what, ": norm weights must be 128 values of qkv's type");
   }
   check_cuda_tensor(positions, "positions");

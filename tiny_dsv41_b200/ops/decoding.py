@@ -213,9 +213,9 @@ def paged_append(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, position
     positions = positions.reshape(-1)
     if not keys.is_cuda:
         return _append_reference(flat, wq, wk, positions, freqs, hq, hkv, eps, keys, values, batch)
-    if flat.stride(1) != 1 or flat.stride(0) % 4 or flat.data_ptr() % 8:
-        flat = _dense(flat, 8)
-    return ext().paged_append(flat, _dense(wq, 8), _dense(wk, 8), positions.contiguous(), freqs.contiguous(), hq,
+    if flat.stride(1) != 1 or flat.stride(0) % 8 or flat.data_ptr() % 16:
+        flat = _dense(flat, 16)
+    return ext().paged_append(flat, wq.contiguous(), wk.contiguous(), positions.contiguous(), freqs.contiguous(), hq,
                               float(eps), keys, values, *_batch_tensors(batch))
 
 
