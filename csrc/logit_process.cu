@@ -165,6 +165,19 @@ struct Change {
   }
 };
 
+// The slice's logits towards L2, which a block asks for before it counts: by one warp, unless a sample of the mask's words
+// says that most of them stay unread.
+template <typename T>
+__device__ __forceinline__ void prefetch_slice(const T* row, int n, const uint32_t* words) {
+  const int lane = threadIdx.x & 31;
+  const bool open = words == nullptr || words[(n / 32) * lane / 32] != 0;
+  if (__popc(__ballot_sync(0xffffffffu, open)) < 8 || lane != 0) return;
+  const uintptr_t start = (reinterpret_cast<uintptr_t>(row) + 15) & ~uintptr_t(15);
+  const uintptr_t end = reinterpret_cast<uintptr_t>(row + n) & ~uintptr_t(15);
+  if (start < end)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(start), "r"(static_cast<uint32_t>(end - start)) : "memory");
+}
+
 // C: the counts' type; void where no token is touched. Dynamic shared memory: counts [slice], list [room].
 template <typename T, typename C>
 __global__ void __launch_bounds__(kThreads, 4)
@@ -185,6 +198,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     __shared__ int listed_ids[kListed];
     __shared__ float listed_values[kListed];
     __shared__ int listed, touched;
+    if (tid < 32) prefetch_slice(row, n, words);
     uint32_t* counts = reinterpret_cast<uint32_t*>(smem);
     uint16_t* list = reinterpret_cast<uint16_t*>(reinterpret_cast<Word*>(smem) + slice);
     for (int i = tid; i < static_cast<int>(slice * sizeof(Word) / 16); i += kThreads) smem[i] = make_uint4(0, 0, 0, 0);

@@ -7,6 +7,7 @@
 //
 // All in fp32, rounded once when stored. The angle is reduced in 64 bits before its sine is taken: fp32 leaves
 // 0.002 of position 40000 times a frequency of 1, half a step of bf16.
+#include "logit_rows.cuh"
 #include "paged.cuh"
 
 namespace tdsv {
@@ -18,16 +19,10 @@ constexpr int kLanes = 8;                   // of a head
 constexpr int kGroups = kThreads / kLanes;  // heads at work
 constexpr int kHalf = kHeadDim / 2;
 
-// 16 bytes of a row.
-template <typename T>
-struct alignas(16) Eight {
-  T v[8];
-};
-
 // Lane l of 8 has dims [8 l, 8 l + 8) and their partners 64 further: a rotation needs no other lane. The values of a
 // block's next heads are on their way while the angles are taken and the heads before them are worked on.
 template <typename T, int TOKENS>
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(
+__global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(
     const T* __restrict__ qkv, int64_t qkv_stride, const T* __restrict__ wq, const T* __restrict__ wk,
     const int64_t* __restrict__ positions, const float* __restrict__ freqs, T* __restrict__ q_out, T* __restrict__ keys,
     T* __restrict__ values, PoolStrides ks, PoolStrides vs, PagedBatch batch, int hq, float eps, int* __restrict__ status) {
@@ -41,11 +36,11 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(
   const T* mine = qkv + first * qkv_stride + 8 * lane;
 
   int t = group / heads, h = group - t * heads;  // token and head of item `group`
-  Eight<T> lo, hi;
+  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
   const auto fetch = [&] {
     const T* from = mine + t * qkv_stride + static_cast<int64_t>(h) * kHeadDim;
-    lo = *reinterpret_cast<const Eight<T>*>(from);
-    hi = *reinterpret_cast<const Eight<T>*>(from + kHalf);
+    lo = load_stream(from);
+    hi = load_stream(from + kHalf);
   };
   if (group < items) fetch();
 
@@ -80,15 +75,18 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(
   for (int base = 0; base < items; base += kGroups) {  // (the same number of turns for all: they shuffle)
     const bool some = base + group < items;
     const int token = t, head = h;
-    float x[16], sum = 0.f;
-    Eight<T> a = lo, b = hi;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = some ? to_float<T>(a.v[j]) : 0.f, x[8 + j] = some ? to_float<T>(b.v[j]) : 0.f;
+    uint4 a = lo, b = hi;
     h += kGroups;
     while (h >= heads) h -= heads, ++t;
     if (base + kGroups + group < items) fetch();
+    F2 x[4], y[4], squares = pair(0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) sum += x[j] * x[j];
+    for (int j = 0; j < 4; ++j) {
+      x[j].f = unpack_pair<T>(a, j);
+      y[j].f = unpack_pair<T>(b, j);
+      squares = fma2(x[j], x[j], fma2(y[j], y[j], squares));
+    }
+    float sum = some ? squares.f.x + squares.f.y : 0.f;
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (!some) continue;
@@ -104,17 +102,23 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(
     }
     if (!plain) {
       const float r = 1.f / sqrtf(sum * (1.f / kHeadDim) + eps);
+      const F2 rr = pair(r, r);
       const float* w = weights[is_q ? 0 : 1] + 8 * lane;
+      uint32_t out[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float c = cosines[token][8 * lane + j], s = sines[token][8 * lane + j];
-        const float u = x[j] * r * w[j], v = x[8 + j] * r * w[kHalf + j];
-        a.v[j] = from_float<T>(u * c - v * s);
-        b.v[j] = from_float<T>(v * c + u * s);
+      for (int j = 0; j < 4; ++j) {
+        const auto two = [&](const float* at) { return pair(at[2 * j], at[2 * j + 1]); };
+        const F2 c = two(&cosines[token][8 * lane]), s = two(&sines[token][8 * lane]);
+        const F2 u = mul2(mul2(x[j], two(w)), rr), v = mul2(mul2(y[j], two(w + kHalf)), rr);
+        const F2 first = fma2(u, c, mul2(pair(-v.f.x, -v.f.y), s)), second = fma2(v, c, mul2(u, s));
+        out[j] = pack_pair<T>(first.f.x, first.f.y);
+        out[4 + j] = pack_pair<T>(second.f.x, second.f.y);
       }
+      a = make_uint4(out[0], out[1], out[2], out[3]);
+      b = make_uint4(out[4], out[5], out[6], out[7]);
     }
-    *reinterpret_cast<Eight<T>*>(to + 8 * lane) = a;
-    *reinterpret_cast<Eight<T>*>(to + kHalf + 8 * lane) = b;
+    *reinterpret_cast<uint4*>(to + 8 * lane) = a;
+    *reinterpret_cast<uint4*>(to + kHalf + 8 * lane) = b;
   }
 }
 
