@@ -16,7 +16,8 @@ struct AttendArgs {
   int group, hq;
   int tile_rows, slot_rows;  // rows of a tile (token x head of the group), and of a slot of `parts`
   float scale_log2;      // scale log2(e)
-  float* parts;          // [2 blocks][slot_rows][kHeadDim] of tiles that lie in several blocks
+  float* parts;          // [2 blocks] slots of slot_rows x kHeadDim sums of tiles that lie in several blocks
+  int part_row, part_dims;  // of a slot: from one row to the next, from four dims to the next four
   float2* part_stats;    // [2 blocks][slot_rows]: m, sum
   int2* blocks_of;       // [rows][hq]: first and last block of a row's tile
   int* status;
@@ -46,9 +47,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// The page of a place of a sequence; a page outside the pool is reported and page 0 read in its stead.
-__device__ __forceinline__ int page_at(const AttendArgs& a, int b, int place) {
-  const int page = a.batch.tables[b * a.batch.table_stride + (place >> a.batch.page_shift)];
+// A page that is in the pool: one outside is reported and page 0 read in its stead.
+__device__ __forceinline__ int checked_page(const AttendArgs& a, int page) {
   if (page >= 0 && page < a.batch.pages) return page;
   report_status(a.status, kOutOfBounds);
   return 0;

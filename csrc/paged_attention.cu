@@ -142,7 +142,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane < boxes) {  // a lane each, so that their pages are looked up together
         const int at = key0 + lane * rows_per_box;
-        const int page = page_at(a, load.b, at), row = at & ((1 << batch.page_shift) - 1);
+        const int page = checked_page(a, batch.tables[load.b * batch.table_stride + (at >> batch.page_shift)]);
+        const int row = at & ((1 << batch.page_shift) - 1);
         const uint32_t box = to + lane * rows_per_box * 128;
         tma_load_4d(box, &key_map, bar, 0, row, load.head, page);
         tma_load_4d(box + kHalfBytes, &key_map, bar, 64, row, load.head, page);
@@ -327,38 +328,68 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// One warp per row of the call and head: joins the parts of rows whose tile lies in several blocks, and writes zeros to
-// rows that no sequence has.
+// Four warps per row of the call and head, a quarter of the parts each: they join the parts of a row whose tile lies in
+// several blocks. Zeros to rows that no sequence has. (One warp took 18 us for the 32 parts of a row of a single
+// sequence, one after another, twice as long as the attention itself.)
 template <typename T>
-__global__ void __launch_bounds__(256) attend_join_kernel(T* __restrict__ out, const __grid_constant__ AttendArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (item >= static_cast<int64_t>(a.batch.rows) * a.hq) return;
-  const int t = static_cast<int>(item / a.hq), h = static_cast<int>(item - static_cast<int64_t>(t) * a.hq);
+__global__ void __launch_bounds__(128) attend_join_kernel(T* __restrict__ out, const __grid_constant__ AttendArgs a) {
+  __shared__ float4 sums[4][32];
+  __shared__ float2 stats[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int item = blockIdx.x, t = item / a.hq, h = item - t * a.hq;
   const int b = paged_find(a.batch, t);
   PagedSequence s;
   if (b < a.batch.seqs) s = paged_sequence(a.batch, b, nullptr);
-  T* to = out + item * kHeadDim + 4 * lane;
+  T* to = out + static_cast<int64_t>(item) * kHeadDim + 4 * lane;
   if (t < s.start || t >= s.start + s.n) {
-    *reinterpret_cast<uint2*>(to) = make_uint2(0, 0);
+    if (warp == 0) *reinterpret_cast<uint2*>(to) = make_uint2(0, 0);
     return;
   }
   const int2 blocks = a.blocks_of[item];
   if (blocks.x == blocks.y) return;
   const int r = ((t - s.start) * a.group + h % a.group) % a.tile_rows;
-  auto slot = [&](int block) { return a.slot(block, blocks.x) + r; };
-  float mx = -INFINITY;
-  for (int x = blocks.x + lane; x <= blocks.y; x += 32) mx = fmaxf(mx, a.part_stats[slot(x)].x);
-  mx = warp_max(mx);
-  const float base = mx == -INFINITY ? 0.f : mx;
-  float sum = 0.f;
+  float mx = -INFINITY, sum = 0.f;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int x = blocks.x; x <= blocks.y; ++x) {
-    const float2 st = a.part_stats[slot(x)];
-    const float4 part = *reinterpret_cast<const float4*>(a.parts + slot(x) * kHeadDim + 4 * lane);
-    const float f = ex2_approx(st.x - base);
-    sum += f * st.y;
+  for (int x0 = blocks.x + warp; x0 <= blocks.y; x0 += 16) {  // four parts at once
+    float2 st[4];
+    float4 part[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int x = x0 + 4 * u;
+      st[u] = make_float2(-INFINITY, 0.f);
+      part[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (x > blocks.y) continue;
+      const int64_t slot = a.slot(x, blocks.x);
+      st[u] = a.part_stats[slot + r];
+      part[u] = *reinterpret_cast<const float4*>(a.parts + slot * kHeadDim + r * a.part_row + lane * a.part_dims);
+    }
+    const float to_max = fmaxf(fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)), mx);
+    const float base = to_max == -INFINITY ? 0.f : to_max, old = ex2_approx(mx - base);
+    mx = to_max;
+    sum *= old;
+    v.x *= old, v.y *= old, v.z *= old, v.w *= old;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float f = ex2_approx(st[u].x - base);
+      sum += f * st[u].y;
+      v.x += f * part[u].x, v.y += f * part[u].y, v.z += f * part[u].z, v.w += f * part[u].w;
+    }
+  }
+  sums[warp][lane] = v;
+  if (lane == 0) stats[warp] = make_float2(mx, sum);
+  __syncthreads();
+  if (warp != 0) return;
+  float whole = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) whole = fmaxf(whole, stats[w].x);
+  const float base = whole == -INFINITY ? 0.f : whole;
+  sum = 0.f;
+  v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = ex2_approx(stats[w].x - base);
+    const float4 part = sums[w][lane];
+    sum += f * stats[w].y;
     v.x += f * part.x, v.y += f * part.y, v.z += f * part.z, v.w += f * part.w;
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -388,7 +419,7 @@ void launch_attend_join(const AttendArgs& a, at::Tensor& out) {
   const int64_t items = static_cast<int64_t>(a.batch.rows) * a.hq;
   auto launch = [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    attend_join_kernel<T><<<static_cast<unsigned>((items + 7) / 8), 256, 0, stream()>>>(static_cast<T*>(out.data_ptr()), a);
+    attend_join_kernel<T><<<static_cast<unsigned>(items), 128, 0, stream()>>>(static_cast<T*>(out.data_ptr()), a);
   };
   if (out.scalar_type() == at::kHalf) launch(static_cast<__half*>(nullptr));
   else launch(static_cast<__nv_bfloat16*>(nullptr));
@@ -407,7 +438,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& keys, const at
   const int64_t rows = q.size(0), hq = q.size(1);
   AttendArgs a{};
   a.batch = paged_batch(keys, values, tables, starts, lengths, rows, what);
-  TDSV_CHECK(hq % a.batch.kv_heads == 0 && rows * hq < (int64_t(1) << 31), what, ": heads must be a multiple of the cache's");
+  TDSV_CHECK(hq % a.batch.kv_heads == 0 && rows * hq < (int64_t(1) << 30), what, ": heads must be a multiple of the cache's");
   a.group = static_cast<int>(hq / a.batch.kv_heads);
   a.hq = static_cast<int>(hq);
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
@@ -429,6 +460,8 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& keys, const at
   const int blocks = num_sms();
   a.tile_rows = many ? kRowsTile / a.group * a.group : kTileRows;
   a.slot_rows = many ? kRowsTile : kTileRows;
+  a.part_row = many ? 4 : kHeadDim;
+  a.part_dims = many ? 4 * kRowsTile : 4;
   const auto f32 = q.options().dtype(at::kFloat);
   auto parts = at::empty({2 * blocks, a.slot_rows, kHeadDim}, f32);
   auto stats = at::empty({2 * blocks, a.slot_rows, 2}, f32);
