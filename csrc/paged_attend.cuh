@@ -9,6 +9,12 @@
 
 namespace tdsv {
 
+// The tile that begins in a block and goes on behind it, which is the block's last one, if there is one (rows > 0).
+struct Split {
+  int last, rows;            // the block that it ends in; rows of the tile
+  int start, first, head;    // the sequence's first row of the call; the tile's first row in it; the group's first head
+};
+
 struct AttendArgs {
   PagedBatch batch;
   const uint32_t* tree;  // [rows, tree_words]
@@ -19,7 +25,7 @@ struct AttendArgs {
   float* parts;          // [2 blocks] slots of slot_rows x kHeadDim sums of tiles that lie in several blocks
   int part_row, part_dims;  // of a slot: from one row to the next, from four dims to the next four
   float2* part_stats;    // [2 blocks][slot_rows]: m, sum
-  int2* blocks_of;       // [rows][hq]: first and last block of a row's tile
+  Split* splits;         // [blocks]
   int* status;
 
   // Where block `block` keeps its part of a tile that begins in block `first`: a block holds at most one part of a
@@ -112,7 +118,7 @@ __device__ __forceinline__ Stretch block_stretch(const AttendArgs& a, StretchScr
 }
 
 // Host, in paged_attention.cu.
-void launch_attend_join(const AttendArgs& a, at::Tensor& out);
+void launch_attend_join(const AttendArgs& a, at::Tensor& out, int blocks);
 // Host, in paged_rows.cu: attention by tiles of up to 256 rows.
 constexpr int kRowsTile = 256;
 void launch_attend_rows(const AttendArgs& a, const CUtensorMap& key_map, const CUtensorMap& value_map, const at::Tensor& q,

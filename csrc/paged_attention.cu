@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const PagedBatch& batch = a.batch;
 
   if (tid == 0) {
+    a.splits[blockIdx.x].rows = 0;
     for (int i = 0; i < kWarps * kStages; ++i) mbar_init(&sm.full[i / kStages][i % kStages], 1);
     fence_barrier_init();
   }
@@ -318,48 +319,63 @@ __global__ void __launch_bounds__(kThreads, 1)
           *reinterpret_cast<float4*>(a.parts + (slot + r) * kHeadDim + d) = v;
           if (d == 0) a.part_stats[slot + r] = make_float2(mx, sum);
         }
-        // (a token's rows may lie in two tiles: each tile writes its own rows' blocks)
-        if (d == 0 && first == static_cast<int>(blockIdx.x))
-          a.blocks_of[static_cast<int64_t>(t) * a.hq + compute.head * a.group + row % a.group] = make_int2(first, last);
       }
+      if (tid == 0 && !whole && first == static_cast<int>(blockIdx.x))
+        a.splits[first] = {last, min(kTileRows, s.n * a.group - compute.tile * kTileRows), s.start, compute.tile * kTileRows,
+                           compute.head * a.group};
       __syncthreads();
     }
     if (i + 1 < count) compute.next(a);
   }
 }
 
-// Four warps per row of the call and head, a quarter of the parts each: they join the parts of a row whose tile lies in
-// several blocks. Zeros to rows that no sequence has. (One warp took 18 us for the 32 parts of a row of a single
-// sequence, one after another, twice as long as the attention itself.)
-template <typename T>
-__global__ void __launch_bounds__(128) attend_join_kernel(T* __restrict__ out, const __grid_constant__ AttendArgs a) {
-  __shared__ float4 sums[4][32];
-  __shared__ float2 stats[4];
+// Joins the parts of tiles that lie in several blocks: WARPS warps a row, each with a share of the parts. (A single
+// sequence's row has 32 of them: one warp took 18 us for it, twice as long as the attention itself.) The first blocks of
+// the grid are for the tiles that begin in each block of the attention; the others look for rows that no sequence has,
+// a thread each, and write zeros there.
+constexpr int kJoinThreads = 256;
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(T* __restrict__ out, const __grid_constant__ AttendArgs a,
+                                                                   int blocks, int per_tile) {
+  constexpr int kRows = kJoinThreads / 32 / WARPS;
+  __shared__ float4 sums[kRows][WARPS][32];
+  __shared__ float2 stats[kRows][WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int item = blockIdx.x, t = item / a.hq, h = item - t * a.hq;
-  const int b = paged_find(a.batch, t);
-  PagedSequence s;
-  if (b < a.batch.seqs) s = paged_sequence(a.batch, b, nullptr);
-  T* to = out + static_cast<int64_t>(item) * kHeadDim + 4 * lane;
-  if (t < s.start || t >= s.start + s.n) {
-    if (warp == 0) *reinterpret_cast<uint2*>(to) = make_uint2(0, 0);
+  if (static_cast<int>(blockIdx.x) >= blocks * per_tile) {
+    const int t = (blockIdx.x - blocks * per_tile) * kJoinThreads + threadIdx.x;
+    if (t >= a.batch.rows) return;
+    int lo = 0, hi = a.batch.seqs;  // the sequences whose rows end at or before t
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (a.batch.starts[mid + 1] <= t) lo = mid + 1;
+      else hi = mid;
+    }
+    if (lo < a.batch.seqs) {
+      const PagedSequence s = paged_sequence(a.batch, lo, nullptr);
+      if (t >= s.start && t < s.start + s.n) return;
+    }
+    uint4* to = reinterpret_cast<uint4*>(out + static_cast<int64_t>(t) * a.hq * kHeadDim);
+    for (int i = 0; i < a.hq * kHeadDim / 8; ++i) to[i] = make_uint4(0, 0, 0, 0);
     return;
   }
-  const int2 blocks = a.blocks_of[item];
-  if (blocks.x == blocks.y) return;
-  const int r = ((t - s.start) * a.group + h % a.group) % a.tile_rows;
+  const int first = blockIdx.x / per_tile;
+  const Split split = a.splits[first];
+  const int r = (blockIdx.x - first * per_tile) * kRows + warp / WARPS, w0 = warp % WARPS;
+  if (r >= split.rows && (WARPS == 1 || kRows == 1 || (r - warp / WARPS) >= split.rows)) return;
+  const bool there = r < split.rows;
+  const int row = split.first + r, last = there ? split.last : -1;
   float mx = -INFINITY, sum = 0.f;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int x0 = blocks.x + warp; x0 <= blocks.y; x0 += 16) {  // four parts at once
+  for (int x0 = first + w0; x0 <= last; x0 += 4 * WARPS) {  // four parts at once
     float2 st[4];
     float4 part[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int x = x0 + 4 * u;
+      const int x = x0 + u * WARPS;
       st[u] = make_float2(-INFINITY, 0.f);
       part[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (x > blocks.y) continue;
-      const int64_t slot = a.slot(x, blocks.x);
+      if (x > last) continue;
+      const int64_t slot = a.slot(x, first);
       st[u] = a.part_stats[slot + r];
       part[u] = *reinterpret_cast<const float4*>(a.parts + slot * kHeadDim + r * a.part_row + lane * a.part_dims);
     }
@@ -375,24 +391,29 @@ __global__ void __launch_bounds__(128) attend_join_kernel(T* __restrict__ out, c
       v.x += f * part[u].x, v.y += f * part[u].y, v.z += f * part[u].z, v.w += f * part[u].w;
     }
   }
-  sums[warp][lane] = v;
-  if (lane == 0) stats[warp] = make_float2(mx, sum);
-  __syncthreads();
-  if (warp != 0) return;
-  float whole = -INFINITY;
+  if constexpr (WARPS > 1) {
+    const int x = warp / WARPS;
+    sums[x][w0][lane] = v;
+    if (lane == 0) stats[x][w0] = make_float2(mx, sum);
+    __syncthreads();
+    if (w0 != 0) return;
+    mx = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) whole = fmaxf(whole, stats[w].x);
-  const float base = whole == -INFINITY ? 0.f : whole;
-  sum = 0.f;
-  v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < WARPS; ++w) mx = fmaxf(mx, stats[x][w].x);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    sum = 0.f;
+    v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float f = ex2_approx(stats[w].x - base);
-    const float4 part = sums[w][lane];
-    sum += f * stats[w].y;
-    v.x += f * part.x, v.y += f * part.y, v.z += f * part.z, v.w += f * part.w;
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = ex2_approx(stats[x][w].x - base);
+      const float4 part = sums[x][w][lane];
+      sum += f * stats[x][w].y;
+      v.x += f * part.x, v.y += f * part.y, v.z += f * part.z, v.w += f * part.w;
+    }
   }
+  if (!there) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* to = out + (static_cast<int64_t>(split.start + row / a.group) * a.hq + split.head + row % a.group) * kHeadDim + 4 * lane;
   *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
 }
 
@@ -415,11 +436,17 @@ CUtensorMap pool_map(const at::Tensor& pool, int box_rows) {
 
 }  // namespace
 
-void launch_attend_join(const AttendArgs& a, at::Tensor& out) {
-  const int64_t items = static_cast<int64_t>(a.batch.rows) * a.hq;
+void launch_attend_join(const AttendArgs& a, at::Tensor& out, int blocks) {
   auto launch = [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    attend_join_kernel<T><<<static_cast<unsigned>(items), 128, 0, stream()>>>(static_cast<T*>(out.data_ptr()), a);
+    auto go = [&](auto kern, int rows) {  // rows of a tile that a block takes
+      const int per_tile = (a.tile_rows + rows - 1) / rows;
+      const unsigned grid = static_cast<unsigned>(blocks * per_tile + (a.batch.rows + kJoinThreads - 1) / kJoinThreads);
+      kern<<<grid, kJoinThreads, 0, stream()>>>(static_cast<T*>(out.data_ptr()), a, blocks, per_tile);
+    };
+    // tiles of many rows have few parts each, unless there are few tiles; those of a step may have one for every block
+    if (a.slot_rows > kTileRows) go(attend_join_kernel<T, 1>, kJoinThreads / 32);
+    else go(attend_join_kernel<T, 4>, kJoinThreads / 32 / 4);
   };
   if (out.scalar_type() == at::kHalf) launch(static_cast<__half*>(nullptr));
   else launch(static_cast<__nv_bfloat16*>(nullptr));
@@ -463,12 +490,12 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& keys, const at
   a.part_row = many ? 4 : kHeadDim;
   a.part_dims = many ? 4 * kRowsTile : 4;
   const auto f32 = q.options().dtype(at::kFloat);
-  auto parts = at::empty({2 * blocks, a.slot_rows, kHeadDim}, f32);
-  auto stats = at::empty({2 * blocks, a.slot_rows, 2}, f32);
-  auto blocks_of = at::empty({rows, hq, 2}, f32.dtype(at::kInt));
-  a.parts = parts.data_ptr<float>();
-  a.part_stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
-  a.blocks_of = reinterpret_cast<int2*>(blocks_of.data_ptr<int>());
+  // parts, their statistics and the splits, in one allocation
+  const int64_t slots = 2 * static_cast<int64_t>(blocks) * a.slot_rows;
+  auto workspace = at::empty({slots * (kHeadDim + 2) + blocks * static_cast<int64_t>(sizeof(Split) / sizeof(float))}, f32);
+  a.parts = workspace.data_ptr<float>();
+  a.part_stats = reinterpret_cast<float2*>(a.parts + slots * kHeadDim);
+  a.splits = reinterpret_cast<Split*>(a.parts + slots * (kHeadDim + 2));
   bind_primary_context();
   const int box_rows = std::min(1 << a.batch.page_shift, many ? 128 : kWarpKeys);
   const CUtensorMap key_map = pool_map(keys, box_rows), value_map = pool_map(values, box_rows);
@@ -487,7 +514,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& keys, const at
     else launch(static_cast<__nv_bfloat16*>(nullptr));
     TDSV_LAUNCH_CHECK();
   }
-  launch_attend_join(a, out);
+  launch_attend_join(a, out, blocks);
   return out;
 }
 

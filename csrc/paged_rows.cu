@@ -25,9 +25,16 @@ constexpr int kHalfRows = 128, kUnitKeys = 128;
 constexpr int kAtomBytes = 128 * 128;    // 128 rows of 64 dims, swizzled
 constexpr int kSlotBytes = 2 * kAtomBytes;
 constexpr int kSlots = 5;
+constexpr int kSplitThread = 64;          // of the first half's softmax, which every tile has
 
 enum : int { kWaitEmpty = 351, kWaitQ, kWaitKeys, kWaitValues, kWaitWeights, kWaitScores, kWaitSums, kWaitTail,
               kWaitPair };
+
+// A warp's wait that polls: a suspended one wakes late, and these are on the path from one product to the next (1.5 % of
+// a long chunk).
+__device__ __forceinline__ bool spin_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code));
+}
 
 template <typename T>
 __device__ __forceinline__ uint32_t product_desc(bool b_mn_major) {
@@ -163,6 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Shared& sm = *reinterpret_cast<Shared*>(ring + kSlots * kSlotBytes);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
+  if (tid == kSplitThread) a.splits[blockIdx.x].rows = 0;
   if (tid == 0) {
     for (int h = 0; h < 2; ++h) {
       mbar_init(&sm.q_full[h], 2 * kHalfRows);
@@ -254,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int slot = 0, slot_round = 0;
         uint32_t q_turn = 0, p_turn = 0;  // parities, a bit for each half
         auto take = [&](int code) {  // the ring's next slot, when it is full
-          ok = ok && mbar_sleep_wait(&sm.kv_full[slot], slot_round & 1, a.status, code);
+          ok = ok && mbar_wait(&sm.kv_full[slot], slot_round & 1, a.status, code);
           const int s = slot;
           if (++slot == kSlots) slot = 0, ++slot_round;
           return s;
@@ -277,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int halves = p.rows > kHalfRows ? 2 : 1;
           const int first = take(kWaitKeys);
           for (int h = 0; ok && h < halves; ++h) {
-            ok = mbar_sleep_wait(&sm.q_full[h], q_turn >> h & 1, a.status, kWaitQ);
+            ok = mbar_wait(&sm.q_full[h], q_turn >> h & 1, a.status, kWaitQ);
             q_turn ^= 1u << h;
             if (!ok) break;
             tc_fence_after();
@@ -290,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int ks = more ? take(kWaitKeys) : 0;
             const int vs = take(kWaitValues);
             for (int h = 0; ok && h < halves; ++h) {
-              ok = mbar_sleep_wait(&sm.p_full[h], p_turn >> h & 1, a.status, kWaitWeights);
+              ok = mbar_wait(&sm.p_full[h], p_turn >> h & 1, a.status, kWaitWeights);
               p_turn ^= 1u << h;
               if (!ok) break;
               tc_fence_after();
@@ -352,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             fence_proxy_async_smem();
           }
-          if (!(ok = warp_wait(&sm.s_full[half], s_turn & 1, a.status, kWaitScores))) break;
+          if (!(ok = spin_wait(&sm.s_full[half], s_turn & 1, a.status, kWaitScores))) break;
           s_turn ^= 1;
           tc_fence_after();
           // what the row sees; nothing is hidden before the tile's first token
@@ -393,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           sm.exchange[half][part][r] = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
           mbar_arrive(pair_bar);
-          if (!(ok = warp_wait(pair_bar, pair_turn & 1, a.status, kWaitPair))) break;
+          if (!(ok = spin_wait(pair_bar, pair_turn & 1, a.status, kWaitPair))) break;
           pair_turn ^= 1;
           const float mx = fmaxf(sm.exchange[half][0][r], sm.exchange[half][1][r]) * a.scale_log2;
           float alpha = 1.f;
@@ -439,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         sm.exchange[half][part][r] = l;
         mbar_arrive(pair_bar);
-        if (!(ok = warp_wait(pair_bar, pair_turn & 1, a.status, kWaitPair))) break;
+        if (!(ok = spin_wait(pair_bar, pair_turn & 1, a.status, kWaitPair))) break;
         pair_turn ^= 1;
         l = sm.exchange[half][0][r] + sm.exchange[half][1][r];
         const int64_t unit0 = sm.line.end - left - unit;  // the tile's place in the line
@@ -476,7 +484,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
         if (there && part == 0 && first != last) a.part_stats[slot + row] = make_float2(m, l);
-        if (there && part == 0 && first == static_cast<int>(blockIdx.x)) a.blocks_of[mine / 2] = make_int2(first, last);
+        if (tid == kSplitThread && first != last && first == static_cast<int>(blockIdx.x))
+          a.splits[first] = {last, p.rows, p.s.start, at.tile * a.tile_rows, at.head * a.group};
       }
       left -= p.count;
       unit = 0;
