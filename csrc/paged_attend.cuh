@@ -21,6 +21,7 @@ struct AttendArgs {
   int tree_words;        // -1: causal
   int group, hq;
   int tile_rows, slot_rows;  // rows of a tile (token x head of the group), and of a slot of `parts`
+  int least;             // units of a block, where there are any
   float scale_log2;      // scale log2(e)
   float* parts;          // [2 blocks] slots of slot_rows x kHeadDim sums of tiles that lie in several blocks
   int part_row, part_dims;  // of a slot: from one row to the next, from four dims to the next four
@@ -96,7 +97,7 @@ __device__ __forceinline__ Stretch block_stretch(const AttendArgs& a, StretchScr
   }
   before -= mine;
   Stretch s;
-  s.share = (total + gridDim.x - 1) / gridDim.x;
+  s.share = max(static_cast<int64_t>(a.least), (total + gridDim.x - 1) / gridDim.x);
   s.begin = min(total, s.share * blockIdx.x);
   s.end = min(total, s.begin + s.share);
   if (s.begin < s.end && s.begin >= before && s.begin < before + mine) {

@@ -487,6 +487,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& keys, const at
   const int blocks = num_sms();
   a.tile_rows = many ? kRowsTile / a.group * a.group : kTileRows;
   a.slot_rows = many ? kRowsTile : kTileRows;
+  a.least = many ? 2 : 1;
   a.part_row = many ? 4 : kHeadDim;
   a.part_dims = many ? 4 * kRowsTile : 4;
   const auto f32 = q.options().dtype(at::kFloat);

@@ -382,9 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           // 32 scores at a time, which is what the registers hold: the first ones are read again for their weights
           uint32_t sv[32];
-          const auto fetch = [&](int c) {
-            tmem_ld_32x32b_x32(s_col + c * 32, sv);
-            tmem_ld_wait();
+          const auto hide = [&](int c) {
             if (masked) {
 #pragma unroll
               for (int j = 0; j < 32; ++j)
@@ -394,7 +392,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            fetch(c);
+            tmem_ld_32x32b_x32(s_col + c * 32, sv);
+            tmem_ld_wait();
+            hide(c);
 #pragma unroll
             for (int j = 0; j < 32; j += 2)
               m4[j / 2 & 3] = max3(m4[j / 2 & 3], __uint_as_float(sv[j]), __uint_as_float(sv[j + 1]));
@@ -425,7 +425,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           F2 sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
           for (int c = 1; c >= 0; --c) {
-            if (c == 0) fetch(0);
+            if (c == 0) {
+              tmem_ld_wait();
+              hide(0);
+            }
             uint32_t packed[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -434,7 +437,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               sums[j & 1] = add2(sums[j & 1], w);
               packed[j] = pack2<T>(w.f.x, w.f.y);
             }
-            tmem_st_32x32b_x16(s_col + c * 32, packed);  // over these scores alone
+            if (c == 1) tmem_ld_32x32b_x32(s_col, sv);  // on its way while these weights leave
+            tmem_st_32x32b_x16(s_col + c * 32, packed);   // over these scores alone
           }
           const F2 sum = add2(sums[0], sums[1]);
           l = l * alpha + (sum.f.x + sum.f.y);

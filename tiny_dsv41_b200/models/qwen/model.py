@@ -30,6 +30,7 @@ from ...parallel.dispatch import TokenDispatcher
 from ...utils.trace import nvtx_range
 from ..common import Linear, LMHead, fusable
 from .config import Qwen3MoeConfig
+from .generation import PagedKVCache
 
 
 class Qwen3MoeRMSNorm(nn.Module):
@@ -73,6 +74,12 @@ class Qwen3MoeAttention(nn.Module):
             qkv = ops.linear(hidden, weight, replayable=True)  # the recompute reuses this product
         else:
             qkv = torch.cat((self.q_proj(hidden), self.k_proj(hidden), self.v_proj(hidden)), dim=-1)
+        if isinstance(cache, PagedKVCache):  # decoding over pages: norms, rotation and the append are one kernel
+            if self.context_parallel.enabled:
+                raise ValueError("the KV cache does not support context parallelism")
+            out = cache.attend(self.layer_id, qkv, self.q_norm.weight, self.k_norm.weight, position_ids, freqs,
+                               self.num_heads, self.num_key_value_heads, self.eps)
+            return self.o_proj(out.reshape(batch, length, -1))
         q, k, v = ops.qk_norm_rope(qkv, self.q_norm.weight, self.k_norm.weight, position_ids, freqs,
                                    self.num_heads, self.num_key_value_heads, self.eps)
         q = q.view(batch, length, self.num_heads, self.head_dim)
