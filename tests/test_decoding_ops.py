@@ -460,6 +460,22 @@ def test_logits_repeated_ids(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_logits_of_long_lists(device):
+    """A history beyond 16-bit counts, and more biases than a block lists, some of them repeated."""
+    vocab = 700
+    x = torch.randn(2, vocab, generator=_gen(1)).bfloat16()
+    history = (torch.rand(2, 40000, generator=_gen(2)) ** 3 * vocab).long()
+    history[0, 20000:] = 3
+    ones = torch.ones(2)
+    _check_logits(x, device, history=history, lengths=torch.tensor([40000, 17000], dtype=torch.int32),
+                  prompts=torch.tensor([100, 0], dtype=torch.int32), repetition=ones * 1.1, presence=ones, frequency=ones * 1e-3)
+    ids = torch.randint(-1, vocab, (2, 1300), generator=_gen(3))
+    _check_logits(x.float(), device, bias_ids=ids, bias=torch.randn(2, 1300, generator=_gen(4)))
+    _check_logits(x, device, history=history[:, :16384], frequency=ones * 1e-3, bias_ids=ids[:, :300],
+                  bias=torch.randn(2, 300, generator=_gen(4)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_logits_layouts(device, dtype):
     """Rows of a wider tensor, several leading dimensions, tables for all rows, numbers for penalties."""
@@ -534,6 +550,16 @@ def test_attention_refusals(device):
         ops.paged_attention(q, three, three, c["batch"])
     with pytest.raises(RuntimeError, match="no gradient"):
         ops.paged_attention(**{**good, "q": q.clone().requires_grad_()})
+
+
+def test_forward_mode_tangents_are_refused():
+    from torch.autograd import forward_ad
+
+    x = torch.randn(1, 10)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="no gradient"):
+            ops.process_logits(forward_ad.make_dual(x, torch.ones_like(x)))
+        ops.process_logits(x)
 
 
 def test_batch_refusals():
