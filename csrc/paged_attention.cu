@@ -17,8 +17,11 @@
 // follows from starts and lengths on the GPU; each block sums them for itself.
 //
 // Four warps take 32 of a unit's keys each, with their own running maximum and sum, and with their own ring of
-// tiles that TMA fills: no warp waits for another until the tile is joined. A key or value crosses HBM once for each
-// 16 rows.
+// tiles that TMA fills (192 KB of an SM on the way or at work): no warp waits for another until the tile is joined. A key or
+// value crosses HBM once for each 16 rows, and the cache's traffic is what bounds a step: 64 sequences of up to 8192 tokens
+// (554 MB) take 106 us, 5.2 TB/s, 8 of up to 40960 tokens 92 us, 5.5 TB/s; one of 4001 tokens 9 us and 3 us for the join.
+// Where a sequence brings more rows the kernel of paged_rows.cu takes them: at 32 drafted tokens (256 rows) this one needs
+// 563 us for what takes 77 there, at 2048 tokens of a prompt 5632 for 505.
 #include "paged_attend.cuh"
 
 namespace tdsv {
@@ -481,13 +484,17 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& keys, const at
   auto out = at::empty_like(q);
   if (rows == 0) return out;
   a.status = status_word_ptr();
-  // A tile of 16 rows reads its keys once for all of a decoding step's rows; where a sequence brings more of them (on
-  // average), tiles of 256 on the tensor cores' own pipeline do.
-  const bool many = a.group <= kRowsTile && rows * a.group > 32 * static_cast<int64_t>(a.batch.seqs);
+  // A tile of 16 rows reads its keys once for all of a decoding step's rows; where a sequence brings more (on average),
+  // tiles of 256 do: 64 sequences of 4000 tokens take 115 us by the one and 131 by the other at 16 rows, 188 and 131 at 24.
+  // While SMs are idle another tile of 16 costs less than the other kernel's longer start: a single sequence of 4000
+  // tokens takes 18 and 25 us at 16 rows, 23 and 29 at 64, 29 and 29 at 128 (512 rows over all heads).
+  const int64_t most_tokens = (static_cast<int64_t>(a.batch.seqs) * a.batch.width) << a.batch.page_shift;
+  const bool idle = rows * hq <= 512 && most_tokens <= 8192;
+  const bool many = a.group <= kRowsTile && rows * a.group > kTileRows * static_cast<int64_t>(a.batch.seqs) && !idle;
   const int blocks = num_sms();
   a.tile_rows = many ? kRowsTile / a.group * a.group : kTileRows;
   a.slot_rows = many ? kRowsTile : kTileRows;
-  a.least = many ? 2 : 1;
+  a.least = many ? 2 : 1;  // (a tile's end costs that kernel as much as some units)
   a.part_row = many ? 4 : kHeadDim;
   a.part_dims = many ? 4 * kRowsTile : 4;
   const auto f32 = q.options().dtype(at::kFloat);

@@ -9,8 +9,13 @@
 //   warps 2-17   softmax, two threads per row, of 64 keys each: scores from tensor memory into registers, the row's mask,
 //                the running maximum (agreed on through shared memory; raised only when it grows by more than 2^8, so that
 //                the sums in tensor memory are rarely rescaled), the weights back over the scores as the A operand of PV
-// While one half's softmax runs, the tensor cores work on the other half. A unit takes the longer of its products (2200
-// cycles) and a half's softmax with its own products; one thread per row took 2600 cycles for its part, which made 4200.
+// While one half's softmax runs, the tensor cores work on the other half. What bounds it is the chain of a half: its
+// softmax (2400 cycles: read 400, the rows' maxima agreed on 300, the exponentials and their way back 1700), then its
+// products (1100), and a wake-up at either end (250 each): 4000 cycles a unit, of which the tensor cores work 2200. Three
+// chunks of prompts (5312 new tokens on 17535 cached, 459 GFLOP) take 0.47 to 0.51 ms, 0.9 to 1.0 PFLOP/s. Tried: one
+// thread a row (the scores spill, to L2, as the ring leaves next to nothing of L1: 1313 us), all 64 scores in registers
+// (172 bytes spilled: 506 us against 463), a part of the exponentials as polynomials (595 and 654 us against 564: the
+// instructions cost more than the special-function unit's time that they save).
 //   TMEM: scores 0 [0, 128), scores 1 [128, 256), sums 0 [256, 384), sums 1 [384, 512).
 // Commits of QK come behind the half's last PV, so a thread that sees its next scores may touch its sums.
 #include "logit_rows.cuh"

@@ -286,6 +286,14 @@ def test_attention_long_and_many():
 
 
 @pytest.mark.gpu
+def test_attention_of_wide_groups():
+    """More heads of one key head than a tile has rows, and as many."""
+    _attend([1, 3], [40, 200], (260, 1), 16, torch.bfloat16, "cuda")
+    _attend([1, 3], [40, 200], (256, 1), 16, torch.bfloat16, "cuda")
+    _attend([2, 1], [300, 7], (200, 1), 64, torch.float16, "cuda", tree=_random_tree([2, 1], 1, 3))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("heads, page, dtype", [((8, 1), 16, torch.bfloat16), ((5, 1), 64, torch.float16),
                                                 ((6, 2), 128, torch.bfloat16), ((48, 1), 32, torch.bfloat16)])
 def test_attention_of_prompts(heads, page, dtype):

@@ -189,8 +189,11 @@ def test_cache_refusals():
         cache.plan([(s, 1), (s, 1)])
     with pytest.raises(ValueError):
         cache.plan([(s, 2)], [[-1]])
+    with pytest.raises(ValueError, match="before its child"):
+        cache.plan([(s, 2)], [[-1, 1]])
     with pytest.raises(KeyError):
         cache.plan([(99, 1)])
+    assert cache.lengths == {s: 20}
     with pytest.raises(ValueError):
         PagedKVCache(config, 0)
     cache.release(s)
@@ -245,6 +248,10 @@ def test_generation_ends_and_repeats(device):
         assert 1 <= len(tokens) == len(scores) <= 12
         assert all(t % 9 for t in tokens[:-1]) and (tokens[-1] % 9 == 0 or len(tokens) == 12)
         assert all(s <= 0 for s in scores)
-    for bad in ((model, [], 3), (model, [[]], 3), (model, prompts, 0), (model, prompts, 5000)):
+    for bad in ((model, [], 3), (model, [[]], 3), (model, prompts, 0), (model, prompts, 5000), (model, [[512]], 3),
+                (model, [[-1]], 3)):
         with pytest.raises(ValueError):
             generate(*bad)
+    for kw in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(bias={512: 1.0})):
+        with pytest.raises(ValueError):
+            generate(model, prompts, 3, **kw)

@@ -13,6 +13,7 @@ a batch of prompts over it, with the penalties, biases and masks of ``ops.proces
 
 from __future__ import annotations
 
+import math
 from typing import Callable, NamedTuple, Sequence
 
 import torch
@@ -76,6 +77,8 @@ class PagedKVCache:
             raise ValueError("a sequence is planned once, with a number of new tokens")
         if parents is not None and [len(p) for p in parents] != [n for _, n in new]:
             raise ValueError("a tree has a parent for each new token")
+        if parents is not None and any(not -1 <= parent < j for tree in parents for j, parent in enumerate(tree)):
+            raise ValueError("a parent is drafted before its child")
         need = [max(0, -(-(self.lengths[s] + n) // self.page) - len(self.pages[s])) for s, n in new]
         if sum(need) > len(self.free):
             raise RuntimeError(f"the cache is full: {sum(need)} pages are needed and {len(self.free)} free")
@@ -158,6 +161,10 @@ def generate(model, prompts: Sequence[Sequence[int]], max_new_tokens: int, *, te
         raise ValueError("generate needs prompts of at least one token")
     if max_new_tokens < 1 or chunk < 1:
         raise ValueError("max_new_tokens and chunk must be positive")
+    if not (math.isfinite(temperature) and temperature >= 0):
+        raise ValueError("temperature must be finite and not negative")
+    if any(not 0 <= t < config.vocab_size for part in (*prompts, bias or ()) for t in part):
+        raise ValueError("prompts and biases hold tokens of the vocabulary")
     if any(len(p) + max_new_tokens > config.max_position_embeddings for p in prompts):
         raise ValueError("a prompt and its answer are longer than max_position_embeddings")
     device, chunk = weight.device, min(chunk, config.max_position_embeddings)

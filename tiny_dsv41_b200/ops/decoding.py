@@ -76,7 +76,7 @@ def _check_cache(keys: torch.Tensor, values: torch.Tensor, batch: PagedBatch) ->
 def _refuse_gradients(what: str, *tensors: torch.Tensor | None) -> None:
     # (forward-mode tangents exist inside a level alone; asking each tensor for one costs a microsecond)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) or (
-            forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+            getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
                                                    for t in tensors)):
         raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad() or with detached tensors")
 
