@@ -24,7 +24,6 @@ struct AttendArgs {
   int least;             // units of a block, where there are any
   float scale_log2;      // scale log2(e)
   float* parts;          // [2 blocks] slots of slot_rows x kHeadDim sums of tiles that lie in several blocks
-  int part_row, part_dims;  // of a slot: from one row to the next, from four dims to the next four
   float2* part_stats;    // [2 blocks][slot_rows]: m, sum
   Split* splits;         // [blocks]
   int* status;

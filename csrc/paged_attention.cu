@@ -21,7 +21,7 @@
 // value crosses HBM once for each 16 rows, and the cache's traffic is what bounds a step: 64 sequences of up to 8192 tokens
 // (554 MB) take 106 us, 5.2 TB/s, 8 of up to 40960 tokens 92 us, 5.5 TB/s; one of 4001 tokens 9 us and 3 us for the join.
 // Where a sequence brings more rows the kernel of paged_rows.cu takes them: at 32 drafted tokens (256 rows) this one needs
-// 563 us for what takes 77 there, at 2048 tokens of a prompt 5632 for 505.
+// 563 us for what takes 72 there, at 2048 tokens of a prompt 5632 for 501.
 #include "paged_attend.cuh"
 
 namespace tdsv {
@@ -332,11 +332,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the parts of tiles that lie in several blocks: WARPS warps a row, each with a share of the parts. (A single
-// sequence's row has 32 of them: one warp took 18 us for it, twice as long as the attention itself.) The first blocks of
-// the grid are for the tiles that begin in each block of the attention; the others look for rows that no sequence has,
-// a thread each, and write zeros there.
+// Rows that no sequence has: zeros, a thread a row.
 constexpr int kJoinThreads = 256;
+template <typename T>
+__device__ __forceinline__ void zero_row(T* out, const AttendArgs& a, int t) {
+  if (t >= a.batch.rows) return;
+  int lo = 0, hi = a.batch.seqs;  // the sequences whose rows end at or before t
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (a.batch.starts[mid + 1] <= t) lo = mid + 1;
+    else hi = mid;
+  }
+  if (lo < a.batch.seqs) {
+    const PagedSequence s = paged_sequence(a.batch, lo, nullptr);
+    if (t >= s.start && t < s.start + s.n) return;
+  }
+  uint4* to = reinterpret_cast<uint4*>(out + static_cast<int64_t>(t) * a.hq * kHeadDim);
+  for (int i = 0; i < a.hq * kHeadDim / 8; ++i) to[i] = make_uint4(0, 0, 0, 0);
+}
+
+// Joins the parts of tiles that lie in several blocks. The first blocks of the grid are for the tiles that begin in each
+// block of the attention, `per_tile` of them for each; the others look for rows that no sequence has.
+//
+// Tiles of 16 rows: WARPS warps a row, each with a share of the parts. (A single sequence's row has 32 of them: one warp took
+// 18 us for it, twice as long as the attention itself.)
 template <typename T, int WARPS>
 __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(T* __restrict__ out, const __grid_constant__ AttendArgs a,
                                                                    int blocks, int per_tile) {
@@ -345,26 +364,13 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(T* __restrict
   __shared__ float2 stats[kRows][WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (static_cast<int>(blockIdx.x) >= blocks * per_tile) {
-    const int t = (blockIdx.x - blocks * per_tile) * kJoinThreads + threadIdx.x;
-    if (t >= a.batch.rows) return;
-    int lo = 0, hi = a.batch.seqs;  // the sequences whose rows end at or before t
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (a.batch.starts[mid + 1] <= t) lo = mid + 1;
-      else hi = mid;
-    }
-    if (lo < a.batch.seqs) {
-      const PagedSequence s = paged_sequence(a.batch, lo, nullptr);
-      if (t >= s.start && t < s.start + s.n) return;
-    }
-    uint4* to = reinterpret_cast<uint4*>(out + static_cast<int64_t>(t) * a.hq * kHeadDim);
-    for (int i = 0; i < a.hq * kHeadDim / 8; ++i) to[i] = make_uint4(0, 0, 0, 0);
+    zero_row(out, a, (blockIdx.x - blocks * per_tile) * kJoinThreads + threadIdx.x);
     return;
   }
   const int first = blockIdx.x / per_tile;
   const Split split = a.splits[first];
   const int r = (blockIdx.x - first * per_tile) * kRows + warp / WARPS, w0 = warp % WARPS;
-  if (r >= split.rows && (WARPS == 1 || kRows == 1 || (r - warp / WARPS) >= split.rows)) return;
+  if (r - warp / WARPS >= split.rows) return;  // (the whole block)
   const bool there = r < split.rows;
   const int row = split.first + r, last = there ? split.last : -1;
   float mx = -INFINITY, sum = 0.f;
@@ -380,7 +386,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(T* __restrict
       if (x > last) continue;
       const int64_t slot = a.slot(x, first);
       st[u] = a.part_stats[slot + r];
-      part[u] = *reinterpret_cast<const float4*>(a.parts + slot * kHeadDim + r * a.part_row + lane * a.part_dims);
+      part[u] = *reinterpret_cast<const float4*>(a.parts + (slot + r) * kHeadDim + 4 * lane);
     }
     const float to_max = fmaxf(fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)), mx);
     const float base = to_max == -INFINITY ? 0.f : to_max, old = ex2_approx(mx - base);
@@ -394,7 +400,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(T* __restrict
       v.x += f * part[u].x, v.y += f * part[u].y, v.z += f * part[u].z, v.w += f * part[u].w;
     }
   }
-  if constexpr (WARPS > 1) {
+  {
     const int x = warp / WARPS;
     sums[x][w0][lane] = v;
     if (lane == 0) stats[x][w0] = make_float2(mx, sum);
@@ -418,6 +424,47 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(T* __restrict
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* to = out + (static_cast<int64_t>(split.start + row / a.group) * a.hq + split.head + row % a.group) * kHeadDim + 4 * lane;
   *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+}
+
+// Tiles of 256 rows, whose parts lie four dims of all rows after the next four: a warp takes eight rows, a lane one of them
+// and every fourth quadruple of dims, so that a part's eight loads a lane are on their way together.
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) attend_join_rows_kernel(T* __restrict__ out, const __grid_constant__ AttendArgs a,
+                                                                        int blocks, int per_tile) {
+  if (static_cast<int>(blockIdx.x) >= blocks * per_tile) {
+    zero_row(out, a, (blockIdx.x - blocks * per_tile) * kJoinThreads + threadIdx.x);
+    return;
+  }
+  const int first = blockIdx.x / per_tile, lane = threadIdx.x & 31;
+  const Split split = a.splits[first];
+  const int r = (blockIdx.x - first * per_tile) * (kJoinThreads / 4) + (threadIdx.x >> 5) * 8 + (lane & 7), d = lane >> 3;
+  if (r >= split.rows) return;
+  float mx = -INFINITY;
+  for (int x = first; x <= split.last; ++x) mx = fmaxf(mx, a.part_stats[a.slot(x, first) + r].x);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f;
+  float4 v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int x = first; x <= split.last; ++x) {
+    const int64_t slot = a.slot(x, first);
+    const float4* from = reinterpret_cast<const float4*>(a.parts + slot * kHeadDim) + r;
+    float4 part[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[i] = from[(d + 4 * i) * kRowsTile];
+    const float2 st = a.part_stats[slot + r];
+    const float f = ex2_approx(st.x - base);
+    sum += f * st.y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i].x += f * part[i].x, v[i].y += f * part[i].y, v[i].z += f * part[i].z, v[i].w += f * part[i].w;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int row = split.first + r;
+  T* to = out + (static_cast<int64_t>(split.start + row / a.group) * a.hq + split.head + row % a.group) * kHeadDim + 4 * d;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    *reinterpret_cast<uint2*>(to + 16 * i) = make_uint2(pack2<T>(v[i].x * inv, v[i].y * inv), pack2<T>(v[i].z * inv, v[i].w * inv));
 }
 
 CUtensorMap pool_map(const at::Tensor& pool, int box_rows) {
@@ -447,8 +494,7 @@ void launch_attend_join(const AttendArgs& a, at::Tensor& out, int blocks) {
       const unsigned grid = static_cast<unsigned>(blocks * per_tile + (a.batch.rows + kJoinThreads - 1) / kJoinThreads);
       kern<<<grid, kJoinThreads, 0, stream()>>>(static_cast<T*>(out.data_ptr()), a, blocks, per_tile);
     };
-    // tiles of many rows have few parts each, unless there are few tiles; those of a step may have one for every block
-    if (a.slot_rows > kTileRows) go(attend_join_kernel<T, 1>, kJoinThreads / 32);
+    if (a.slot_rows > kTileRows) go(attend_join_rows_kernel<T>, kJoinThreads / 4);
     else go(attend_join_kernel<T, 4>, kJoinThreads / 32 / 4);
   };
   if (out.scalar_type() == at::kHalf) launch(static_cast<__half*>(nullptr));
@@ -495,8 +541,6 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& keys, const at
   a.tile_rows = many ? kRowsTile / a.group * a.group : kTileRows;
   a.slot_rows = many ? kRowsTile : kTileRows;
   a.least = many ? 2 : 1;  // (a tile's end costs that kernel as much as some units)
-  a.part_row = many ? 4 : kHeadDim;
-  a.part_dims = many ? 4 * kRowsTile : 4;
   const auto f32 = q.options().dtype(at::kFloat);
   // parts, their statistics and the splits, in one allocation
   const int64_t slots = 2 * static_cast<int64_t>(blocks) * a.slot_rows;
